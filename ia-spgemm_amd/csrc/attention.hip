@@ -1,0 +1,292 @@
+// attention.hip — block-sparse attention: entry points, argument checks and
+// launches (ias_block_* of include/ias.h).  The reference has no counterpart.
+#include "ias.h"
+#include "ias_internal.hpp"
+#include "attention_kernels.hpp"
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+namespace ias {
+namespace {
+
+#define HIPC(x)                                                                   \
+    do {                                                                          \
+        hipError_t _e = (x);                                                      \
+        if (_e != hipSuccess) {                                                   \
+            set_last_error("%s failed: %s", #x, hipGetErrorString(_e));           \
+            return _e == hipErrorOutOfMemory ? IAS_ERROR_OUT_OF_MEMORY : IAS_ERROR_DEVICE; \
+        }                                                                         \
+    } while (0)
+
+// Makes `device` current for the call and puts the caller's back.
+struct OnDevice {
+    int before = -1;
+    hipError_t to(int device) {
+        hipError_t e = hipGetDevice(&before);
+        if (e == hipSuccess && before != device) e = hipSetDevice(device);
+        else if (e == hipSuccess) before = -1;
+        return e;
+    }
+    ~OnDevice() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+#define REFUSE(status, ...)          \
+    do {                             \
+        set_last_error(__VA_ARGS__); \
+        return status;               \
+    } while (0)
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+ias_status check_attention(const ias_attention *a, bool pattern) {
+    if (!a) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "no ias_attention");
+    if (a->dtype != IAS_DTYPE_BF16 && a->dtype != IAS_DTYPE_F16)
+        REFUSE(IAS_ERROR_UNSUPPORTED, "dtype %d: bf16 and f16 are supported", a->dtype);
+    if (a->device < 0) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "device %d", a->device);
+    if (a->batch < 0 || a->q_len < 0 || a->k_len < 0 || a->batch > INT32_MAX)
+        REFUSE(IAS_ERROR_INVALID_ARGUMENT, "batch %lld, q_len %lld, k_len %lld", (long long)a->batch,
+               (long long)a->q_len, (long long)a->k_len);
+    if (a->q_heads < 1 || a->k_heads < 1 || a->q_heads % a->k_heads)
+        REFUSE(IAS_ERROR_DIMENSION_MISMATCH, "q_heads %d is not a multiple of k_heads %d", a->q_heads, a->k_heads);
+    if (a->q_heads / a->k_heads > 64)
+        REFUSE(IAS_ERROR_UNSUPPORTED, "%d query heads for a key head: at most 64", a->q_heads / a->k_heads);
+    if (a->head_dim < 8 || a->head_dim > 128 || a->head_dim % 8)
+        REFUSE(IAS_ERROR_UNSUPPORTED, "head_dim %d: a multiple of 8 up to 128", a->head_dim);
+    if (a->block < 64 || a->block > 1024 || a->block % 64)
+        REFUSE(IAS_ERROR_UNSUPPORTED, "block %d: a multiple of 64 up to 1024", a->block);
+    if (pattern && (a->keep < 1 || a->keep > 256)) REFUSE(IAS_ERROR_UNSUPPORTED, "keep %d: 1 to 256", a->keep);
+    if (ceil_div(a->k_len, a->block) > 16384)
+        REFUSE(IAS_ERROR_UNSUPPORTED, "%lld blocks of keys: at most 16384", (long long)ceil_div(a->k_len, a->block));
+    if (a->q_len > (1 << 24)) REFUSE(IAS_ERROR_UNSUPPORTED, "q_len %lld: at most 2^24", (long long)a->q_len);
+    if (!std::isfinite(a->scale)) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "scale is not finite");
+    if (a->table) {
+        if (a->num_buckets < 1 || a->num_buckets > 64)
+            REFUSE(IAS_ERROR_UNSUPPORTED, "%d buckets: 1 to 64", a->num_buckets);
+        if (a->num_buckets > 1 && !a->edges) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "table without edges");
+    }
+    // workgroups of a launch and the products the kernels form of these
+    if (a->batch * (int64_t)a->q_heads > INT32_MAX / std::max<int64_t>(1, a->q_len) ||
+        a->batch * (int64_t)a->k_heads > INT32_MAX / std::max<int64_t>(1, a->k_len))
+        REFUSE(IAS_ERROR_OVERFLOW, "batch x heads x length beyond 2^31 rows");
+    return IAS_SUCCESS;
+}
+
+ias_status check_heads(const ias_heads *h, const char *name, int64_t batch, int64_t n, int64_t heads) {
+    if (!h) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "no %s", name);
+    if (batch == 0 || n == 0) return IAS_SUCCESS;
+    if (!h->data) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "%s: no data", name);
+    if (((uintptr_t)h->data & 15) || (batch > 1 && h->batch % 8) || (n > 1 && h->token % 8) || (heads > 1 && h->head % 8))
+        REFUSE(IAS_ERROR_UNSUPPORTED, "%s: data has to be 16-byte aligned and its strides multiples of 8", name);
+    return IAS_SUCCESS;
+}
+
+dev::AttnShape shape_of(const ias_attention *a) {
+    dev::AttnShape s{};
+    s.q_len = a->q_len; s.k_len = a->k_len;
+    s.batch = (int32_t)a->batch; s.q_heads = a->q_heads; s.k_heads = a->k_heads;
+    s.group = a->q_heads / a->k_heads;
+    s.dim = a->head_dim; s.block = a->block; s.keep = a->keep; s.causal = a->causal != 0;
+    s.nblocks = (int32_t)ceil_div(a->k_len, a->block);
+    s.scale = a->scale;
+    s.q_lens = a->q_lens; s.k_lens = a->k_lens;
+    s.table = static_cast<const uint16_t *>(a->table);
+    s.num_buckets = a->table ? a->num_buckets : 0;
+    return s;
+}
+dev::Side side(const ias_heads *h) { return {static_cast<const uint16_t *>(h->data), h->batch, h->token, h->head}; }
+dev::SideOut side_out(const ias_heads *h) { return {static_cast<uint16_t *>(h->data), h->batch, h->token, h->head}; }
+
+// Parts of a workspace, each on a boundary of 256 bytes.
+struct Space {
+    int64_t used = 0;
+    char *base = nullptr;
+    template <class T> T *part(int64_t count) {
+        T *p = base ? reinterpret_cast<T *>(base + used) : nullptr;
+        used += (count * (int64_t)sizeof(T) + 255) / 256 * 256;
+        return p;
+    }
+};
+
+int64_t map_size(const ias_attention *a) { return 2 * a->k_len + a->q_len; }
+
+ias_status launched() {
+    HIPC(hipGetLastError());
+    return IAS_SUCCESS;
+}
+
+ias_status bucket_map(const ias_attention *a, dev::AttnShape &s, uint8_t *map) {
+    const int64_t n = map_size(a);
+    dev::k_bucket_map<<<dim3((unsigned)ceil_div(n, 256)), 256, 0, (hipStream_t)a->stream>>>(a->k_len, n, a->num_buckets, a->edges, map);
+    s.map = map;
+    return launched();
+}
+
+struct Forward {
+    uint8_t *map;
+    explicit Forward(const ias_attention *a, Space &w) { map = a->table ? w.part<uint8_t>(map_size(a)) : nullptr; }
+};
+struct Backward {
+    uint8_t *map;
+    float *delta, *sums;
+    explicit Backward(const ias_attention *a, Space &w) {
+        map = a->table ? w.part<uint8_t>(map_size(a)) : nullptr;
+        delta = w.part<float>(a->batch * a->q_heads * a->q_len);
+        sums = a->table ? w.part<float>(a->batch * a->q_heads * a->q_len * a->num_buckets) : nullptr;
+    }
+};
+
+ias_status check_workspace(const void *p, int64_t have, int64_t need) {
+    if (need == 0) return IAS_SUCCESS;
+    if (!p || have < need)
+        REFUSE(IAS_ERROR_INSUFFICIENT_CAPACITY, "workspace of %lld bytes: %lld are needed", (long long)(p ? have : 0), (long long)need);
+    if ((uintptr_t)p & 255) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "the workspace has to be aligned to 256 bytes");
+    return IAS_SUCCESS;
+}
+
+template <class T>
+ias_status attend(const ias_attention *a, const ias_heads *q, const ias_heads *k, const ias_heads *v,
+                  const int32_t *blocks, const ias_heads *out, float *lse, const Forward &f) {
+    dev::AttnShape s = shape_of(a);
+    if (a->table) IAS_TRY(bucket_map(a, s, f.map));
+    const int64_t rows = a->batch * a->q_heads * a->q_len;
+    dev::k_attend_plain<T><<<dim3((unsigned)rows), 64, 0, (hipStream_t)a->stream>>>(s, side(q), side(k), side(v), blocks, side_out(out), lse);
+    return launched();
+}
+
+template <class T>
+ias_status gradients(const ias_attention *a, const ias_heads *dout, const ias_heads *q, const ias_heads *k,
+                     const ias_heads *v, const ias_heads *out, const float *lse, const int32_t *blocks,
+                     const ias_heads *dq, const ias_heads *dk, const ias_heads *dv, void *dtable, const Backward &w) {
+    dev::AttnShape s = shape_of(a);
+    hipStream_t st = (hipStream_t)a->stream;
+    if (a->table) IAS_TRY(bucket_map(a, s, w.map));
+    const int64_t rows = a->batch * a->q_heads * a->q_len, keys = a->batch * a->k_heads * a->k_len;
+    if (rows) {
+        dev::k_grad_q_plain<T><<<dim3((unsigned)rows), 64, 0, st>>>(s, side(dout), side(q), side(k), side(v), side(out), lse, blocks,
+                                                                    side_out(dq), w.delta, dtable ? w.sums : nullptr);
+        IAS_TRY(launched());
+    }
+    if (keys) {
+        dev::k_grad_kv_plain<T><<<dim3((unsigned)keys), 64, 0, st>>>(s, side(dout), side(q), side(k), side(v), lse, w.delta, blocks,
+                                                                     side_out(dk), side_out(dv));
+        IAS_TRY(launched());
+    }
+    if (a->table && dtable) {
+        dev::k_grad_table<T><<<dim3((unsigned)(a->q_heads * a->num_buckets)), 256, 0, st>>>(
+            a->batch * a->q_len, a->q_heads, a->num_buckets, w.sums, static_cast<uint16_t *>(dtable));
+        IAS_TRY(launched());
+    }
+    return IAS_SUCCESS;
+}
+
+}  // namespace
+}  // namespace ias
+
+using namespace ias;
+
+extern "C" ias_status ias_block_summary(const ias_attention *a, const ias_heads *k, int64_t fresh, void *summary) {
+    IAS_TRY(check_attention(a, false));
+    IAS_TRY(check_heads(k, "k", a->batch, a->k_len, a->k_heads));
+    if (fresh < 0) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "fresh %lld", (long long)fresh);
+    if (a->batch == 0 || a->k_len == 0) return IAS_SUCCESS;
+    if (!summary) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "no summary");
+    OnDevice on;
+    HIPC(on.to(a->device));
+    const dev::AttnShape s = shape_of(a);
+    const int32_t per = fresh > 0 ? (int32_t)std::min<int64_t>(s.nblocks, (std::min(fresh, a->k_len) + a->block - 2) / a->block + 1) : s.nblocks;
+    const dim3 grid((unsigned)(a->batch * a->k_heads * per));
+    uint16_t *o = static_cast<uint16_t *>(summary);
+    if (a->dtype == IAS_DTYPE_BF16) dev::k_block_summary<dev::Bf16><<<grid, 256, 0, (hipStream_t)a->stream>>>(s, side(k), fresh, per, o);
+    else dev::k_block_summary<dev::Fp16><<<grid, 256, 0, (hipStream_t)a->stream>>>(s, side(k), fresh, per, o);
+    return launched();
+}
+
+extern "C" ias_status ias_block_select(const ias_attention *a, const ias_heads *q, const void *summary, int32_t first,
+                                       int32_t local, int32_t *blocks) {
+    IAS_TRY(check_attention(a, true));
+    IAS_TRY(check_heads(q, "q", a->batch, a->q_len, a->q_heads));
+    if (first < 0 || local < 0 || (int64_t)first + local > a->keep)
+        REFUSE(IAS_ERROR_INVALID_ARGUMENT, "first %d + local %d of keep %d", first, local, a->keep);
+    if (local > 0 && !a->causal) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "local blocks are those of a causal call");
+    if (a->batch == 0 || a->q_len == 0) return IAS_SUCCESS;
+    if ((!summary && a->k_len > 0) || !blocks) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "no summary or blocks");
+    OnDevice on;
+    HIPC(on.to(a->device));
+    const dev::AttnShape s = shape_of(a);
+    const dim3 grid((unsigned)(a->batch * a->k_heads * a->q_len));
+    const size_t lds = 8 * (size_t)s.nblocks + 4 * (size_t)((s.nblocks + 31) / 32);
+    const uint16_t *m = static_cast<const uint16_t *>(summary);
+    if (a->dtype == IAS_DTYPE_BF16) {
+        HIPC(hipFuncSetAttribute((const void *)dev::k_block_select<dev::Bf16>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        dev::k_block_select<dev::Bf16><<<grid, 64, lds, (hipStream_t)a->stream>>>(s, side(q), m, first, local, blocks);
+    } else {
+        HIPC(hipFuncSetAttribute((const void *)dev::k_block_select<dev::Fp16>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        dev::k_block_select<dev::Fp16><<<grid, 64, lds, (hipStream_t)a->stream>>>(s, side(q), m, first, local, blocks);
+    }
+    return launched();
+}
+
+extern "C" ias_status ias_block_attention_workspace(const ias_attention *a, int64_t *forward, int64_t *backward) {
+    IAS_TRY(check_attention(a, true));
+    Space f, b;
+    (void)Forward(a, f);
+    (void)Backward(a, b);
+    if (forward) *forward = f.used;
+    if (backward) *backward = b.used;
+    return IAS_SUCCESS;
+}
+
+extern "C" ias_status ias_block_attention(const ias_attention *a, const ias_heads *q, const ias_heads *k,
+                                          const ias_heads *v, const int32_t *blocks, const ias_heads *out,
+                                          float *lse, void *workspace, int64_t workspace_bytes) {
+    IAS_TRY(check_attention(a, true));
+    IAS_TRY(check_heads(q, "q", a->batch, a->q_len, a->q_heads));
+    IAS_TRY(check_heads(k, "k", a->batch, a->k_len, a->k_heads));
+    IAS_TRY(check_heads(v, "v", a->batch, a->k_len, a->k_heads));
+    IAS_TRY(check_heads(out, "out", a->batch, a->q_len, a->q_heads));
+    if (a->batch == 0 || a->q_len == 0) return IAS_SUCCESS;
+    if (!blocks) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "no blocks");
+    Space need;
+    (void)Forward(a, need);
+    IAS_TRY(check_workspace(workspace, workspace_bytes, need.used));
+    Space w;
+    w.base = static_cast<char *>(workspace);
+    const Forward f(a, w);
+    OnDevice on;
+    HIPC(on.to(a->device));
+    return a->dtype == IAS_DTYPE_BF16 ? attend<dev::Bf16>(a, q, k, v, blocks, out, lse, f)
+                                      : attend<dev::Fp16>(a, q, k, v, blocks, out, lse, f);
+}
+
+extern "C" ias_status ias_block_attention_grad(const ias_attention *a, const ias_heads *dout, const ias_heads *q,
+                                               const ias_heads *k, const ias_heads *v, const ias_heads *out,
+                                               const float *lse, const int32_t *blocks, const ias_heads *dq,
+                                               const ias_heads *dk, const ias_heads *dv, void *dtable, void *workspace,
+                                               int64_t workspace_bytes) {
+    IAS_TRY(check_attention(a, true));
+    IAS_TRY(check_heads(dout, "dout", a->batch, a->q_len, a->q_heads));
+    IAS_TRY(check_heads(q, "q", a->batch, a->q_len, a->q_heads));
+    IAS_TRY(check_heads(k, "k", a->batch, a->k_len, a->k_heads));
+    IAS_TRY(check_heads(v, "v", a->batch, a->k_len, a->k_heads));
+    IAS_TRY(check_heads(out, "out", a->batch, a->q_len, a->q_heads));
+    IAS_TRY(check_heads(dq, "dq", a->batch, a->q_len, a->q_heads));
+    IAS_TRY(check_heads(dk, "dk", a->batch, a->k_len, a->k_heads));
+    IAS_TRY(check_heads(dv, "dv", a->batch, a->k_len, a->k_heads));
+    if (dtable && !a->table) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "dtable without a table");
+    if (a->batch > 0 && a->q_len > 0 && (!blocks || !lse)) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "no blocks or lse");
+    Space need;
+    (void)Backward(a, need);
+    IAS_TRY(check_workspace(workspace, workspace_bytes, need.used));
+    Space w;
+    w.base = static_cast<char *>(workspace);
+    const Backward f(a, w);
+    OnDevice on;
+    HIPC(on.to(a->device));
+    return a->dtype == IAS_DTYPE_BF16 ? gradients<dev::Bf16>(a, dout, q, k, v, out, lse, blocks, dq, dk, dv, dtable, f)
+                                      : gradients<dev::Fp16>(a, dout, q, k, v, out, lse, blocks, dq, dk, dv, dtable, f);
+}

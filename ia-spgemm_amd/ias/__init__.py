@@ -91,6 +91,19 @@ class MtxInfo(C.Structure):
                 ("nnz_file", C.c_int64)]
 
 
+class Heads(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("batch", C.c_int64), ("token", C.c_int64), ("head", C.c_int64)]
+
+
+class Attention(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("device", C.c_int32), ("stream", C.c_void_p),
+                ("batch", C.c_int64), ("q_len", C.c_int64), ("k_len", C.c_int64),
+                ("q_heads", C.c_int32), ("k_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("block", C.c_int32), ("keep", C.c_int32), ("causal", C.c_int32),
+                ("scale", C.c_float), ("num_buckets", C.c_int32),
+                ("q_lens", C.c_void_p), ("k_lens", C.c_void_p), ("table", C.c_void_p), ("edges", C.c_void_p)]
+
+
 # every symbol include/ias.h declares (checked by tests/test_abi.py)
 EXPORTS = [
     "ias_abi_version", "ias_status_string", "ias_last_diag", "ias_device_count", "ias_opts_default",
@@ -112,6 +125,8 @@ EXPORTS = [
     "ias_mkl_available", "ias_mkl_sp2m",
     "ias_features", "ias_density_image", "ias_matnet_load", "ias_matnet_free", "ias_matnet_shape",
     "ias_matnet_predict",
+    "ias_block_summary", "ias_block_select", "ias_block_attention_workspace", "ias_block_attention",
+    "ias_block_attention_grad", "ias_rel_bias", "ias_rel_bias_grad_workspace", "ias_rel_bias_grad",
 ]
 
 
@@ -192,6 +207,19 @@ def _load():
         "ias_matnet_free": (C.c_int, [C.c_void_p]),
         "ias_matnet_shape": (C.c_int, [C.c_void_p, i32p, i32p]),
         "ias_matnet_predict": (C.c_int, [C.c_void_p, i64p, i64p, f64p, C.POINTER(C.c_float), i32p]),
+        "ias_block_summary": (C.c_int, [P(Attention), P(Heads), C.c_int64, C.c_void_p]),
+        "ias_block_select": (C.c_int, [P(Attention), P(Heads), C.c_void_p, C.c_int32, C.c_int32, C.c_void_p]),
+        "ias_block_attention_workspace": (C.c_int, [P(Attention), i64p, i64p]),
+        "ias_block_attention": (C.c_int, [P(Attention), P(Heads), P(Heads), P(Heads), C.c_void_p, P(Heads),
+                                          C.c_void_p, C.c_void_p, C.c_int64]),
+        "ias_block_attention_grad": (C.c_int, [P(Attention)] + [P(Heads)] * 5 + [C.c_void_p] * 2 + [P(Heads)] * 3
+                                     + [C.c_void_p, C.c_void_p, C.c_int64]),
+        "ias_rel_bias": (C.c_int, [C.c_int32, C.c_int32, C.c_int64, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p,
+                                   C.c_void_p, C.c_int32, C.c_void_p]),
+        "ias_rel_bias_grad_workspace": (C.c_int, [C.c_int64, C.c_int32, C.c_int64, C.c_int64, C.c_int32, i64p]),
+        "ias_rel_bias_grad": (C.c_int, [C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_int64, C.c_int32,
+                                        C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p,
+                                        C.c_void_p, C.c_int64, C.c_int32, C.c_void_p]),
     }
     for name, (res, args) in sig.items():
         f = getattr(lib, name)

@@ -1,0 +1,213 @@
+"""Block-sparse attention and the relative position bias on torch tensors
+(the ias_block_* and ias_rel_bias* entry points of include/ias.h).
+
+q is (batch, q_len, q_heads, dim), k and v are (batch, k_len, k_heads, dim),
+bf16 or fp16 on one HIP device; any strides whose last is 1 and whose others
+are multiples of 8.  Calls enqueue work on the current stream of the tensors'
+device and return without waiting; outputs and workspaces come from torch's
+allocator on that stream, so the calls can be captured into a graph.
+
+    m      = block_summary(k)
+    blocks = block_select(q, m, keep=16, k_len=k.shape[1])
+    out, lse = block_attention(q, k, v, blocks)
+    dq, dk, dv, _ = block_attention_grad(dout, q, k, v, out, lse, blocks)
+
+There is no autograd function here: the gradient is a call of its own.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple
+
+import torch
+
+from . import Attention, Heads, check, lib
+
+_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _device(t: torch.Tensor) -> int:
+    if not t.is_cuda:
+        raise ValueError("ias.attention takes tensors of a HIP device")
+    return t.device.index
+
+
+def _stream(t: torch.Tensor) -> int:
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _heads(t: torch.Tensor, shape, dtype, device, name: str) -> Heads:
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} is {tuple(t.shape)}, not {tuple(shape)}")
+    if t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} is {t.dtype} on {t.device}, not {dtype} on {device}")
+    if t.stride(3) != 1 and t.numel():
+        raise ValueError(f"{name}: the last dimension has to be contiguous")
+    return Heads(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+
+
+def _plain(t: Optional[torch.Tensor], shape, dtype, device, name: str) -> Optional[int]:
+    """Address of a contiguous tensor of that shape and type."""
+    if t is None:
+        return None
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} has to be a contiguous {dtype} {tuple(shape)} on {device}, not {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _attention(like: torch.Tensor, batch, q_len, k_len, q_heads, k_heads, dim, block, keep, causal, scale, q_lens,
+               k_lens, table=None, edges=None) -> Attention:
+    _device(like)
+    if like.dtype not in _DTYPE:
+        raise ValueError(f"{like.dtype} is not supported")
+    a = Attention()
+    a.dtype, a.device, a.stream = _DTYPE[like.dtype], _device(like), _stream(like)
+    a.batch, a.q_len, a.k_len, a.q_heads, a.k_heads, a.head_dim = batch, q_len, k_len, q_heads, k_heads, dim
+    a.block, a.keep, a.causal = block, keep, int(bool(causal))
+    a.scale = float(scale) if scale is not None else (dim ** -0.5 if dim else 1.0)
+    a.q_lens = _plain(q_lens, (batch,), torch.int32, like.device, "q_lens")
+    a.k_lens = _plain(k_lens, (batch,), torch.int32, like.device, "k_lens")
+    if (table is None) != (edges is None):
+        raise ValueError("table and edges go together")
+    if table is not None:
+        a.num_buckets = table.shape[0]
+        a.table = _plain(table, (edges.numel() + 1, q_heads), like.dtype, like.device, "table")
+        a.edges = _plain(edges, (table.shape[0] - 1,), torch.int32, like.device, "edges")
+        if table.shape[0] == 1:
+            a.edges = a.table  # no edge to read
+    return a
+
+
+def _out(out, shape, like, lens, name="out"):
+    """`out`, or a new tensor: zeros where rows behind a sequence's end stay unwritten."""
+    if out is not None:
+        return out
+    return (torch.empty if lens is None else torch.zeros)(shape, dtype=like.dtype, device=like.device)
+
+
+def block_summary(k: torch.Tensor, *, block: int = 64, k_lens: Optional[torch.Tensor] = None, fresh: int = 0,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """(batch, k_heads, blocks, dim): the mean of each block of keys.  With
+    `fresh`, `out` is the summary of a cache that has grown by that many tokens
+    since: only the blocks that hold them are written."""
+    b, n, h, d = k.shape
+    if fresh and out is None:
+        raise ValueError("fresh brings an existing summary up to date: pass it as out")
+    a = _attention(k, b, 0, n, h, h, d, block, 1, True, None, None, k_lens)
+    shape = (b, h, -(-n // block) if block > 0 else 0, d)
+    if out is None:
+        out = torch.empty(shape, dtype=k.dtype, device=k.device)
+    check(lib.ias_block_summary(C.byref(a), C.byref(_heads(k, k.shape, k.dtype, k.device, "k")), fresh,
+                                _plain(out, shape, k.dtype, k.device, "out")), "ias_block_summary")
+    return out
+
+
+def block_select(q: torch.Tensor, summary: torch.Tensor, keep: int, *, k_len: int, block: int = 64, causal: bool = True,
+                 first: int = 1, local: int = 1, q_lens: Optional[torch.Tensor] = None,
+                 k_lens: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """(batch, k_heads, q_len, keep) int32: the blocks that each query reads,
+    ascending, -1 behind.  `first` blocks and (causal) the `local` last ones
+    always, then those whose summary scores highest."""
+    b, n, hq, d = q.shape
+    a = _attention(q, b, n, k_len, hq, summary.shape[1], d, block, keep, causal, None, q_lens, k_lens)
+    m = -(-k_len // block) if block > 0 else 0
+    if out is None:
+        shape = (b, summary.shape[1], n, max(keep, 0))
+        out = torch.empty(shape, dtype=torch.int32, device=q.device) if q_lens is None else \
+            torch.full(shape, -1, dtype=torch.int32, device=q.device)
+    check(lib.ias_block_select(C.byref(a), C.byref(_heads(q, q.shape, q.dtype, q.device, "q")),
+                               _plain(summary, (b, summary.shape[1], m, d), q.dtype, q.device, "summary"), first,
+                               local if causal else 0,
+                               _plain(out, (b, summary.shape[1], n, keep), torch.int32, q.device, "out")),
+          "ias_block_select")
+    return out
+
+
+def _shapes(q, k, blocks, block, causal, scale, q_lens, k_lens, table, edges):
+    b, n, hq, d = q.shape
+    nk, hkv = k.shape[1], k.shape[2]
+    a = _attention(q, b, n, nk, hq, hkv, d, block, blocks.shape[-1], causal, scale, q_lens, k_lens, table, edges)
+    return a, (b, n, hq, d), (b, nk, hkv, d), _plain(blocks, (b, hkv, n, blocks.shape[-1]), torch.int32, q.device, "blocks")
+
+
+def _workspace(a: Attention, like: torch.Tensor, backward: bool):
+    f, g = C.c_int64(0), C.c_int64(0)
+    check(lib.ias_block_attention_workspace(C.byref(a), C.byref(f), C.byref(g)), "ias_block_attention_workspace")
+    n = g.value if backward else f.value
+    return torch.empty(n, dtype=torch.uint8, device=like.device), n
+
+
+def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, blocks: torch.Tensor, *, block: int = 64,
+                    causal: bool = True, scale: Optional[float] = None, q_lens: Optional[torch.Tensor] = None,
+                    k_lens: Optional[torch.Tensor] = None, table: Optional[torch.Tensor] = None,
+                    edges: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None
+                    ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(out, lse): softmax(scale q k^T + bias) v over the pattern, and the
+    logarithm of each row's sum, (batch, q_heads, q_len) in fp32.  Rows behind
+    q_lens are 0 / -inf in new tensors and left alone in a given `out`."""
+    a, qs, ks, pb = _shapes(q, k, blocks, block, causal, scale, q_lens, k_lens, table, edges)
+    out = _out(out, qs, q, q_lens)
+    lse = torch.empty((qs[0], qs[2], qs[1]), dtype=torch.float32, device=q.device) if q_lens is None else \
+        torch.full((qs[0], qs[2], qs[1]), float("-inf"), dtype=torch.float32, device=q.device)
+    ws, n = _workspace(a, q, False)
+    h = [_heads(t, s, q.dtype, q.device, x) for t, s, x in ((q, qs, "q"), (k, ks, "k"), (v, ks, "v"), (out, qs, "out"))]
+    check(lib.ias_block_attention(C.byref(a), C.byref(h[0]), C.byref(h[1]), C.byref(h[2]), pb, C.byref(h[3]),
+                                  lse.data_ptr(), ws.data_ptr(), n), "ias_block_attention")
+    return out, lse
+
+
+def block_attention_grad(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                         lse: torch.Tensor, blocks: torch.Tensor, *, block: int = 64, causal: bool = True,
+                         scale: Optional[float] = None, q_lens: Optional[torch.Tensor] = None,
+                         k_lens: Optional[torch.Tensor] = None, table: Optional[torch.Tensor] = None,
+                         edges: Optional[torch.Tensor] = None):
+    """(dq, dk, dv, dtable) from the forward call's arguments and results;
+    dtable is None without a table."""
+    a, qs, ks, pb = _shapes(q, k, blocks, block, causal, scale, q_lens, k_lens, table, edges)
+    dq, dk, dv = _out(None, qs, q, q_lens), _out(None, ks, q, k_lens), _out(None, ks, q, k_lens)
+    dtable = None if table is None else torch.empty_like(table)
+    pl = _plain(lse, (qs[0], qs[2], qs[1]), torch.float32, q.device, "lse")
+    ws, n = _workspace(a, q, True)
+    h = [_heads(t, s, q.dtype, q.device, x) for t, s, x in (
+        (dout, qs, "dout"), (q, qs, "q"), (k, ks, "k"), (v, ks, "v"), (out, qs, "out"), (dq, qs, "dq"), (dk, ks, "dk"),
+        (dv, ks, "dv"))]
+    p = [C.byref(x) for x in h]
+    check(lib.ias_block_attention_grad(C.byref(a), p[0], p[1], p[2], p[3], p[4], pl, pb, p[5], p[6], p[7],
+                                       None if dtable is None else dtable.data_ptr(), ws.data_ptr(), n),
+          "ias_block_attention_grad")
+    return dq, dk, dv, dtable
+
+
+def rel_bias(table: torch.Tensor, edges: torch.Tensor, q_len: int, k_len: int) -> torch.Tensor:
+    """(heads, q_len, k_len): table[bucket(j - i - (k_len - q_len)), h], where
+    bucket(d) is how many of the ascending `edges` are <= d."""
+    device = _device(table)
+    if table.dtype not in _DTYPE:
+        raise ValueError(f"{table.dtype} is not supported")
+    pt = _plain(table, (edges.numel() + 1, table.shape[1]), table.dtype, table.device, "table")
+    pe = _plain(edges, (edges.numel(),), torch.int32, table.device, "edges") or pt
+    out = torch.empty((table.shape[1], q_len, k_len), dtype=table.dtype, device=table.device)
+    check(lib.ias_rel_bias(_DTYPE[table.dtype], table.shape[1], q_len, k_len, table.shape[0], pt, pe, out.data_ptr(),
+                           device, _stream(table)), "ias_rel_bias")
+    return out
+
+
+def rel_bias_grad(grad: torch.Tensor, edges: torch.Tensor) -> torch.Tensor:
+    """(buckets, heads) of grad's type: the sum of grad (batch, heads, q_len,
+    k_len) over each bucket of each head."""
+    device = _device(grad)
+    if grad.dtype not in _DTYPE or grad.dim() != 4:
+        raise ValueError(f"grad: {grad.dtype} {tuple(grad.shape)} is not supported")
+    b, h, n, m = grad.shape
+    if grad.numel() and grad.stride(3) != 1:
+        raise ValueError("grad: the last dimension has to be contiguous")
+    pe = _plain(edges, (edges.numel(),), torch.int32, grad.device, "edges")
+    buckets = edges.numel() + 1
+    out = torch.empty((buckets, h), dtype=grad.dtype, device=grad.device)
+    need = C.c_int64(0)
+    check(lib.ias_rel_bias_grad_workspace(b, h, n, m, buckets, C.byref(need)), "ias_rel_bias_grad_workspace")
+    ws = torch.empty(need.value, dtype=torch.uint8, device=grad.device)
+    check(lib.ias_rel_bias_grad(_DTYPE[grad.dtype], b, h, n, m, buckets, grad.data_ptr(), grad.stride(0), grad.stride(1),
+                                grad.stride(2), pe or out.data_ptr(), out.data_ptr(), ws.data_ptr(), need.value, device,
+                                _stream(grad)), "ias_rel_bias_grad")
+    return out

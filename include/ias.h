@@ -36,7 +36,8 @@ extern "C" {
                                3: ias_csr_mul_csr_into (single pass);
                                4: input-aware selector (features, images, MatNet);
                                5: ias_report.stream_launches;
-                               6: ias_last_diag */
+                               6: ias_last_diag;
+                               functions added since change none of the above */
 
 typedef enum ias_status {
     IAS_SUCCESS = 0,
@@ -406,6 +407,110 @@ ias_status ias_dist_allgatherv_csr(ias_dist *dist, const ias_csr *C_local, ias_c
  * device, library-allocated. */
 ias_status ias_dist_csr_mul_csr(ias_dist *dist, const ias_csr *A, const ias_csr *B, ias_csr *C,
                                 int32_t gather, int32_t order, ias_report *report);
+
+/* ---------------------------------------------------------------- block-sparse attention
+ * Products whose pattern is sparse and whose operands are dense: for every
+ * query a few blocks of keys are chosen by a cheap score, and the softmax of
+ * the scores and its product with the values run over those blocks only.  No
+ * reference counterpart (the reference multiplies sparse by sparse).
+ *
+ * All pointers are device memory of `device`; every call only enqueues work on
+ * `stream` (NULL: the device's default stream), allocates nothing, waits for
+ * nothing and may be captured into a HIP graph.  The workspace belongs to the
+ * call until its work is done: two calls that may run at once need two.  The
+ * calling thread's current device is left as it was.
+ *
+ * Shapes: q, out, dout, dq are batch x q_len x q_heads x head_dim, k, v, dk, dv
+ * batch x k_len x k_heads x head_dim (ias_heads: strides of the first three in
+ * elements, the last is contiguous; data 16-byte aligned and the strides
+ * multiples of 8).  Query head h reads key head h / (q_heads / k_heads).  A
+ * sequence's queries are its last tokens: with q_lens / k_lens (int32 per batch
+ * element, NULL: all q_len / k_len; values are clamped to [0, q_len] and
+ * [0, k_len]) query i stands at position i + k_lens[b] - q_lens[b], and causal
+ * lets it read the keys up to that position.  Output rows at or beyond a
+ * sequence's length are not written.  What a padded or masked key, or one of a
+ * block that a query did not choose, holds (infinities and NaN too) does not
+ * reach that query's results.
+ *
+ * Pattern (`blocks`, int32, batch x k_heads x q_len x keep): the blocks of
+ * `block` keys that a query reads, one choice for the query heads of a key
+ * head.  The entries are a set: order is free, a repeated one counts once, and
+ * one outside [0, ceil(k_len / block)) is ignored (-1 marks unused places).
+ *
+ * Relative position bias: scores[i][j] += table[bucket(j - position(i))][head],
+ * bucket(d) = how many of the num_buckets - 1 ascending `edges` are <= d; table
+ * is num_buckets x q_heads of the call's type.  table NULL: none.
+ *
+ * Limits, IAS_ERROR_UNSUPPORTED beyond: dtype bf16 or f16; head_dim a multiple
+ * of 8 up to 128; block a multiple of 64 up to 1024; keep up to 256; at most
+ * 64 query heads for a key head, 16384 blocks, 64 buckets. */
+typedef enum ias_dtype { IAS_DTYPE_F32 = 0, IAS_DTYPE_BF16 = 1, IAS_DTYPE_F16 = 2 } ias_dtype;
+
+typedef struct ias_heads {
+    void *data;
+    int64_t batch, token, head;   /* strides, in elements */
+} ias_heads;
+
+typedef struct ias_attention {
+    int32_t dtype, device;        /* ias_dtype, HIP ordinal */
+    void   *stream;               /* hipStream_t */
+    int64_t batch, q_len, k_len;
+    int32_t q_heads, k_heads, head_dim;
+    int32_t block, keep;          /* keys of a block, places of a pattern row */
+    int32_t causal;
+    float   scale;                /* of q.k */
+    int32_t num_buckets;          /* rows of table (with table only) */
+    const int32_t *q_lens, *k_lens;
+    const void    *table;
+    const int32_t *edges;
+} ias_attention;
+
+/* summary (batch x k_heads x ceil(k_len / block) x head_dim, of the call's
+ * type): the mean of each block's keys below k_lens, summed and divided in 64
+ * bits; 0 for a block without keys.  fresh > 0: only the blocks that hold any
+ * of a sequence's last `fresh` keys are written (a cache that grew by `fresh`
+ * tokens since its last summary), fresh = 0: all.  `keep` is not read. */
+ias_status ias_block_summary(const ias_attention *a, const ias_heads *k, int64_t fresh, void *summary);
+/* blocks: for each query the first `first` of the blocks that it may read, the
+ * last `local` of them (causal only), then those of the highest score, up to
+ * `keep`; ascending, -1 behind.  A block's score is the largest q_h . mean of
+ * the key head's query heads, compared in 64 bits (NaN below everything); of
+ * equal scores the lower block wins.  first + local <= keep. */
+ias_status ias_block_select(const ias_attention *a, const ias_heads *q, const void *summary,
+                            int32_t first, int32_t local, int32_t *blocks);
+/* Bytes of workspace that ias_block_attention (forward) and
+ * ias_block_attention_grad (backward) take for these shapes; either may be NULL. */
+ias_status ias_block_attention_workspace(const ias_attention *a, int64_t *forward, int64_t *backward);
+/* out = softmax(scale q k^T + bias) v over the pattern; lse (f32, batch x
+ * q_heads x q_len, NULL: not wanted) = log of the sum of the exponentials.  A
+ * query that reads nothing: out = 0, lse = -infinity. */
+ias_status ias_block_attention(const ias_attention *a, const ias_heads *q, const ias_heads *k,
+                               const ias_heads *v, const int32_t *blocks, const ias_heads *out,
+                               float *lse, void *workspace, int64_t workspace_bytes);
+/* Gradients of the call above from its out and lse: dq, dk, dv and, where the
+ * call had a table and dtable is not NULL, dtable (as table).  Sums run in a
+ * fixed order: the same inputs give the same bits. */
+ias_status ias_block_attention_grad(const ias_attention *a, const ias_heads *dout, const ias_heads *q,
+                                    const ias_heads *k, const ias_heads *v, const ias_heads *out,
+                                    const float *lse, const int32_t *blocks, const ias_heads *dq,
+                                    const ias_heads *dk, const ias_heads *dv, void *dtable,
+                                    void *workspace, int64_t workspace_bytes);
+
+/* The bias by itself, a matrix of constant diagonals for each head:
+ * out[h][i][j] = table[bucket(j - i - (k_len - q_len))][h] (heads x q_len x
+ * k_len, contiguous; table num_buckets x heads; types f32, bf16, f16; at most
+ * 64 buckets), and its gradient dtable[n][h] = sum of grad[b][h][i][j] over b
+ * and the (i, j) of bucket n, summed in f32 in a fixed order (grad: strides of
+ * the first three in elements, the last is contiguous).  workspace:
+ * ias_rel_bias_grad_workspace bytes. */
+ias_status ias_rel_bias(int32_t dtype, int32_t heads, int64_t q_len, int64_t k_len, int32_t num_buckets,
+                        const void *table, const int32_t *edges, void *out, int32_t device, void *stream);
+ias_status ias_rel_bias_grad_workspace(int64_t batch, int32_t heads, int64_t q_len, int64_t k_len,
+                                       int32_t num_buckets, int64_t *bytes);
+ias_status ias_rel_bias_grad(int32_t dtype, int64_t batch, int32_t heads, int64_t q_len, int64_t k_len,
+                             int32_t num_buckets, const void *grad, int64_t stride_batch,
+                             int64_t stride_head, int64_t stride_row, const int32_t *edges, void *dtable,
+                             void *workspace, int64_t workspace_bytes, int32_t device, void *stream);
 
 /* ---------------------------------------------------------------- synthetic inputs
  * Deterministic host generators (counter-based splitmix64; identical on every

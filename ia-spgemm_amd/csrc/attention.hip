@@ -3,6 +3,7 @@
 #include "ias.h"
 #include "ias_internal.hpp"
 #include "attention_kernels.hpp"
+#include "attention_fwd.hpp"
 
 #include <hip/hip_runtime.h>
 
@@ -112,7 +113,8 @@ struct Space {
     }
 };
 
-int64_t map_size(const ias_attention *a) { return 2 * a->k_len + a->q_len; }
+// every distance from a position to a key, the last block's end included
+int64_t map_size(const ias_attention *a) { return 2 * a->k_len + a->q_len + a->block + 8; }
 
 ias_status launched() {
     HIPC(hipGetLastError());
@@ -126,9 +128,36 @@ ias_status bucket_map(const ias_attention *a, dev::AttnShape &s, uint8_t *map) {
     return launched();
 }
 
+// How k_attend shares out the rows.  16 rows fill one matrix tile, 32 let more
+// queries share a walk and each fragment of K and V feed two tiles; 64 only
+// where one query has that many heads.  Few rows (single tokens) are split along
+// the walk until about every CU has a workgroup, two blocks of keys each at least.
+struct Rows {
+    int mt, dp;
+    dev::AttendPlan plan{};
+    int64_t tiles, part, stat;   // all tiles; floats of the splits' results
+    explicit Rows(const ias_attention *a) {
+        const int group = a->q_heads / a->k_heads;
+        mt = group > 32 ? 4 : group > 16 || a->q_len * group > 16 ? 2 : 1;
+        dp = a->head_dim > 64 ? 128 : 64;
+        plan.nq = (int32_t)std::max<int64_t>(1, std::min<int64_t>({16 * mt / group, 32, a->q_len}));
+        plan.tiles = (int32_t)ceil_div(a->q_len, plan.nq);
+        plan.most = (int32_t)std::max<int64_t>(1, std::min<int64_t>((int64_t)plan.nq * a->keep, ceil_div(a->k_len, a->block)));
+        tiles = a->batch * a->k_heads * plan.tiles;
+        plan.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({ceil_div(512, std::max<int64_t>(1, tiles)), ceil_div(plan.most, 2), 64}));
+        part = plan.splits > 1 ? tiles * plan.splits * 16 * mt * dp : 0;
+        stat = plan.splits > 1 ? tiles * plan.splits * 16 * mt * 2 : 0;
+    }
+};
+
 struct Forward {
     uint8_t *map;
-    explicit Forward(const ias_attention *a, Space &w) { map = a->table ? w.part<uint8_t>(map_size(a)) : nullptr; }
+    Rows rows;
+    explicit Forward(const ias_attention *a, Space &w) : rows(a) {
+        map = a->table ? w.part<uint8_t>(map_size(a)) : nullptr;
+        rows.plan.part = rows.part ? w.part<float>(rows.part) : nullptr;
+        rows.plan.stat = rows.stat ? w.part<float>(rows.stat) : nullptr;
+    }
 };
 struct Backward {
     uint8_t *map;
@@ -148,14 +177,43 @@ ias_status check_workspace(const void *p, int64_t have, int64_t need) {
     return IAS_SUCCESS;
 }
 
+// A launch with `lds` bytes of dynamic LDS; more than 64 KB are asked for.
+template <class K, class... P>
+ias_status launch(K kernel, int64_t grid, int threads, size_t lds, void *stream, P... args) {
+    if (lds > 64 * 1024) HIPC(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    kernel<<<dim3((unsigned)grid), threads, lds, (hipStream_t)stream>>>(args...);
+    return launched();
+}
+
+template <class T, int DP, int MT>
+ias_status attend_rows(const ias_attention *a, const dev::AttnShape &s, const ias_heads *q, const ias_heads *k,
+                       const ias_heads *v, const int32_t *blocks, const ias_heads *out, float *lse, const Rows &r) {
+    const int64_t grid = ceil_div(r.tiles * r.plan.splits, 8) * 8;
+    const size_t lds = dev::attend_lds(DP, MT, s.nblocks, r.plan.most, s.num_buckets * s.group);
+    if (a->table)
+        IAS_TRY(launch(dev::k_attend<T, DP, MT, true>, grid, 256, lds, a->stream, s, r.plan, side(q), side(k), side(v), blocks, side_out(out), lse));
+    else
+        IAS_TRY(launch(dev::k_attend<T, DP, MT, false>, grid, 256, lds, a->stream, s, r.plan, side(q), side(k), side(v), blocks, side_out(out), lse));
+    if (r.plan.splits > 1)
+        IAS_TRY(launch(dev::k_attend_join<T>, r.tiles * r.plan.nq * s.group, 64, 0, a->stream, s, r.plan, DP, 16 * MT,
+                       a->table ? dev::LOG2E : 1.0f, side_out(out), lse));
+    return IAS_SUCCESS;
+}
+
 template <class T>
 ias_status attend(const ias_attention *a, const ias_heads *q, const ias_heads *k, const ias_heads *v,
                   const int32_t *blocks, const ias_heads *out, float *lse, const Forward &f) {
     dev::AttnShape s = shape_of(a);
     if (a->table) IAS_TRY(bucket_map(a, s, f.map));
-    const int64_t rows = a->batch * a->q_heads * a->q_len;
-    dev::k_attend_plain<T><<<dim3((unsigned)rows), 64, 0, (hipStream_t)a->stream>>>(s, side(q), side(k), side(v), blocks, side_out(out), lse);
-    return launched();
+    const Rows &r = f.rows;
+    if (r.dp == 64) {
+        if (r.mt == 1) return attend_rows<T, 64, 1>(a, s, q, k, v, blocks, out, lse, r);
+        if (r.mt == 2) return attend_rows<T, 64, 2>(a, s, q, k, v, blocks, out, lse, r);
+        return attend_rows<T, 64, 4>(a, s, q, k, v, blocks, out, lse, r);
+    }
+    if (r.mt == 1) return attend_rows<T, 128, 1>(a, s, q, k, v, blocks, out, lse, r);
+    if (r.mt == 2) return attend_rows<T, 128, 2>(a, s, q, k, v, blocks, out, lse, r);
+    return attend_rows<T, 128, 4>(a, s, q, k, v, blocks, out, lse, r);
 }
 
 template <class T>

@@ -205,51 +205,6 @@ __device__ inline bool first_entry(const int32_t *row, int t, int nblocks) {
     return true;
 }
 
-template <class T>
-__global__ __launch_bounds__(64) void k_attend_plain(AttnShape s, Side q, Side k, Side v,
-                                                     const int32_t *__restrict__ blocks, SideOut out,
-                                                     float *__restrict__ lse) {
-    __shared__ float qs[128], ps[64];
-    int64_t w = blockIdx.x;
-    const int h = (int)(w % s.q_heads);
-    w /= s.q_heads;
-    const int i = (int)(w % s.q_len), b = (int)(w / s.q_len), lane = threadIdx.x, g = h / s.group;
-    const int ql = s.ql(b), kl = s.kl(b);
-    if (i >= ql) return;
-    const int p = i + kl - ql, end = s.causal ? min(kl, p + 1) : kl;
-    for (int d = lane; d < s.dim; d += 64) qs[d] = T::up(q.at(b, i, h)[d]);
-    __syncthreads();
-    const int32_t *row = blocks + ((((int64_t)b * s.k_heads + g) * s.q_len) + i) * s.keep;
-    float top = -INFINITY, total = 0.0f, o[2] = {0.0f, 0.0f};
-    for (int t = 0; t < s.keep; ++t) {
-        if (!first_entry(row, t, s.nblocks)) continue;
-        for (int64_t j0 = (int64_t)row[t] * s.block; j0 < (int64_t)(row[t] + 1) * s.block && j0 < end; j0 += 64) {
-            const int64_t j = j0 + lane;
-            float x = -INFINITY;
-            if (j < end) {
-                x = dot_row<T>(qs, k.at(b, j, g), s.dim) * s.scale;
-                if (s.table) x += T::up(s.table[s.map[j - p + s.k_len - 1] * s.q_heads + h]);
-            }
-            const float m = fmaxf(top, wave_max(x)), base = m == -INFINITY ? 0.0f : m;
-            const float e = expf(x - base), f = expf(top - base);
-            total = total * f + wave_sum(e);
-            top = m;
-            ps[lane] = e;
-            __syncthreads();
-            for (int u = 0; u < 2; ++u) {
-                const int d = lane + 64 * u;
-                if (d >= s.dim) continue;
-                o[u] *= f;
-                for (int n = 0; n < 64 && j0 + n < end; ++n) o[u] += ps[n] * T::up(v.at(b, j0 + n, g)[d]);
-            }
-            __syncthreads();
-        }
-    }
-    for (int u = 0; u < 2; ++u)
-        if (lane + 64 * u < s.dim) out.at(b, i, h)[lane + 64 * u] = T::down(total > 0.0f || total != total ? o[u] / total : 0.0f);
-    if (lse && lane == 0) lse[((int64_t)b * s.q_heads + h) * s.q_len + i] = total == 0.0f ? -INFINITY : top + logf(total);
-}
-
 // dq and the row's sums by bucket (sums: batch x q_len x q_heads x buckets), and delta.
 template <class T>
 __global__ __launch_bounds__(64) void k_grad_q_plain(AttnShape s, Side dout, Side q, Side k, Side v, Side out,

@@ -3,7 +3,7 @@
 #include "ias.h"
 #include "ias_internal.hpp"
 #include "attention_kernels.hpp"
-#include "attention_fwd.hpp"
+#include "attention_bwd.hpp"
 
 #include <hip/hip_runtime.h>
 
@@ -128,20 +128,22 @@ ias_status bucket_map(const ias_attention *a, dev::AttnShape &s, uint8_t *map) {
     return launched();
 }
 
-// How k_attend shares out the rows.  16 rows fill one matrix tile, 32 let more
-// queries share a walk and each fragment of K and V feed two tiles; 64 only
-// where one query has that many heads.  Few rows (single tokens) are split along
-// the walk until about every CU has a workgroup, two blocks of keys each at least.
+// How the walks share out the rows.  16 rows fill one matrix tile; 32 let more
+// queries share a walk and each fragment of K and V feed two tiles.  Few rows
+// (single tokens) are split along the walk until about every CU has two workgroups,
+// two blocks of keys each at least.
 struct Rows {
     int mt, dp;
-    dev::AttendPlan plan{};
+    dev::RowPlan plan{};
     int64_t tiles, part, stat;   // all tiles; floats of the splits' results
-    explicit Rows(const ias_attention *a) {
+    explicit Rows(const ias_attention *a, bool small = false) {
         const int group = a->q_heads / a->k_heads;
-        mt = group > 32 ? 4 : group > 16 || a->q_len * group > 16 ? 2 : 1;
+        mt = small || a->q_len * group <= 16 ? 1 : 2;
         dp = a->head_dim > 64 ? 128 : 64;
-        plan.nq = (int32_t)std::max<int64_t>(1, std::min<int64_t>({16 * mt / group, 32, a->q_len}));
-        plan.tiles = (int32_t)ceil_div(a->q_len, plan.nq);
+        plan.span = std::min(group, 16 * mt);
+        plan.parts = (int32_t)ceil_div(group, plan.span);
+        plan.nq = plan.parts > 1 ? 1 : (int32_t)std::max<int64_t>(1, std::min<int64_t>(16 * mt / group, a->q_len));
+        plan.tiles = (int32_t)ceil_div(a->q_len, plan.nq) * plan.parts;
         plan.most = (int32_t)std::max<int64_t>(1, std::min<int64_t>((int64_t)plan.nq * a->keep, ceil_div(a->k_len, a->block)));
         tiles = a->batch * a->k_heads * plan.tiles;
         plan.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({ceil_div(512, std::max<int64_t>(1, tiles)), ceil_div(plan.most, 2), 64}));
@@ -159,13 +161,35 @@ struct Forward {
         rows.plan.stat = rows.stat ? w.part<float>(rows.stat) : nullptr;
     }
 };
+// The backward pass: k_grad_q's rows (as the forward's; with the bias's gradient
+// the lanes' sums by bucket take 1 KB of LDS for each bucket and 16 rows, so 32 rows
+// only up to 32 buckets), and the items of k_grad_kv: about 2048 rows each, which
+// keeps the f32 results of blocks that many queries chose small beside their work.
 struct Backward {
     uint8_t *map;
-    float *delta, *sums;
-    explicit Backward(const ias_attention *a, Space &w) {
+    Rows rows;
+    dev::GradPlan q{};
+    dev::KeyPlan k{};
+    uint32_t *bits;
+    int32_t *count, *first;
+    int64_t items;      // at most
+    explicit Backward(const ias_attention *a, Space &w) : rows(a, a->table && a->num_buckets > 32) {
+        const int64_t group = a->q_heads / a->k_heads, bh = a->batch * a->k_heads, nblocks = ceil_div(a->k_len, a->block);
+        q.nq = rows.plan.nq; q.span = rows.plan.span; q.parts = rows.plan.parts;
+        q.tiles = rows.plan.tiles; q.most = rows.plan.most;
         map = a->table ? w.part<uint8_t>(map_size(a)) : nullptr;
-        delta = w.part<float>(a->batch * a->q_heads * a->q_len);
-        sums = a->table ? w.part<float>(a->batch * a->q_heads * a->q_len * a->num_buckets) : nullptr;
+        q.delta = w.part<float>(a->batch * a->q_heads * a->q_len);
+        q.sums = a->table ? w.part<float>(bh * q.tiles * q.span * a->num_buckets) : nullptr;
+        k.nw = (int32_t)ceil_div(a->q_len, 32);
+        k.per = (int32_t)std::max<int64_t>(32, 2048 / group);
+        k.subs = a->block / 64;
+        k.entries = bh * nblocks;
+        items = k.entries + bh * a->q_len * std::min<int64_t>(a->keep, nblocks) / k.per;
+        k.bits = bits = w.part<uint32_t>(k.entries * k.nw);
+        k.count = count = w.part<int32_t>(k.entries);
+        k.first = first = w.part<int32_t>(k.entries + 1);
+        k.delta = q.delta;
+        k.part = w.part<float>(items * k.subs * 2 * 64 * rows.dp);
     }
 };
 
@@ -195,7 +219,7 @@ ias_status attend_rows(const ias_attention *a, const dev::AttnShape &s, const ia
     else
         IAS_TRY(launch(dev::k_attend<T, DP, MT, false>, grid, 256, lds, a->stream, s, r.plan, side(q), side(k), side(v), blocks, side_out(out), lse));
     if (r.plan.splits > 1)
-        IAS_TRY(launch(dev::k_attend_join<T>, r.tiles * r.plan.nq * s.group, 64, 0, a->stream, s, r.plan, DP, 16 * MT,
+        IAS_TRY(launch(dev::k_attend_join<T>, r.tiles * r.plan.nq * r.plan.span, 64, 0, a->stream, s, r.plan, DP, 16 * MT,
                        a->table ? dev::LOG2E : 1.0f, side_out(out), lse));
     return IAS_SUCCESS;
 }
@@ -206,40 +230,65 @@ ias_status attend(const ias_attention *a, const ias_heads *q, const ias_heads *k
     dev::AttnShape s = shape_of(a);
     if (a->table) IAS_TRY(bucket_map(a, s, f.map));
     const Rows &r = f.rows;
-    if (r.dp == 64) {
-        if (r.mt == 1) return attend_rows<T, 64, 1>(a, s, q, k, v, blocks, out, lse, r);
-        if (r.mt == 2) return attend_rows<T, 64, 2>(a, s, q, k, v, blocks, out, lse, r);
-        return attend_rows<T, 64, 4>(a, s, q, k, v, blocks, out, lse, r);
+    if (r.dp == 64)
+        return r.mt == 1 ? attend_rows<T, 64, 1>(a, s, q, k, v, blocks, out, lse, r) : attend_rows<T, 64, 2>(a, s, q, k, v, blocks, out, lse, r);
+    return r.mt == 1 ? attend_rows<T, 128, 1>(a, s, q, k, v, blocks, out, lse, r) : attend_rows<T, 128, 2>(a, s, q, k, v, blocks, out, lse, r);
+}
+
+template <class T, int DP, int MT>
+ias_status grad_rows(const ias_attention *a, const dev::AttnShape &s, const dev::GradPlan &p, const ias_heads *dout, const ias_heads *q,
+                     const ias_heads *k, const ias_heads *v, const ias_heads *out, const float *lse, const int32_t *blocks,
+                     const ias_heads *dq) {
+    const int64_t tiles = a->batch * a->k_heads * p.tiles, grid = ceil_div(tiles, 8) * 8;
+    const size_t lds = dev::grad_q_lds(DP, MT, s.nblocks, p.most, s.group, s.num_buckets, p.sums);
+    const int32_t area = (int32_t)dev::grad_q_lds(DP, MT, 0, 0, s.group, s.num_buckets, p.sums) - 16 - 4 * s.group * s.num_buckets;
+    if (a->table)
+        return launch(dev::k_grad_q<T, DP, MT, true>, grid, 256, lds, a->stream, s, p, area, side(dout), side(q), side(k), side(v), side(out), lse,
+                      blocks, side_out(dq));
+    return launch(dev::k_grad_q<T, DP, MT, false>, grid, 256, lds, a->stream, s, p, area, side(dout), side(q), side(k), side(v), side(out), lse, blocks,
+                  side_out(dq));
+}
+
+template <class T, int DP>
+ias_status grad_all(const ias_attention *a, const ias_heads *dout, const ias_heads *q, const ias_heads *k, const ias_heads *v,
+                    const ias_heads *out, const float *lse, const int32_t *blocks, const ias_heads *dq, const ias_heads *dk,
+                    const ias_heads *dv, void *dtable, const Backward &w) {
+    dev::AttnShape s = shape_of(a);
+    dev::GradPlan p = w.q;
+    if (!dtable) p.sums = nullptr;
+    if (a->table) IAS_TRY(bucket_map(a, s, w.map));
+    const int64_t bh = a->batch * a->k_heads;
+    if (bh > 0 && a->q_len > 0) {
+        const int mt = w.rows.mt;
+        if (mt == 1) IAS_TRY((grad_rows<T, DP, 1>(a, s, p, dout, q, k, v, out, lse, blocks, dq)));
+        else IAS_TRY((grad_rows<T, DP, 2>(a, s, p, dout, q, k, v, out, lse, blocks, dq)));
     }
-    if (r.mt == 1) return attend_rows<T, 128, 1>(a, s, q, k, v, blocks, out, lse, r);
-    if (r.mt == 2) return attend_rows<T, 128, 2>(a, s, q, k, v, blocks, out, lse, r);
-    return attend_rows<T, 128, 4>(a, s, q, k, v, blocks, out, lse, r);
+    if (w.k.entries > 0) {
+        IAS_TRY(launch(dev::k_clear, ceil_div(w.k.entries, 256), 256, 0, a->stream, w.k.entries, w.count));
+        if (a->q_len > 0)
+            IAS_TRY(launch(dev::k_invert, bh * w.k.nw, 256, 4 * (size_t)s.nblocks, a->stream, s, w.k.nw, blocks, w.bits, w.count));
+        IAS_TRY(launch(dev::k_items, 1, 1024, 0, a->stream, w.k.entries, w.k.per, w.count, w.first));
+        const size_t lds = 4 * 32 * (size_t)DP * 2 + 2 * 5 * 32 * 4 + 4 * (size_t)w.k.per + 32 + 4 * (size_t)s.group * s.num_buckets;
+        const int64_t grid = ceil_div(w.items * w.k.subs, 8) * 8;
+        if (a->q_len > 0) {
+            if (a->table)
+                IAS_TRY(launch(dev::k_grad_kv<T, DP, true>, grid, 256, lds, a->stream, s, w.k, side(dout), side(q), side(k), side(v), lse, side_out(dk), side_out(dv)));
+            else
+                IAS_TRY(launch(dev::k_grad_kv<T, DP, false>, grid, 256, lds, a->stream, s, w.k, side(dout), side(q), side(k), side(v), lse, side_out(dk), side_out(dv)));
+        }
+        IAS_TRY(launch(dev::k_grad_kv_join<T>, w.k.entries * w.k.subs, 256, 0, a->stream, s, w.k, DP, side_out(dk), side_out(dv)));
+    }
+    if (dtable)
+        IAS_TRY(launch(dev::k_grad_table<T>, (int64_t)a->q_heads * a->num_buckets, 256, 0, a->stream, s, p, static_cast<uint16_t *>(dtable)));
+    return IAS_SUCCESS;
 }
 
 template <class T>
 ias_status gradients(const ias_attention *a, const ias_heads *dout, const ias_heads *q, const ias_heads *k,
                      const ias_heads *v, const ias_heads *out, const float *lse, const int32_t *blocks,
                      const ias_heads *dq, const ias_heads *dk, const ias_heads *dv, void *dtable, const Backward &w) {
-    dev::AttnShape s = shape_of(a);
-    hipStream_t st = (hipStream_t)a->stream;
-    if (a->table) IAS_TRY(bucket_map(a, s, w.map));
-    const int64_t rows = a->batch * a->q_heads * a->q_len, keys = a->batch * a->k_heads * a->k_len;
-    if (rows) {
-        dev::k_grad_q_plain<T><<<dim3((unsigned)rows), 64, 0, st>>>(s, side(dout), side(q), side(k), side(v), side(out), lse, blocks,
-                                                                    side_out(dq), w.delta, dtable ? w.sums : nullptr);
-        IAS_TRY(launched());
-    }
-    if (keys) {
-        dev::k_grad_kv_plain<T><<<dim3((unsigned)keys), 64, 0, st>>>(s, side(dout), side(q), side(k), side(v), lse, w.delta, blocks,
-                                                                     side_out(dk), side_out(dv));
-        IAS_TRY(launched());
-    }
-    if (a->table && dtable) {
-        dev::k_grad_table<T><<<dim3((unsigned)(a->q_heads * a->num_buckets)), 256, 0, st>>>(
-            a->batch * a->q_len, a->q_heads, a->num_buckets, w.sums, static_cast<uint16_t *>(dtable));
-        IAS_TRY(launched());
-    }
-    return IAS_SUCCESS;
+    return w.rows.dp == 64 ? grad_all<T, 64>(a, dout, q, k, v, out, lse, blocks, dq, dk, dv, dtable, w)
+                           : grad_all<T, 128>(a, dout, q, k, v, out, lse, blocks, dq, dk, dv, dtable, w);
 }
 
 }  // namespace

@@ -1,0 +1,551 @@
+// attention_bwd.hpp — block-sparse attention, backward.
+//
+// dS = P (dP - delta), with P = exp(x - lse) recomputed and delta = dout . out.
+// k_grad_q walks as the forward pass does (rows of a few queries, the union of
+// their blocks, one piece of 32 keys per wave): dQ^T += K^T dS^T, and the
+// bias's gradient by bucket.  k_grad_kv takes a block of keys and the queries that
+// chose it, which the pattern's transpose lists: dV += P^T dO, dK += dS^T Q.
+// Nothing is added atomically in floating point, every sum has a fixed order.
+#pragma once
+
+#include "attention_fwd.hpp"
+
+namespace ias {
+namespace dev {
+
+// ------------------------------------------------------------------ dq
+struct GradPlan {
+    int32_t nq, span, parts, tiles, most;   // as RowPlan
+    float *delta;                           // [batch][q_heads][q_len]
+    float *sums;                            // [tile][span][num_buckets], null: no dtable
+};
+
+// LDS of k_grad_q: the waves' K tiles and the lanes' sums by bucket, over which
+// the end's sums are laid; the lists; the bias table.
+inline size_t grad_q_lds(int dp, int mt, int nblocks, int most, int group, int buckets, bool sums) {
+    const size_t v = 4 * 32 * (size_t)dp * 2 + (sums ? (size_t)mt * buckets * 256 * 4 : 0), o = 4 * 16 * (size_t)mt * (dp + 4) * 4;
+    return (v > o ? v : o) + 8 * (size_t)((nblocks + 31) / 32) + 8 * (size_t)most + 16 + 4 * (size_t)group * buckets;
+}
+
+template <class T, int DP, int MT, bool BIAS>
+__global__ __launch_bounds__(256, 2) void k_grad_q(AttnShape s, GradPlan plan, int32_t area, Side dout, Side q, Side k,
+                                                                 Side v, Side out, const float *__restrict__ lse,
+                                                                 const int32_t *__restrict__ blocks, SideOut dq) {
+    constexpr int R = 16 * MT, KS = DP / 32, DT = DP / 16, CH = DP / 8;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    float *sums = reinterpret_cast<float *>(lds);                           // [4][R][DP + 4], at the end
+    float *hist = reinterpret_cast<float *>(lds + 4 * 32 * DP * 2);         // [MT][buckets][256]
+    int32_t *scratch = reinterpret_cast<int32_t *>(lds + area);             // total, flag
+    int32_t *ids = scratch + 4;
+    uint32_t *masks = reinterpret_cast<uint32_t *>(ids + plan.most);
+    uint32_t *words = masks + plan.most;
+    float *table = reinterpret_cast<float *>(words + 2 * ((s.nblocks + 31) / 32));
+
+    int64_t w = work_of((int64_t)s.batch * s.k_heads * plan.tiles);
+    if (w >= (int64_t)s.batch * s.k_heads * plan.tiles) return;
+    const int64_t tile_id = w;
+    const int64_t i0 = (w % plan.tiles) / plan.parts * plan.nq;
+    const int h0 = (int)(w % plan.tiles % plan.parts) * plan.span;
+    w /= plan.tiles;
+    const int g = (int)(w % s.k_heads), b = (int)(w / s.k_heads);
+    const int ql = s.ql(b), kl = s.kl(b);
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, col = lane & 15, quad = lane >> 4;
+    if (i0 >= ql) {
+        if (BIAS && plan.sums)
+            for (int e = tid; e < plan.span * s.num_buckets; e += 256) plan.sums[tile_id * plan.span * s.num_buckets + e] = 0.0f;
+        return;
+    }
+    const int nq = min(plan.nq, ql - (int)i0), rows = (nq - 1) * plan.span + min(plan.span, s.group - h0);
+    char *tile = lds + wave * 32 * DP * 2;
+
+    if (BIAS) {
+        for (int e = tid; e < s.num_buckets * s.group; e += 256)
+            table[e] = T::up(s.table[(e / s.group) * s.q_heads + g * s.group + e % s.group]);
+        if (plan.sums)
+            for (int e = tid; e < MT * s.num_buckets * 256; e += 256) hist[e] = 0.0f;
+    }
+    const int found = __builtin_amdgcn_readfirstlane(block_union(s, blocks, b, g, i0, nq, ql, kl, words, ids, masks, scratch));
+
+    s16x8 qf[MT][KS], df[MT][KS];
+    int qi[MT], end[MT], pos[MT], hr[MT];
+    float shift[MT], delta[MT];
+    const float c = BIAS ? s.scale : s.scale * LOG2E;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int r = m * 16 + col;
+        const bool there = r < rows;
+        qi[m] = there ? r / plan.span : 0;
+        hr[m] = h0 + (there ? r % plan.span : 0);
+        pos[m] = (int)i0 + qi[m] + kl - ql;
+        end[m] = !there ? 0 : s.causal ? min(kl, pos[m] + 1) : kl;
+        const int64_t h = (int64_t)g * s.group + hr[m], at = ((int64_t)b * s.q_heads + h) * s.q_len + i0 + qi[m];
+        const uint16_t *qr = q.at(b, i0 + qi[m], h), *dr = dout.at(b, i0 + qi[m], h), *orow = out.at(b, i0 + qi[m], h);
+        float t = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int d = 32 * ks + 8 * quad;
+            const bool on = there && d < s.dim;
+            qf[m][ks] = on ? load8(qr + d) : s16x8{};
+            df[m][ks] = on ? load8(dr + d) : s16x8{};
+            const s16x8 of = on ? load8(orow + d) : s16x8{};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t = fmaf(T::up((uint16_t)df[m][ks][e]), T::up((uint16_t)of[e]), t);
+        }
+        t += __shfl_xor(t, 16);
+        t += __shfl_xor(t, 32);
+        delta[m] = t;
+        const float l = there ? lse[at] : -INFINITY;
+        // a row that read nothing has lse = -inf: exp(x - inf) = 0
+        shift[m] = l == -INFINITY ? INFINITY : BIAS ? l : l * LOG2E;
+        if (wave == 0 && quad == 0 && there) plan.delta[at] = t;
+    }
+    const int per_block = s.block / 32, u1 = found * per_block;
+
+    // turn 0 and the rest as in k_attend: here it is zeros of dS times infinities of K
+    for (int turn = 0; turn <= nq; ++turn) {
+        const uint32_t only = turn == 0 ? ~0u : 1u << (turn - 1);
+        const int vend = turn == 0 || !s.causal ? kl : min(kl, (int)i0 + turn - 1 + kl - ql + 1);
+        f32x4 o[MT][DT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int t = 0; t < DT; ++t) o[m][t] = f32x4{};
+        s16x8 kf[2][KS], vf[2][KS];
+        auto at = [&](int u) { return __builtin_amdgcn_readfirstlane(ids[u / per_block]) * s.block + (u % per_block) * 32; };
+        auto chose = [&](int u) { return (uint32_t)__builtin_amdgcn_readfirstlane(masks[u / per_block]) & only; };
+        auto next = [&](int u) {
+            while (u < u1 && !chose(u)) u += 4;
+            return u;
+        };
+        auto fetch = [&](s16x8 (&f)[2][KS], const Side &x, int u) {
+            const int j0 = at(u);
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub) {
+                const int j = j0 + 16 * sub + col;
+                const uint16_t *row = x.at(b, min(j, kl - 1), g);
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const int d = 32 * ks + 8 * quad;
+                    f[sub][ks] = j < vend && d < s.dim ? load8(row + d) : s16x8{};
+                }
+            }
+        };
+        int u = next(wave);
+        if (u < u1) {
+            fetch(kf, k, u);
+            fetch(vf, v, u);
+        }
+        while (u < u1) {
+            const int j0 = at(u);
+            const uint32_t mask = chose(u);
+            f32x4 x[MT][2], dp[MT][2];
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+                    *reinterpret_cast<s16x8 *>(Tile<DP>::chunk(tile, col, 4 * ks + quad) + 16 * sub * DP * 2) = kf[sub][ks];
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int sub = 0; sub < 2; ++sub) {
+                    f32x4 a{}, e{};
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) {
+                        a = Mma<T>::run(kf[sub][ks], qf[m][ks], a);
+                        e = Mma<T>::run(vf[sub][ks], df[m][ks], e);
+                    }
+                    x[m][sub] = a;
+                    dp[m][sub] = e;
+                }
+            const int un = next(u + 4);
+            if (un < u1) {
+                fetch(kf, k, un);
+                fetch(vf, v, un);
+            }
+            s16x8 sf[MT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const int lim = (mask >> qi[m] & 1u) ? end[m] - j0 - 4 * quad : INT32_MIN;
+                float y[8];
+#pragma unroll
+                for (int sub = 0; sub < 2; ++sub) {
+                    uint32_t bucket = 0;
+                    if (BIAS) __builtin_memcpy(&bucket, s.map + ((int64_t)j0 + 16 * sub + 4 * quad - pos[m] + s.k_len - 1), 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float t = x[m][sub][e] * c;
+                        if (BIAS) t += table[(bucket >> (8 * e) & 255) * s.group + hr[m]];
+                        const float p = BIAS ? __builtin_amdgcn_exp2f((t - shift[m]) * LOG2E) : __builtin_amdgcn_exp2f(t - shift[m]);
+                        const float ds = 16 * sub + e < lim ? p * (dp[m][sub][e] - delta[m]) : 0.0f;
+                        y[4 * sub + e] = ds;
+                        // each lane has a column of its own: the order of these sums is the walk's
+                        if (BIAS && plan.sums && turn == 0)
+                            __hip_atomic_fetch_add(hist + (m * s.num_buckets + (bucket >> (8 * e) & 255)) * 256 + tid, ds, __ATOMIC_RELAXED,
+                                                   __HIP_MEMORY_SCOPE_WAVEFRONT);
+                    }
+                }
+                sf[m] = Mma<T>::pack(y);
+            }
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                const s16x8 kt = Tile<DP>::transposed(tile, 0, t, lane);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) o[m][t] = Mma<T>::run(kt, sf[m], o[m][t]);
+            }
+            u = un;
+        }
+        if (tid == 0) scratch[1] = 0;
+        __syncthreads();
+        if (BIAS && plan.sums && turn == 0) {
+            for (int e = tid; e < plan.span * s.num_buckets; e += 256) {
+                const int h = e / s.num_buckets, n = e % s.num_buckets;
+                float t = 0.0f;
+                for (int r = h; r < rows; r += plan.span) {
+                    const float *from = hist + ((r / 16) * s.num_buckets + n) * 256 + r % 16;
+                    for (int a = 0; a < 16; ++a) t += from[16 * a];
+                }
+                plan.sums[tile_id * plan.span * s.num_buckets + e] = t;
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+                *reinterpret_cast<f32x4 *>(sums + (wave * R + m * 16 + col) * (DP + 4) + 16 * t + 4 * quad) = o[m][t];
+        __syncthreads();
+        bool fine = true;
+        for (int e = tid; e < R * CH; e += 256) {
+            const int r = e / CH, ch = e % CH;
+            if (r >= rows || ch * 8 >= s.dim) continue;
+            const int rq = r / plan.span;
+            if (!(only >> rq & 1u)) continue;
+            float y[8] = {};
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int d = 0; d < 8; ++d) y[d] += sums[(n * R + r) * (DP + 4) + ch * 8 + d];
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+                fine = fine && fabsf(y[d]) < INFINITY;
+                y[d] *= s.scale;
+            }
+            *reinterpret_cast<s16x8 *>(dq.at(b, i0 + rq, (int64_t)g * s.group + h0 + r % plan.span) + ch * 8) = Mma<T>::pack(y);
+        }
+        if (turn == 0) {
+            if (!fine) scratch[1] = 1;
+            __syncthreads();
+            if (scratch[1] == 0) break;
+        }
+        __syncthreads();
+    }
+}
+
+// dtable[n][h]: the tiles' sums, one workgroup for each (bucket, head).
+template <class T>
+__global__ __launch_bounds__(256) void k_grad_table(AttnShape s, GradPlan plan, uint16_t *__restrict__ dtable) {
+    __shared__ float part[256];
+    const int h = blockIdx.x % s.q_heads, n = blockIdx.x / s.q_heads, g = h / s.group, hh = h % s.group;
+    const int32_t each = plan.tiles / plan.parts;   // tiles with this head, of a batch element and key head
+    float t = 0.0f;
+    for (int64_t r = threadIdx.x; r < (int64_t)s.batch * each; r += 256) {
+        const int64_t tile = (r / each * s.k_heads + g) * plan.tiles + r % each * plan.parts + hh / plan.span;
+        t += plan.sums[(tile * plan.span + hh % plan.span) * s.num_buckets + n];
+    }
+    part[threadIdx.x] = t;
+    __syncthreads();
+    for (int d = 128; d; d >>= 1) {
+        if ((int)threadIdx.x < d) part[threadIdx.x] += part[threadIdx.x + d];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) dtable[(int64_t)n * s.q_heads + h] = T::down(part[0]);
+}
+
+// ------------------------------------------------------------------ the pattern's transpose
+// bits[batch x k_heads][block][q_len / 32]: who chose the block and can read of
+// it; count[..][block]: how many.  One workgroup for 32 queries.
+__global__ __launch_bounds__(256) inline void k_invert(AttnShape s, int32_t nw, const int32_t *__restrict__ blocks,
+                                                       uint32_t *__restrict__ bits, int32_t *__restrict__ count) {
+    extern __shared__ uint32_t word[];   // nblocks
+    const int64_t bh = blockIdx.x / nw;
+    const int q32 = (int)(blockIdx.x % nw), b = (int)(bh / s.k_heads);
+    const int ql = s.ql(b), kl = s.kl(b), i0 = q32 * 32;
+    for (int c = threadIdx.x; c < s.nblocks; c += 256) word[c] = 0;
+    __syncthreads();
+    const int n = max(0, min(32, ql - i0)) * s.keep;
+    for (int e = threadIdx.x; e < n; e += 256) {
+        const int i = i0 + e / s.keep, c = blocks[(bh * s.q_len + i0) * s.keep + e];
+        const int end = s.causal ? min(kl, i + kl - ql + 1) : kl;
+        if (c >= 0 && c < s.nblocks && (int64_t)c * s.block < end) atomicOr(&word[c], 1u << (i - i0));
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < s.nblocks; c += 256) {
+        const uint32_t x = word[c];
+        bits[(bh * s.nblocks + c) * nw + q32] = x;
+        if (x) atomicAdd(&count[bh * s.nblocks + c], __popc(x));
+    }
+}
+
+// first[e] = items of the blocks before e, an item being up to `per` queries of a block; first[n] = all.
+__global__ __launch_bounds__(1024) inline void k_items(int64_t n, int32_t per, const int32_t *__restrict__ count, int32_t *__restrict__ first) {
+    __shared__ int32_t part[1024];
+    const int tid = threadIdx.x;
+    const int64_t share = (n + 1023) / 1024, lo = min(n, tid * share), hi = min(n, lo + share);
+    int32_t sum = 0;
+    for (int64_t e = lo; e < hi; ++e) sum += (count[e] + per - 1) / per;
+    part[tid] = sum;
+    __syncthreads();
+    for (int d = 1; d < 1024; d <<= 1) {
+        const int32_t t = tid >= d ? part[tid - d] : 0;
+        __syncthreads();
+        part[tid] += t;
+        __syncthreads();
+    }
+    int32_t at = part[tid] - sum;
+    for (int64_t e = lo; e < hi; ++e) {
+        first[e] = at;
+        at += (count[e] + per - 1) / per;
+    }
+    if (tid == 1023) first[n] = part[1023];
+}
+
+__global__ __launch_bounds__(256) inline void k_clear(int64_t n, int32_t *__restrict__ p) {
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (e < n) p[e] = 0;
+}
+
+// ------------------------------------------------------------------ dk, dv
+struct KeyPlan {
+    int32_t nw, per, subs;      // words of a block's bits, queries of an item, 64-key parts of a block
+    int64_t entries;            // batch x k_heads x nblocks
+    const uint32_t *bits;
+    const int32_t *count, *first;
+    const float *delta;
+    float *part;                // [item][sub][dk, dv][64][DP] of blocks with more than one item
+};
+
+// One workgroup for an item and 64 of its block's keys; wave w has 16 of them,
+// with K and V resident as the right operands of S = Q K^T and dP = dO V^T.
+// Their results hold one key and 2 x 4 rows in a lane, as the left operands of
+// dV += P^T dO and dK += dS^T Q want them; dO and Q come from LDS both ways.
+// P and dS are rounded to the inputs' type for these products (half a step of
+// each), sums are fp32.
+template <class T, int DP, bool BIAS>
+__global__ __launch_bounds__(256, 2) void k_grad_kv(AttnShape s, KeyPlan plan, Side dout, Side q, Side k, Side v,
+                                                    const float *__restrict__ lse, SideOut dk, SideOut dv) {
+    constexpr int KS = DP / 32, DT = DP / 16, CH = DP / 8, TILE = 32 * DP * 2, LD = 32 * CH / 256;
+    extern __shared__ __attribute__((aligned(16))) char lds[];   // [2][Q, dO] tiles
+    float *fig = reinterpret_cast<float *>(lds + 4 * TILE);       // [2][32] of (shift, delta, end, position, head)
+    int32_t *list = reinterpret_cast<int32_t *>(fig + 2 * 5 * 32);
+    int32_t *scratch = list + plan.per;                           // flag, prefix of the list's words
+    float *table = reinterpret_cast<float *>(scratch + 8);
+
+    const int64_t total = (int64_t)plan.first[plan.entries] * plan.subs;
+    int64_t w = work_of((int64_t)gridDim.x);
+    if (w >= total) return;
+    const int sub = (int)(w % plan.subs);
+    const int32_t item = (int32_t)(w / plan.subs);
+    int64_t lo = 0, hi = plan.entries;   // the block with first[e] <= item < first[e + 1]
+    while (hi - lo > 1) {
+        const int64_t mid = (lo + hi) / 2;
+        if (plan.first[mid] <= item) lo = mid;
+        else hi = mid;
+    }
+    const int64_t entry = lo;
+    const int part = item - plan.first[entry], items = plan.first[entry + 1] - plan.first[entry];
+    const int c = (int)(entry % s.nblocks), g = (int)(entry / s.nblocks % s.k_heads), b = (int)(entry / s.nblocks / s.k_heads);
+    const int ql = s.ql(b), kl = s.kl(b), j0 = c * s.block + sub * 64;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, col = lane & 15, quad = lane >> 4;
+    const int nqueries = min(plan.per, plan.count[entry] - part * plan.per);
+
+    if (BIAS)
+        for (int e = tid; e < s.num_buckets * s.group; e += 256)
+            table[e] = T::up(s.table[(e / s.group) * s.q_heads + g * s.group + e % s.group]);
+    // the queries of this item: those whose rank among the block's bits is in [part * per, + per)
+    if (wave == 0) {
+        int before = 0;
+        const uint32_t *bits = plan.bits + entry * plan.nw;
+        for (int w0 = 0; w0 < plan.nw && before < part * plan.per + nqueries; w0 += 64) {
+            uint32_t x = w0 + lane < plan.nw ? bits[w0 + lane] : 0;
+            int sum = __popc(x);
+            const int mine = sum;
+            for (int d = 1; d < 64; d <<= 1) {
+                const int t = __shfl_up(sum, d);
+                if (lane >= d) sum += t;
+            }
+            int rank = before + sum - mine - part * plan.per;
+            for (; x; x &= x - 1, ++rank)
+                if (rank >= 0 && rank < nqueries) list[rank] = (w0 + lane) * 32 + __ffs(x) - 1;
+            before += __shfl(sum, 63);
+        }
+    }
+    // this wave's keys
+    const int key = j0 + 16 * wave + col;
+    s16x8 kf[KS], vf[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        const int d = 32 * ks + 8 * quad;
+        const bool on = key < kl && d < s.dim;
+        kf[ks] = on ? load8(k.at(b, key, g) + d) : s16x8{};
+        vf[ks] = on ? load8(v.at(b, key, g) + d) : s16x8{};
+    }
+    __syncthreads();
+    const int rows = nqueries * s.group;
+    const float cs = BIAS ? s.scale : s.scale * LOG2E;
+
+    // turn 0: 32 rows at a time.  If anything in the result is not finite (zeros of P and dS
+    // times a row's infinities), once more with one row at a time, added only to the keys that it reads.
+    for (int turn = 0; turn < 2; ++turn) {
+        const int step = turn == 0 ? 32 : 1;
+        f32x4 ak[DT], av[DT];
+#pragma unroll
+        for (int t = 0; t < DT; ++t) ak[t] = av[t] = f32x4{};
+        s16x8 qn[LD], dn[LD];
+        float fn[5];
+        auto fetch = [&](int r0) {
+#pragma unroll
+            for (int n = 0; n < LD; ++n) {
+                const int e = n * 256 + tid, r = r0 + e / CH, ch = e % CH;
+                const bool on = e / CH < step && r < rows && ch * 8 < s.dim;
+                const int i = on ? list[r / s.group] : 0;
+                const int64_t h = (int64_t)g * s.group + r % s.group;
+                qn[n] = on ? load8(q.at(b, i, h) + ch * 8) : s16x8{};
+                dn[n] = on ? load8(dout.at(b, i, h) + ch * 8) : s16x8{};
+            }
+            if (tid < 32) {
+                const int r = r0 + tid;
+                const bool on = tid < step && r < rows;
+                const int i = on ? list[r / s.group] : 0, p = i + kl - ql;
+                const int64_t at = ((int64_t)b * s.q_heads + (int64_t)g * s.group + r % s.group) * s.q_len + i;
+                const float l = on ? lse[at] : -INFINITY;
+                fn[0] = l == -INFINITY ? INFINITY : BIAS ? l : l * LOG2E;
+                fn[1] = on ? plan.delta[at] : 0.0f;
+                fn[2] = __int_as_float(!on ? 0 : s.causal ? min(kl, p + 1) : kl);
+                fn[3] = __int_as_float(p);
+                fn[4] = __int_as_float(on ? r % s.group : 0);
+            }
+        };
+        auto put = [&](int buf) {
+#pragma unroll
+            for (int n = 0; n < LD; ++n) {
+                const int e = n * 256 + tid;
+                *reinterpret_cast<s16x8 *>(Tile<DP>::chunk(lds + buf * 2 * TILE, e / CH, e % CH)) = qn[n];
+                *reinterpret_cast<s16x8 *>(Tile<DP>::chunk(lds + buf * 2 * TILE + TILE, e / CH, e % CH)) = dn[n];
+            }
+            if (tid < 32)
+#pragma unroll
+                for (int f = 0; f < 5; ++f) fig[(buf * 5 + f) * 32 + tid] = fn[f];
+        };
+        fetch(0);
+        int buf = 0;
+        for (int r0 = 0; r0 < rows; r0 += step, buf ^= 1) {
+            put(buf);
+            __syncthreads();
+            if (r0 + step < rows) fetch(r0 + step);
+            char *qt = lds + buf * 2 * TILE, *dt = qt + TILE;
+            const float *f = fig + buf * 5 * 32;
+            float p[8], ds[8];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                __builtin_amdgcn_sched_barrier(0);
+                f32x4 x{}, dp{};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    x = Mma<T>::run(*reinterpret_cast<s16x8 *>(Tile<DP>::chunk(qt, col, 4 * ks + quad) + 16 * m * DP * 2), kf[ks], x);
+                    dp = Mma<T>::run(*reinterpret_cast<s16x8 *>(Tile<DP>::chunk(dt, col, 4 * ks + quad) + 16 * m * DP * 2), vf[ks], dp);
+                }
+                const int at = 16 * m + 4 * quad;
+                const f32x4 shift = *reinterpret_cast<const f32x4 *>(f + at), delta = *reinterpret_cast<const f32x4 *>(f + 32 + at);
+                const f32x4 end = *reinterpret_cast<const f32x4 *>(f + 64 + at);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float t = x[e] * cs;
+                    if (BIAS) {
+                        const int pos = __float_as_int(f[96 + at + e]), hr = __float_as_int(f[128 + at + e]);
+                        t += table[s.map[(int64_t)key - pos + s.k_len - 1] * s.group + hr];
+                    }
+                    const bool on = key < __float_as_int(end[e]);
+                    const float y = BIAS ? __builtin_amdgcn_exp2f((t - shift[e]) * LOG2E) : __builtin_amdgcn_exp2f(t - shift[e]);
+                    p[4 * m + e] = on ? y : 0.0f;
+                    ds[4 * m + e] = on ? y * (dp[e] - delta[e]) : 0.0f;
+                }
+            }
+            const s16x8 pf = Mma<T>::pack(p), sf = Mma<T>::pack(ds);
+            const int last = __float_as_int(f[64]) - (j0 + 16 * wave + 4 * quad);   // one row: the keys below are its own
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                if (t % 2 == 0) __builtin_amdgcn_sched_barrier(0);   // else every fragment is read ahead and spilled
+                const s16x8 dtr = Tile<DP>::transposed(dt, 0, t, lane), qtr = Tile<DP>::transposed(qt, 0, t, lane);
+                if (turn == 0) {
+                    av[t] = Mma<T>::run(pf, dtr, av[t]);
+                    ak[t] = Mma<T>::run(sf, qtr, ak[t]);
+                } else {
+                    const f32x4 y = Mma<T>::run(pf, dtr, f32x4{}), z = Mma<T>::run(sf, qtr, f32x4{});
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        av[t][e] = e < last ? av[t][e] + y[e] : av[t][e];
+                        ak[t][e] = e < last ? ak[t][e] + z[e] : ak[t][e];
+                    }
+                }
+            }
+        }
+        if (tid == 0) scratch[0] = 0;
+        __syncthreads();
+        bool fine = true;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            __builtin_amdgcn_sched_barrier(0);   // one row's addresses at a time
+            const int n = 16 * wave + 4 * quad + e, j = j0 + n;
+            uint16_t *tk = dk.at(b, min(j, kl - 1), g) + col, *tv = dv.at(b, min(j, kl - 1), g) + col;
+            float *to = plan.part + (((int64_t)item * plan.subs + sub) * 2 * 64 + n) * DP + col;
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                if (16 * t + col >= s.dim) continue;
+                fine = fine && fabsf(ak[t][e]) < INFINITY && fabsf(av[t][e]) < INFINITY;
+                if (items > 1) {
+                    to[16 * t] = ak[t][e];
+                    to[64 * DP + 16 * t] = av[t][e];
+                } else if (j < kl) {
+                    tk[16 * t] = T::down(ak[t][e] * s.scale);
+                    tv[16 * t] = T::down(av[t][e]);
+                }
+            }
+        }
+        if (turn == 0) {
+            if (!fine) scratch[0] = 1;
+            __syncthreads();
+            if (scratch[0] == 0) break;
+        }
+        __syncthreads();
+    }
+}
+
+// dk and dv of the blocks that no query or more than one item read.
+template <class T>
+__global__ __launch_bounds__(256) void k_grad_kv_join(AttnShape s, KeyPlan plan, int32_t dp, SideOut dk, SideOut dv) {
+    const int sub = (int)(blockIdx.x % plan.subs);
+    const int64_t entry = blockIdx.x / plan.subs;
+    const int32_t first = plan.first[entry], items = plan.first[entry + 1] - first;
+    if (items == 1) return;
+    const int c = (int)(entry % s.nblocks), g = (int)(entry / s.nblocks % s.k_heads), b = (int)(entry / s.nblocks / s.k_heads);
+    const int kl = s.kl(b), j0 = c * s.block + sub * 64, chunks = s.dim / 8;
+    for (int e = threadIdx.x; e < 64 * chunks; e += 256) {
+        const int n = e / chunks, d = e % chunks * 8;
+        if (j0 + n >= kl) continue;
+        float x[8] = {}, y[8] = {};
+        for (int t = 0; t < items; ++t) {
+            const float *from = plan.part + ((((int64_t)first + t) * plan.subs + sub) * 2 * 64 + n) * dp + d;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] += from[i];
+                y[i] += from[64 * dp + i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= s.scale;
+        *reinterpret_cast<s16x8 *>(dk.at(b, j0 + n, g) + d) = Mma<T>::pack(x);
+        *reinterpret_cast<s16x8 *>(dv.at(b, j0 + n, g) + d) = Mma<T>::pack(y);
+    }
+}
+
+}  // namespace dev
+}  // namespace ias

@@ -1,8 +1,8 @@
 // attention_fwd.hpp — block-sparse attention, forward (k_attend, k_attend_join).
 //
-// A workgroup takes the rows of one key head's query heads for a few
-// consecutive queries (16 * MT rows; row r is query r / group, head r % group)
-// and walks the union of the blocks that these queries chose, each block once:
+// A workgroup takes up to 16 * MT rows of one key head: its query heads for a few
+// consecutive queries (row r is query r / span, head r % span), or some of the heads
+// of one query where there are more of them than rows.  It walks the union of the blocks that these queries chose, each block once:
 // neighbouring queries choose mostly the same blocks, and where they do not the
 // walk reads no more than the queries would one by one.  A row that did not
 // choose a block masks it.  The four waves share nothing while they walk: wave w
@@ -72,9 +72,8 @@ template <int DP> struct Tile {
         typedef __attribute__((address_space(3))) s16x4 lds4;
         const int r = row0 + 4 * (lane >> 4) + ((lane & 15) >> 2);
         char *a = t + r * ROW + column(r, col) * 32 + (lane & 3) * 8;
-        char *b = t + (r + 16) * ROW + column(r + 16, col) * 32 + (lane & 3) * 8;
         const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)a);
-        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)b);
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(a + 16 * ROW));   // 16 rows on, the same columns
         return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     }
 };
@@ -135,8 +134,8 @@ __device__ inline int block_union(const AttnShape &s, const int32_t *__restrict_
     return found;
 }
 
-struct AttendPlan {
-    int32_t nq;        // queries of a workgroup
+struct RowPlan {
+    int32_t nq, span, parts;   // queries and heads of a workgroup, workgroups of one query's heads
     int32_t tiles;     // per batch element and key head
     int32_t splits;    // workgroups that share a tile's walk
     int32_t most;      // bound on the blocks of a union
@@ -153,7 +152,7 @@ inline size_t attend_lds(int dp, int mt, int nblocks, int most, int table) {
 }
 
 template <class T, int DP, int MT, bool BIAS>
-__global__ __launch_bounds__(256, MT == 4 ? 1 : 2) void k_attend(AttnShape s, AttendPlan plan, Side q, Side k, Side v,
+__global__ __launch_bounds__(256, 2) void k_attend(AttnShape s, RowPlan plan, Side q, Side k, Side v,
                                                 const int32_t *__restrict__ blocks, SideOut out, float *__restrict__ lse) {
     constexpr int R = 16 * MT, KS = DP / 32, DT = DP / 16, VL = 32 * DP * 2 / 1024, CH = DP / 8;
     constexpr int AREA = attend_out_bytes<DP, MT>() > 4 * 32 * DP * 2 ? attend_out_bytes<DP, MT>() : 4 * 32 * DP * 2;
@@ -171,12 +170,13 @@ __global__ __launch_bounds__(256, MT == 4 ? 1 : 2) void k_attend(AttnShape s, At
     const int split = (int)(w % plan.splits);
     w /= plan.splits;
     const int64_t tile_id = w;
-    const int64_t i0 = (w % plan.tiles) * plan.nq;
+    const int64_t i0 = (w % plan.tiles) / plan.parts * plan.nq;
+    const int h0 = (int)(w % plan.tiles % plan.parts) * plan.span;   // of the key head's query heads
     w /= plan.tiles;
     const int g = (int)(w % s.k_heads), b = (int)(w / s.k_heads);
     const int ql = s.ql(b), kl = s.kl(b);
     if (i0 >= ql) return;
-    const int nq = min(plan.nq, ql - (int)i0), rows = nq * s.group;
+    const int nq = min(plan.nq, ql - (int)i0), rows = (nq - 1) * plan.span + min(plan.span, s.group - h0);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, col = lane & 15, quad = lane >> 4;
     char *tile = lds + wave * 32 * DP * 2;
 
@@ -192,8 +192,8 @@ __global__ __launch_bounds__(256, MT == 4 ? 1 : 2) void k_attend(AttnShape s, At
     for (int m = 0; m < MT; ++m) {
         const int r = m * 16 + col;
         const bool there = r < rows;
-        qi[m] = there ? r / s.group : 0;
-        hr[m] = there ? r % s.group : 0;
+        qi[m] = there ? r / plan.span : 0;
+        hr[m] = h0 + (there ? r % plan.span : 0);
         pos[m] = (int)i0 + qi[m] + kl - ql;
         end[m] = !there ? 0 : s.causal ? min(kl, pos[m] + 1) : kl;
         const uint16_t *row = q.at(b, i0 + qi[m], (int64_t)g * s.group + hr[m]);
@@ -350,7 +350,7 @@ __global__ __launch_bounds__(256, MT == 4 ? 1 : 2) void k_attend(AttnShape s, At
         for (int e = tid; e < R * CH; e += 256) {
             const int r = e / CH, ch = e % CH;
             if (r >= rows || ch * 8 >= s.dim) continue;
-            const int rq = r / s.group;
+            const int rq = r / plan.span;
             if (!(only >> rq & 1u)) continue;
             float all = -INFINITY, l = 0.0f, y[8] = {};
             for (int n = 0; n < 4; ++n) all = fmaxf(all, stat[(n * R + r) * 2]);
@@ -373,7 +373,7 @@ __global__ __launch_bounds__(256, MT == 4 ? 1 : 2) void k_attend(AttnShape s, At
                 float z[8];
 #pragma unroll
                 for (int d = 0; d < 8; ++d) z[d] = y[d] * inv;
-                const int64_t h = (int64_t)g * s.group + r % s.group;
+                const int64_t h = (int64_t)g * s.group + h0 + r % plan.span;
                 *reinterpret_cast<s16x8 *>(out.at(b, i0 + rq, h) + ch * 8) = Mma<T>::pack(z);
                 if (lse && ch == 0)
                     lse[((int64_t)b * s.q_heads + h) * s.q_len + i0 + rq] =
@@ -394,15 +394,16 @@ __global__ __launch_bounds__(256, MT == 4 ? 1 : 2) void k_attend(AttnShape s, At
 
 // Joins the splits of a tile: one wave for each row.
 template <class T>
-__global__ __launch_bounds__(64) void k_attend_join(AttnShape s, AttendPlan plan, int32_t dp, int32_t tile_rows, float unit,
+__global__ __launch_bounds__(64) void k_attend_join(AttnShape s, RowPlan plan, int32_t dp, int32_t tile_rows, float unit,
                                                     SideOut out, float *__restrict__ lse) {
     int64_t w = blockIdx.x;
-    const int r = (int)(w % (plan.nq * s.group));
-    w /= plan.nq * s.group;
-    const int64_t tile_id = w, i = (w % plan.tiles) * plan.nq + r / s.group;
+    const int r = (int)(w % (plan.nq * plan.span));
+    w /= plan.nq * plan.span;
+    const int64_t tile_id = w, i = (w % plan.tiles) / plan.parts * plan.nq + r / plan.span;
+    const int hh = (int)(w % plan.tiles % plan.parts) * plan.span + r % plan.span;
     w /= plan.tiles;
     const int g = (int)(w % s.k_heads), b = (int)(w / s.k_heads), lane = threadIdx.x;
-    if (i >= s.ql(b)) return;
+    if (i >= s.ql(b) || hh >= s.group) return;
     float all = -INFINITY, l = 0.0f, y[2] = {};
     for (int n = 0; n < plan.splits; ++n) all = fmaxf(all, plan.stat[((tile_id * plan.splits + n) * tile_rows + r) * 2]);
     for (int n = 0; n < plan.splits; ++n) {
@@ -414,7 +415,7 @@ __global__ __launch_bounds__(64) void k_attend_join(AttnShape s, AttendPlan plan
         for (int u = 0; u < 2; ++u)
             if (2 * lane + u < s.dim) y[u] += plan.part[at * dp + 2 * lane + u] * f;
     }
-    const int64_t h = (int64_t)g * s.group + r % s.group;
+    const int64_t h = (int64_t)g * s.group + hh;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (2 * lane < s.dim) {
         uint16_t *to = out.at(b, i, h) + 2 * lane;

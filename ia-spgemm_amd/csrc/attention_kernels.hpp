@@ -180,161 +180,5 @@ __global__ __launch_bounds__(256) void k_bucket_map(int64_t k_len, int64_t n, in
     map[e] = (uint8_t)lo;
 }
 
-// ------------------------------------------------------------------ plain forms
-// One wave for each (batch, query, head): 64 keys at a time, a key per lane.
-__device__ inline float wave_max(float x) {
-    for (int d = 32; d; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
-    return x;
-}
-__device__ inline float wave_sum(float x) {
-    for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
-    return x;
-}
-
-template <class T> __device__ float dot_row(const float *a, const uint16_t *x, int dim) {
-    float t = 0.0f;
-    for (int d = 0; d < dim; ++d) t += a[d] * T::up(x[d]);
-    return t;
-}
-
-__device__ inline bool first_entry(const int32_t *row, int t, int nblocks) {
-    const int c = row[t];
-    if (c < 0 || c >= nblocks) return false;
-    for (int u = 0; u < t; ++u)
-        if (row[u] == c) return false;
-    return true;
-}
-
-// dq and the row's sums by bucket (sums: batch x q_len x q_heads x buckets), and delta.
-template <class T>
-__global__ __launch_bounds__(64) void k_grad_q_plain(AttnShape s, Side dout, Side q, Side k, Side v, Side out,
-                                                     const float *__restrict__ lse, const int32_t *__restrict__ blocks,
-                                                     SideOut dq, float *__restrict__ delta, float *__restrict__ sums) {
-    __shared__ float qs[128], ds[128], ps[64], hist[64];
-    int64_t w = blockIdx.x;
-    const int h = (int)(w % s.q_heads);
-    w /= s.q_heads;
-    const int i = (int)(w % s.q_len), b = (int)(w / s.q_len), lane = threadIdx.x, g = h / s.group;
-    const int ql = s.ql(b), kl = s.kl(b);
-    hist[lane] = 0.0f;
-    __syncthreads();
-    if (i < ql) {
-        const int p = i + kl - ql, end = s.causal ? min(kl, p + 1) : kl;
-        float part = 0.0f;
-        for (int d = lane; d < s.dim; d += 64) {
-            qs[d] = T::up(q.at(b, i, h)[d]);
-            ds[d] = T::up(dout.at(b, i, h)[d]);
-            part += ds[d] * T::up(out.at(b, i, h)[d]);
-        }
-        const float dl = wave_sum(part), l = lse[((int64_t)b * s.q_heads + h) * s.q_len + i];
-        if (lane == 0) delta[((int64_t)b * s.q_heads + h) * s.q_len + i] = dl;
-        __syncthreads();
-        const int32_t *row = blocks + ((((int64_t)b * s.k_heads + g) * s.q_len) + i) * s.keep;
-        float o[2] = {0.0f, 0.0f};
-        for (int t = 0; t < s.keep; ++t) {
-            if (!first_entry(row, t, s.nblocks)) continue;
-            for (int64_t j0 = (int64_t)row[t] * s.block; j0 < (int64_t)(row[t] + 1) * s.block && j0 < end; j0 += 64) {
-                const int64_t j = j0 + lane;
-                float e = 0.0f;
-                if (j < end && l != -INFINITY) {
-                    float x = dot_row<T>(qs, k.at(b, j, g), s.dim) * s.scale;
-                    const int bucket = s.table ? s.map[j - p + s.k_len - 1] : 0;
-                    if (s.table) x += T::up(s.table[bucket * s.q_heads + h]);
-                    e = expf(x - l) * (dot_row<T>(ds, v.at(b, j, g), s.dim) - dl);
-                }
-                ps[lane] = e;
-                __syncthreads();
-                for (int u = 0; u < 2; ++u) {
-                    const int d = lane + 64 * u;
-                    if (d >= s.dim) continue;
-                    for (int n = 0; n < 64 && j0 + n < end; ++n) o[u] += ps[n] * T::up(k.at(b, j0 + n, g)[d]);
-                }
-                if (s.table && lane == 0)
-                    for (int n = 0; n < 64 && j0 + n < end; ++n) hist[s.map[j0 + n - p + s.k_len - 1]] += ps[n];
-                __syncthreads();
-            }
-        }
-        for (int u = 0; u < 2; ++u)
-            if (lane + 64 * u < s.dim) dq.at(b, i, h)[lane + 64 * u] = T::down(o[u] * s.scale);
-    }
-    if (sums && lane < s.num_buckets)
-        sums[(((int64_t)b * s.q_len + i) * s.q_heads + h) * s.num_buckets + lane] = hist[lane];
-}
-
-// One wave for each (batch, key head, key): every query that reads its block.
-template <class T>
-__global__ __launch_bounds__(64) void k_grad_kv_plain(AttnShape s, Side dout, Side q, Side k, Side v,
-                                                      const float *__restrict__ lse, const float *__restrict__ delta,
-                                                      const int32_t *__restrict__ blocks, SideOut dk, SideOut dv) {
-    __shared__ float ks[128], vs[128];
-    int64_t w = blockIdx.x;
-    const int g = (int)(w % s.k_heads);
-    w /= s.k_heads;
-    const int j = (int)(w % s.k_len), b = (int)(w / s.k_len), lane = threadIdx.x;
-    const int ql = s.ql(b), kl = s.kl(b);
-    if (j >= kl) return;
-    for (int d = lane; d < s.dim; d += 64) {
-        ks[d] = T::up(k.at(b, j, g)[d]);
-        vs[d] = T::up(v.at(b, j, g)[d]);
-    }
-    __syncthreads();
-    const int c = j / s.block;
-    float ok[2] = {}, ov[2] = {};
-    for (int i0 = 0; i0 < ql; i0 += 64) {
-        const int i = i0 + lane;
-        bool on = false;
-        if (i < ql && (!s.causal || j <= i + kl - ql)) {
-            const int32_t *row = blocks + ((((int64_t)b * s.k_heads + g) * s.q_len) + i) * s.keep;
-            for (int t = 0; t < s.keep; ++t) on = on || row[t] == c;
-        }
-        for (unsigned long long m = __ballot(on); m; m &= m - 1) {
-            const int r = i0 + __ffsll(m) - 1;
-            for (int h = g * s.group; h < (g + 1) * s.group; ++h) {
-                const int64_t at = ((int64_t)b * s.q_heads + h) * s.q_len + r;
-                float a = 0.0f, e = 0.0f, x[2] = {}, y[2] = {};
-                for (int u = 0; u < 2; ++u) {
-                    const int d = lane + 64 * u;
-                    if (d >= s.dim) continue;
-                    x[u] = T::up(q.at(b, r, h)[d]);
-                    y[u] = T::up(dout.at(b, r, h)[d]);
-                    a += x[u] * ks[d];
-                    e += y[u] * vs[d];
-                }
-                a = wave_sum(a) * s.scale;
-                e = wave_sum(e);
-                if (s.table) a += T::up(s.table[s.map[j - (r + kl - ql) + s.k_len - 1] * s.q_heads + h]);
-                if (lse[at] == -INFINITY) continue;
-                const float pr = expf(a - lse[at]), dsv = pr * (e - delta[at]);
-                for (int u = 0; u < 2; ++u) {
-                    ov[u] += pr * y[u];
-                    ok[u] += dsv * x[u];
-                }
-            }
-        }
-    }
-    for (int u = 0; u < 2; ++u)
-        if (lane + 64 * u < s.dim) {
-            dk.at(b, j, g)[lane + 64 * u] = T::down(ok[u] * s.scale);
-            dv.at(b, j, g)[lane + 64 * u] = T::down(ov[u]);
-        }
-}
-
-// dtable from the rows' sums, in a fixed order.
-template <class T>
-__global__ __launch_bounds__(256) void k_grad_table(int64_t rows, int32_t heads, int32_t nb,
-                                                    const float *__restrict__ sums, uint16_t *__restrict__ dtable) {
-    __shared__ float part[256];
-    const int h = blockIdx.x % heads, n = blockIdx.x / heads;
-    float t = 0.0f;
-    for (int64_t r = threadIdx.x; r < rows; r += 256) t += sums[(r * heads + h) * nb + n];
-    part[threadIdx.x] = t;
-    __syncthreads();
-    for (int d = 128; d; d >>= 1) {
-        if ((int)threadIdx.x < d) part[threadIdx.x] += part[threadIdx.x + d];
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) dtable[(int64_t)n * heads + h] = T::down(part[0]);
-}
-
 }  // namespace dev
 }  // namespace ias

@@ -4,6 +4,7 @@
 #include "ias_internal.hpp"
 #include "attention_kernels.hpp"
 #include "attention_bwd.hpp"
+#include "attention_select.hpp"
 
 #include <hip/hip_runtime.h>
 
@@ -210,6 +211,35 @@ ias_status launch(K kernel, int64_t grid, int threads, size_t lds, void *stream,
 }
 
 template <class T, int DP, int MT>
+ias_status select_rows(const ias_attention *a, const dev::AttnShape &s, const dev::SelectPlan &p, int threads, const ias_heads *q,
+                       const void *summary, int32_t *blocks) {
+    const int64_t grid = ceil_div(a->batch * a->k_heads * p.tiles, 8) * 8;
+    return launch(dev::k_block_select<T, DP, MT>, grid, threads, dev::select_lds(p.nq, p.stride, threads / 64), a->stream, s, p, side(q),
+                  static_cast<const uint16_t *>(summary), blocks);
+}
+
+// 64 rows to a workgroup, so that a summary is read for many queries, while the
+// queries' keys take at most 64 KB of LDS.  Where there are few workgroups and 16
+// rows are enough (single tokens), more waves share the blocks.
+template <class T, int DP>
+ias_status select(const ias_attention *a, const ias_heads *q, const void *summary, int32_t first, int32_t local, int32_t *blocks) {
+    const dev::AttnShape s = shape_of(a);
+    dev::SelectPlan p{};
+    p.first = first; p.local = local;
+    p.stride = std::max(1, s.nblocks);
+    p.nq = (int32_t)std::min<int64_t>({64 / s.group, a->q_len, std::max(1, 16384 / p.stride)});
+    p.tiles = (int32_t)ceil_div(a->q_len, p.nq);
+    const int rows = p.nq * s.group;
+    if (rows <= 16) {
+        const int64_t few = a->batch * a->k_heads * p.tiles < 512;
+        const int threads = few ? (int)std::min<int64_t>(1024, std::max<int64_t>(256, ceil_div(p.stride, 32) * 64)) : 256;
+        return select_rows<T, DP, 1>(a, s, p, threads, q, summary, blocks);
+    }
+    if (rows <= 32) return select_rows<T, DP, 2>(a, s, p, 256, q, summary, blocks);
+    return select_rows<T, DP, 4>(a, s, p, 256, q, summary, blocks);
+}
+
+template <class T, int DP, int MT>
 ias_status attend_rows(const ias_attention *a, const dev::AttnShape &s, const ias_heads *q, const ias_heads *k,
                        const ias_heads *v, const int32_t *blocks, const ias_heads *out, float *lse, const Rows &r) {
     const int64_t grid = ceil_div(r.tiles * r.plan.splits, 8) * 8;
@@ -324,18 +354,11 @@ extern "C" ias_status ias_block_select(const ias_attention *a, const ias_heads *
     if ((!summary && a->k_len > 0) || !blocks) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "no summary or blocks");
     OnDevice on;
     HIPC(on.to(a->device));
-    const dev::AttnShape s = shape_of(a);
-    const dim3 grid((unsigned)(a->batch * a->k_heads * a->q_len));
-    const size_t lds = 8 * (size_t)s.nblocks + 4 * (size_t)((s.nblocks + 31) / 32);
-    const uint16_t *m = static_cast<const uint16_t *>(summary);
-    if (a->dtype == IAS_DTYPE_BF16) {
-        HIPC(hipFuncSetAttribute((const void *)dev::k_block_select<dev::Bf16>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
-        dev::k_block_select<dev::Bf16><<<grid, 64, lds, (hipStream_t)a->stream>>>(s, side(q), m, first, local, blocks);
-    } else {
-        HIPC(hipFuncSetAttribute((const void *)dev::k_block_select<dev::Fp16>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
-        dev::k_block_select<dev::Fp16><<<grid, 64, lds, (hipStream_t)a->stream>>>(s, side(q), m, first, local, blocks);
-    }
-    return launched();
+    if (a->head_dim <= 64)
+        return a->dtype == IAS_DTYPE_BF16 ? select<dev::Bf16, 64>(a, q, summary, first, local, blocks)
+                                          : select<dev::Fp16, 64>(a, q, summary, first, local, blocks);
+    return a->dtype == IAS_DTYPE_BF16 ? select<dev::Bf16, 128>(a, q, summary, first, local, blocks)
+                                      : select<dev::Fp16, 128>(a, q, summary, first, local, blocks);
 }
 
 extern "C" ias_status ias_block_attention_workspace(const ias_attention *a, int64_t *forward, int64_t *backward) {

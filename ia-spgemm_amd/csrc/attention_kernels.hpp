@@ -96,74 +96,6 @@ __global__ __launch_bounds__(256) void k_block_summary(AttnShape s, Side k, int6
     }
 }
 
-// ------------------------------------------------------------------ selection
-__device__ inline unsigned long long order_key(double x) {
-    x = x + 0.0;   // -0 ranks as +0
-    const unsigned long long u = (unsigned long long)__double_as_longlong(x);
-    return (u >> 63) ? ~u : u | (1ull << 63);
-}
-
-template <class T>
-__global__ __launch_bounds__(64) void k_block_select(AttnShape s, Side q, const uint16_t *__restrict__ summary,
-                                                     int32_t first, int32_t local, int32_t *__restrict__ blocks) {
-    extern __shared__ unsigned long long key[];   // nblocks, then the chosen bits
-    uint32_t *chosen = reinterpret_cast<uint32_t *>(key + s.nblocks);
-    int64_t w = blockIdx.x;
-    const int i = (int)(w % s.q_len);
-    w /= s.q_len;
-    const int g = (int)(w % s.k_heads), b = (int)(w / s.k_heads), lane = threadIdx.x;
-    const int ql = s.ql(b), kl = s.kl(b);
-    if (i >= ql) return;
-    const int p = i + kl - ql;
-    const int seen = s.causal ? (p < 0 ? 0 : p / s.block + 1) : (kl + s.block - 1) / s.block;
-    for (int n = lane; n < (s.nblocks + 31) / 32; n += 64) chosen[n] = 0;
-    for (int c = lane; c < seen; c += 64) {
-        const uint16_t *m = summary + (((int64_t)b * s.k_heads + g) * s.nblocks + c) * s.dim;
-        double best = -INFINITY;
-        for (int h = 0; h < s.group; ++h) {
-            const uint16_t *x = q.at(b, i, g * s.group + h);
-            double t = 0.0;
-            for (int d = 0; d < s.dim; ++d) t += (double)T::up(x[d]) * (double)T::up(m[d]);
-            if (t > best) best = t;
-        }
-        key[c] = order_key(best);
-    }
-    __syncthreads();
-    int left = min(s.keep, seen);
-    auto take = [&](int c) {
-        if (lane == 0) {
-            chosen[c / 32] |= 1u << (c % 32);
-            key[c] = 0;
-        }
-        --left;
-        __syncthreads();
-    };
-    for (int c = 0; c < min(first, seen); ++c) take(c);
-    for (int c = max(min(first, seen), seen - local); c < seen; ++c) take(c);
-    while (left > 0) {
-        unsigned long long top = 0;
-        int at = INT32_MAX;
-        for (int c = lane; c < seen; c += 64)
-            if (key[c] > top) { top = key[c]; at = c; }
-        for (int d = 32; d; d >>= 1) {
-            const unsigned long long t = __shfl_xor(top, d);
-            const int a = __shfl_xor(at, d);
-            if (t > top || (t == top && a < at)) { top = t; at = a; }
-        }
-        take(at);
-    }
-    int32_t *row = blocks + ((((int64_t)b * s.k_heads + g) * s.q_len) + i) * s.keep;
-    int n = 0;
-    for (int c0 = 0; c0 < seen; c0 += 64) {
-        const int c = c0 + lane;
-        const bool on = c < seen && (chosen[c / 32] >> (c % 32) & 1);
-        const unsigned long long m = __ballot(on);
-        if (on) row[n + __popcll(m & ((1ull << lane) - 1))] = c;
-        n += __popcll(m);
-    }
-    for (int t = n + lane; t < s.keep; t += 64) row[t] = -1;
-}
-
 // ------------------------------------------------------------------ bucket map
 // map[d + k_len - 1] = how many edges are <= d, for every distance of a call.
 __global__ __launch_bounds__(256) void k_bucket_map(int64_t k_len, int64_t n, int32_t num_buckets,

@@ -84,6 +84,8 @@ ias_status check_heads(const ias_heads *h, const char *name, int64_t batch, int6
     if (!h->data) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "%s: no data", name);
     if (((uintptr_t)h->data & 15) || (batch > 1 && h->batch % 8) || (n > 1 && h->token % 8) || (heads > 1 && h->head % 8))
         REFUSE(IAS_ERROR_UNSUPPORTED, "%s: data has to be 16-byte aligned and its strides multiples of 8", name);
+    if (n > 1 && (h->token < 0 || h->token > (1 << 24)))   // 32 rows by a 32-bit offset
+        REFUSE(IAS_ERROR_UNSUPPORTED, "%s: token stride %lld: 0 to 2^24", name, (long long)h->token);
     return IAS_SUCCESS;
 }
 

@@ -20,10 +20,10 @@ struct GradPlan {
     float *sums;                            // [tile][span][num_buckets], null: no dtable
 };
 
-// LDS of k_grad_q: the waves' K tiles and the lanes' sums by bucket, over which
+// LDS of k_grad_q: the waves' K and V tiles and the lanes' sums by bucket, over which
 // the end's sums are laid; the lists; the bias table.
 inline size_t grad_q_lds(int dp, int mt, int nblocks, int most, int group, int buckets, bool sums) {
-    const size_t v = 4 * 32 * (size_t)dp * 2 + (sums ? (size_t)mt * buckets * 256 * 4 : 0), o = 4 * 16 * (size_t)mt * (dp + 4) * 4;
+    const size_t v = 4 * 2 * 32 * (size_t)dp * 2 + (sums ? (size_t)mt * buckets * 256 * 4 : 0), o = 4 * 16 * (size_t)mt * (dp + 4) * 4;
     return (v > o ? v : o) + 8 * (size_t)((nblocks + 31) / 32) + 8 * (size_t)most + 16 + 4 * (size_t)group * buckets;
 }
 
@@ -34,7 +34,7 @@ __global__ __launch_bounds__(256, 2) void k_grad_q(AttnShape s, GradPlan plan, i
     constexpr int R = 16 * MT, KS = DP / 32, DT = DP / 16, CH = DP / 8;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float *sums = reinterpret_cast<float *>(lds);                           // [4][R][DP + 4], at the end
-    float *hist = reinterpret_cast<float *>(lds + 4 * 32 * DP * 2);         // [MT][buckets][256]
+    float *hist = reinterpret_cast<float *>(lds + 4 * 2 * 32 * DP * 2);       // [MT][buckets][256]
     int32_t *scratch = reinterpret_cast<int32_t *>(lds + area);             // total, flag
     int32_t *ids = scratch + 4;
     uint32_t *masks = reinterpret_cast<uint32_t *>(ids + plan.most);
@@ -56,7 +56,8 @@ __global__ __launch_bounds__(256, 2) void k_grad_q(AttnShape s, GradPlan plan, i
         return;
     }
     const int nq = min(plan.nq, ql - (int)i0), rows = (nq - 1) * plan.span + min(plan.span, s.group - h0);
-    char *tile = lds + wave * 32 * DP * 2;
+    const Tile<DP> tile(lds + wave * 2 * Tile<DP>::BYTES, lane);   // K, then V
+    constexpr int KT = 0, VT = Tile<DP>::BYTES;
 
     if (BIAS) {
         for (int e = tid; e < s.num_buckets * s.group; e += 256)
@@ -69,7 +70,7 @@ __global__ __launch_bounds__(256, 2) void k_grad_q(AttnShape s, GradPlan plan, i
     s16x8 qf[MT][KS], df[MT][KS];
     int qi[MT], end[MT], pos[MT], hr[MT];
     float shift[MT], delta[MT];
-    const float c = BIAS ? s.scale : s.scale * LOG2E;
+    const float c = fabsf(BIAS ? s.scale : s.scale * LOG2E);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         const int r = m * 16 + col;
@@ -86,20 +87,22 @@ __global__ __launch_bounds__(256, 2) void k_grad_q(AttnShape s, GradPlan plan, i
             const int d = 32 * ks + 8 * quad;
             const bool on = there && d < s.dim;
             qf[m][ks] = on ? load8(qr + d) : s16x8{};
+            if (s.scale < 0.0f) qf[m][ks] = negated(qf[m][ks]);
             df[m][ks] = on ? load8(dr + d) : s16x8{};
             const s16x8 of = on ? load8(orow + d) : s16x8{};
 #pragma unroll
             for (int e = 0; e < 8; ++e) t = fmaf(T::up((uint16_t)df[m][ks][e]), T::up((uint16_t)of[e]), t);
         }
-        t += __shfl_xor(t, 16);
-        t += __shfl_xor(t, 32);
+        t = quad_sum(t);
         delta[m] = t;
         const float l = there ? lse[at] : -INFINITY;
         // a row that read nothing has lse = -inf: exp(x - inf) = 0
         shift[m] = l == -INFINITY ? INFINITY : BIAS ? l : l * LOG2E;
         if (wave == 0 && quad == 0 && there) plan.delta[at] = t;
     }
-    const int per_block = s.block / 32, u1 = found * per_block;
+    const int per_block = s.block / 32;
+    const int sure = s.causal ? min(kl, (int)i0 + kl - ql + 1) : kl;
+    const Piece<DP> kp(k, b, g, lane, s.dim, kl), vp(v, b, g, lane, s.dim, kl);
 
     // turn 0 and the rest as in k_attend: here it is zeros of dS times infinities of K
     for (int turn = 0; turn <= nq; ++turn) {
@@ -110,100 +113,120 @@ __global__ __launch_bounds__(256, 2) void k_grad_q(AttnShape s, GradPlan plan, i
         for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int t = 0; t < DT; ++t) o[m][t] = f32x4{};
-        s16x8 kf[2][KS], vf[2][KS];
-        auto at = [&](int u) { return __builtin_amdgcn_readfirstlane(ids[u / per_block]) * s.block + (u % per_block) * 32; };
-        auto chose = [&](int u) { return (uint32_t)__builtin_amdgcn_readfirstlane(masks[u / per_block]) & only; };
-        auto next = [&](int u) {
-            while (u < u1 && !chose(u)) u += 4;
-            return u;
+        s16x8 kr[Piece<DP>::N], vr[Piece<DP>::N];
+        Walk at(wave, per_block);
+        auto skip = [&]() {
+            while (turn > 0 && at.step < found && !(masks[at.step] & only)) at.on();
         };
-        auto fetch = [&](s16x8 (&f)[2][KS], const Side &x, int u) {
-            const int j0 = at(u);
-#pragma unroll
-            for (int sub = 0; sub < 2; ++sub) {
-                const int j = j0 + 16 * sub + col;
-                const uint16_t *row = x.at(b, min(j, kl - 1), g);
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    const int d = 32 * ks + 8 * quad;
-                    f[sub][ks] = j < vend && d < s.dim ? load8(row + d) : s16x8{};
-                }
-            }
-        };
-        int u = next(wave);
-        if (u < u1) {
-            fetch(kf, k, u);
-            fetch(vf, v, u);
+        skip();
+        int j0 = 0;
+        uint32_t mask = 0;
+        if (at.step < found) {
+            j0 = __builtin_amdgcn_readfirstlane(ids[at.step]) * s.block + at.part * 32;
+            mask = __builtin_amdgcn_readfirstlane(masks[at.step]) & only;
+            kp.load(kr, j0, vend);
+            vp.load(vr, j0, vend);
         }
-        while (u < u1) {
-            const int j0 = at(u);
-            const uint32_t mask = chose(u);
+        while (at.step < found) {
+            at.on();
+            skip();
+            const bool more = at.step < found;
+            const int id = more ? ids[at.step] : 0;
+            const uint32_t chose = more ? masks[at.step] : 0;
+            tile.fill(kr, KT);
+            tile.fill(vr, VT);
             f32x4 x[MT][2], dp[MT][2];
 #pragma unroll
-            for (int sub = 0; sub < 2; ++sub)
+            for (int sub = 0; sub < 2; ++sub) {
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-                    *reinterpret_cast<s16x8 *>(Tile<DP>::chunk(tile, col, 4 * ks + quad) + 16 * sub * DP * 2) = kf[sub][ks];
+                for (int m = 0; m < MT; ++m) x[m][sub] = dp[m][sub] = f32x4{};
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+                for (int ks = 0; ks < KS; ++ks) {
+                    const s16x8 kf = tile.natural(KT, 16 * sub, ks), vf = tile.natural(VT, 16 * sub, ks);
 #pragma unroll
-                for (int sub = 0; sub < 2; ++sub) {
-                    f32x4 a{}, e{};
-#pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        a = Mma<T>::run(kf[sub][ks], qf[m][ks], a);
-                        e = Mma<T>::run(vf[sub][ks], df[m][ks], e);
+                    for (int m = 0; m < MT; ++m) {
+                        x[m][sub] = Mma<T>::run(kf, qf[m][ks], x[m][sub]);
+                        dp[m][sub] = Mma<T>::run(vf, df[m][ks], dp[m][sub]);
                     }
-                    x[m][sub] = a;
-                    dp[m][sub] = e;
                 }
-            const int un = next(u + 4);
-            if (un < u1) {
-                fetch(kf, k, un);
-                fetch(vf, v, un);
             }
+            const int jn = __builtin_amdgcn_readfirstlane(id) * s.block + at.part * 32;
+            const uint32_t maskn = __builtin_amdgcn_readfirstlane(chose) & only;
+            if (more) {
+                kp.load(kr, jn, vend);
+                vp.load(vr, jn, vend);
+            }
+            const bool whole = j0 + 32 <= sure;
             s16x8 sf[MT];
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                const int lim = (mask >> qi[m] & 1u) ? end[m] - j0 - 4 * quad : INT32_MIN;
+                const bool sel = mask >> qi[m] & 1u;
+                const float off = sel ? shift[m] : INFINITY;   // exp(x - inf) = 0
                 float y[8];
+                uint32_t bucket[2] = {};
 #pragma unroll
                 for (int sub = 0; sub < 2; ++sub) {
-                    uint32_t bucket = 0;
-                    if (BIAS) __builtin_memcpy(&bucket, s.map + ((int64_t)j0 + 16 * sub + 4 * quad - pos[m] + s.k_len - 1), 4);
+                    if (BIAS) __builtin_memcpy(&bucket[sub], s.map + ((int64_t)j0 + 16 * sub + 4 * quad - pos[m] + s.k_len - 1), 4);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float t = x[m][sub][e] * c;
-                        if (BIAS) t += table[(bucket >> (8 * e) & 255) * s.group + hr[m]];
-                        const float p = BIAS ? __builtin_amdgcn_exp2f((t - shift[m]) * LOG2E) : __builtin_amdgcn_exp2f(t - shift[m]);
-                        const float ds = 16 * sub + e < lim ? p * (dp[m][sub][e] - delta[m]) : 0.0f;
-                        y[4 * sub + e] = ds;
-                        // each lane has a column of its own: the order of these sums is the walk's
-                        if (BIAS && plan.sums && turn == 0)
-                            __hip_atomic_fetch_add(hist + (m * s.num_buckets + (bucket >> (8 * e) & 255)) * 256 + tid, ds, __ATOMIC_RELAXED,
-                                                   __HIP_MEMORY_SCOPE_WAVEFRONT);
+                        float p;
+                        if (BIAS)
+                            p = __builtin_amdgcn_exp2f((__builtin_fmaf(x[m][sub][e], c, table[(bucket[sub] >> (8 * e) & 255) * s.group + hr[m]]) - off) * LOG2E);
+                        else
+                            p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[m][sub][e], c, -off));
+                        y[4 * sub + e] = p * (dp[m][sub][e] - delta[m]);
+                    }
+                }
+                if (!whole) {
+                    const int lim = end[m] - j0 - 4 * quad;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = 16 * (e / 4) + e % 4 < lim ? y[e] : 0.0f;
+                }
+                if (BIAS && plan.sums && turn == 0) {
+                    // Each lane has a column of its own, so plain sums do, in the walk's order (an
+                    // atomic LDS add takes some 200 cycles a wave).  Far keys share a bucket, mostly
+                    // for a whole wave: then their sum goes in at once.
+                    float *mine = hist + m * s.num_buckets * 256 + tid;
+                    if (!sel)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[e] = 0.0f;
+#pragma unroll
+                    for (int sub = 0; sub < 2; ++sub) {
+                        const uint32_t n = bucket[sub] & 255;
+                        if (__all(bucket[sub] == n * 0x01010101u)) {
+                            mine[n * 256] += (y[4 * sub] + y[4 * sub + 1]) + (y[4 * sub + 2] + y[4 * sub + 3]);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) mine[(bucket[sub] >> (8 * e) & 255) * 256] += y[4 * sub + e];
+                        }
                     }
                 }
                 sf[m] = Mma<T>::pack(y);
             }
 #pragma unroll
             for (int t = 0; t < DT; ++t) {
-                const s16x8 kt = Tile<DP>::transposed(tile, 0, t, lane);
+                const s16x8 kf = tile.transposed(KT, t);
 #pragma unroll
-                for (int m = 0; m < MT; ++m) o[m][t] = Mma<T>::run(kt, sf[m], o[m][t]);
+                for (int m = 0; m < MT; ++m) o[m][t] = Mma<T>::run(kf, sf[m], o[m][t]);
             }
-            u = un;
+            j0 = jn;
+            mask = maskn;
         }
         if (tid == 0) scratch[1] = 0;
         __syncthreads();
         if (BIAS && plan.sums && turn == 0) {
+            // a row's 16 columns first: each 16 threads take a (bucket, 16 rows), starting
+            // at different columns so that the four of a wave lie in different banks
+            for (int e = tid / 16; e < MT * s.num_buckets; e += 16) {
+                float t = 0.0f;
+                for (int a = 0; a < 16; ++a) t += hist[e * 256 + (((a + e) & 15) << 4) + (tid & 15)];
+                hist[e * 256 + (tid & 15)] = t;   // read by this thread alone (column 0) up to here
+            }
+            __syncthreads();
             for (int e = tid; e < plan.span * s.num_buckets; e += 256) {
                 const int h = e / s.num_buckets, n = e % s.num_buckets;
                 float t = 0.0f;
-                for (int r = h; r < rows; r += plan.span) {
-                    const float *from = hist + ((r / 16) * s.num_buckets + n) * 256 + r % 16;
-                    for (int a = 0; a < 16; ++a) t += from[16 * a];
-                }
+                for (int r = h; r < rows; r += plan.span) t += hist[((r / 16) * s.num_buckets + n) * 256 + r % 16];
                 plan.sums[tile_id * plan.span * s.num_buckets + e] = t;
             }
             __syncthreads();
@@ -378,6 +401,7 @@ __global__ __launch_bounds__(256, 2) void k_grad_kv(AttnShape s, KeyPlan plan, S
             before += __shfl(sum, 63);
         }
     }
+    const Tile<DP> tile(lds, lane);
     // this wave's keys
     const int key = j0 + 16 * wave + col;
     s16x8 kf[KS], vf[KS];
@@ -428,8 +452,9 @@ __global__ __launch_bounds__(256, 2) void k_grad_kv(AttnShape s, KeyPlan plan, S
 #pragma unroll
             for (int n = 0; n < LD; ++n) {
                 const int e = n * 256 + tid;
-                *reinterpret_cast<s16x8 *>(Tile<DP>::chunk(lds + buf * 2 * TILE, e / CH, e % CH)) = qn[n];
-                *reinterpret_cast<s16x8 *>(Tile<DP>::chunk(lds + buf * 2 * TILE + TILE, e / CH, e % CH)) = dn[n];
+                char *to = lds + buf * 2 * TILE + Tile<DP>::chunk(e / CH, e % CH);
+                *reinterpret_cast<s16x8 *>(to) = qn[n];
+                *reinterpret_cast<s16x8 *>(to + TILE) = dn[n];
             }
             if (tid < 32)
 #pragma unroll
@@ -441,7 +466,7 @@ __global__ __launch_bounds__(256, 2) void k_grad_kv(AttnShape s, KeyPlan plan, S
             put(buf);
             __syncthreads();
             if (r0 + step < rows) fetch(r0 + step);
-            char *qt = lds + buf * 2 * TILE, *dt = qt + TILE;
+            const int qt = buf * 2 * TILE, dt = qt + TILE;
             const float *f = fig + buf * 5 * 32;
             float p[8], ds[8];
 #pragma unroll
@@ -450,8 +475,8 @@ __global__ __launch_bounds__(256, 2) void k_grad_kv(AttnShape s, KeyPlan plan, S
                 f32x4 x{}, dp{};
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    x = Mma<T>::run(*reinterpret_cast<s16x8 *>(Tile<DP>::chunk(qt, col, 4 * ks + quad) + 16 * m * DP * 2), kf[ks], x);
-                    dp = Mma<T>::run(*reinterpret_cast<s16x8 *>(Tile<DP>::chunk(dt, col, 4 * ks + quad) + 16 * m * DP * 2), vf[ks], dp);
+                    x = Mma<T>::run(tile.natural(qt, 16 * m, ks), kf[ks], x);
+                    dp = Mma<T>::run(tile.natural(dt, 16 * m, ks), vf[ks], dp);
                 }
                 const int at = 16 * m + 4 * quad;
                 const f32x4 shift = *reinterpret_cast<const f32x4 *>(f + at), delta = *reinterpret_cast<const f32x4 *>(f + 32 + at);
@@ -474,7 +499,7 @@ __global__ __launch_bounds__(256, 2) void k_grad_kv(AttnShape s, KeyPlan plan, S
 #pragma unroll
             for (int t = 0; t < DT; ++t) {
                 if (t % 2 == 0) __builtin_amdgcn_sched_barrier(0);   // else every fragment is read ahead and spilled
-                const s16x8 dtr = Tile<DP>::transposed(dt, 0, t, lane), qtr = Tile<DP>::transposed(qt, 0, t, lane);
+                const s16x8 dtr = tile.transposed(dt, t), qtr = tile.transposed(qt, t);
                 if (turn == 0) {
                     av[t] = Mma<T>::run(pf, dtr, av[t]);
                     ak[t] = Mma<T>::run(sf, qtr, ak[t]);

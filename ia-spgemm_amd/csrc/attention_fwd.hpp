@@ -9,16 +9,15 @@
 // takes every fourth piece of 32 keys and keeps its own running maximum, sum and
 // output (softmax in one pass), and the four meet once at the end.
 //
-// Per piece: S^T = K Q^T with K straight from memory into the matrix
-// instruction's registers (a lane holds 8 consecutive channels of one key) and
-// Q^T resident.  In S^T's result a lane holds one row and 2 x 4 keys, which is
+// Per piece: K and V go from memory through registers (the next piece's loads run
+// under this one's work) into the wave's own LDS tiles.  S^T = K Q^T with Q^T
+// resident in registers.  In S^T's result a lane holds one row and 2 x 4 keys, which is
 // just what the right operand of O^T += V^T P^T asks for, so P never leaves the
 // registers; it is rounded to the inputs' type for that product (off by half a
 // step relative to each probability, as the values are), everything else is
-// fp32.  V^T's fragments need the keys of one channel side by side: V goes
-// through a wave's own LDS tile and comes back by transposed reads.  The tile's
-// 32-byte columns are permuted by row, so that the 8 rows which half a wave
-// reads lie in 8 different groups of banks.
+// fp32.  V^T's fragments need the keys of one channel side by side: transposed
+// LDS reads.  The tiles' 32-byte columns are permuted by row, so that the 8 rows
+// which half a wave reads lie in 8 different groups of banks.
 #pragma once
 
 #include "attention_kernels.hpp"
@@ -60,20 +59,43 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 __device__ inline s16x8 load8(const uint16_t *p) { return *reinterpret_cast<const s16x8 *>(p); }
 
-// A tile of DP channels (16 bits) by rows in LDS, 32-byte columns permuted by row.
+// A tile of 32 rows by DP channels (16 bits) in LDS, 32-byte columns permuted by row:
+// column c of row r lies at c ^ mix(r).  Addresses are LDS offsets; all of one lane's
+// come from three by xor and constant offsets.
 template <int DP> struct Tile {
-    static constexpr int ROW = DP * 2;   // bytes
-    static __device__ int column(int row, int c) { return DP == 128 ? c ^ (row & 7) : c ^ ((row >> 1) & 3); }
-    // 16-byte chunk `c` of a row
-    static __device__ char *chunk(char *t, int row, int c) { return t + row * ROW + column(row, c >> 1) * 32 + (c & 1) * 16; }
-    // Fragment of the transposed tile: channel 16 * col + (lane & 15), keys
-    // row0 + 4 * (lane >> 4) + 0..3 and 16 more.
-    static __device__ s16x8 transposed(char *t, int row0, int col, int lane) {
-        typedef __attribute__((address_space(3))) s16x4 lds4;
-        const int r = row0 + 4 * (lane >> 4) + ((lane & 15) >> 2);
-        char *a = t + r * ROW + column(r, col) * 32 + (lane & 3) * 8;
+    typedef __attribute__((address_space(3))) s16x8 lds8;
+    typedef __attribute__((address_space(3))) s16x4 lds4;
+    static constexpr int ROW = DP * 2, BYTES = 32 * ROW, CH = DP / 8, N = 32 * CH / 64, STEP = 64 / CH;
+    static __device__ uint32_t mix(int row) { return DP == 128 ? row & 7 : (row >> 1) & 3; }
+    // 16-byte chunk c of a row
+    static __device__ uint32_t chunk(int row, int c) { return row * ROW + ((((uint32_t)c >> 1) ^ mix(row)) * 32) + (c & 1) * 16; }
+    static __device__ uint32_t offset(const char *lds) {
+        return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)lds;
+    }
+    uint32_t even, odd, nat, tr;
+    __device__ Tile(const char *lds, int lane) {
+        const uint32_t base = offset(lds);
+        even = base + chunk(lane / CH, lane % CH);
+        odd = base + chunk(STEP + lane / CH, lane % CH);   // mix has a period of 8 rows
+        const int r = 4 * (lane >> 4) + ((lane & 15) >> 2);
+        nat = base + chunk(lane & 15, lane >> 4);
+        tr = base + r * ROW + mix(r) * 32 + (lane & 3) * 8;
+    }
+    // A piece that lies in registers as Piece::load leaves it; `at`: a tile's offset from the lane's.
+    __device__ void fill(const s16x8 (&f)[N], int at) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            if (STEP == 8) *(lds8 *)(even + at + n * 8 * ROW) = f[n];
+            else *(lds8 *)((n % 2 ? odd : even) + at + n / 2 * 8 * ROW) = f[n];
+        }
+    }
+    // Fragment of the tile as it is: row row0 + (lane & 15), channels 32 * ks + 8 * (lane >> 4) + 0..7.
+    __device__ s16x8 natural(int at, int row0, int ks) const { return *(lds8 *)((nat ^ (ks * 64)) + at + row0 * ROW); }
+    // Fragment of the transposed tile: channel 16 * c + (lane & 15), rows 4 * (lane >> 4) + 0..3 and 16 more.
+    __device__ s16x8 transposed(int at, int c) const {
+        const uint32_t a = (tr ^ (c * 32)) + at;
         const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)a);
-        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(a + 16 * ROW));   // 16 rows on, the same columns
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(a + 16 * ROW));
         return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     }
 };
@@ -134,6 +156,65 @@ __device__ inline int block_union(const AttnShape &s, const int32_t *__restrict_
     return found;
 }
 
+// Maximum and sum over the four lanes that hold a row's keys (lanes 16 and 32 apart).
+__device__ inline float quad_max(float x) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ inline float quad_sum(float x) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+__device__ inline s16x8 negated(s16x8 x) { return x ^ (short)0x8000; }
+
+// A wave's way along the union: pieces of 32 keys, every fourth is its own.
+struct Walk {
+    int step, part, per;   // block of the union, piece of the block, pieces of a block
+    __device__ Walk(int start, int per_block) : step(start / per_block), part(start % per_block), per(per_block) {}
+    __device__ void on() {
+        for (part += 4; part >= per; part -= per) ++step;
+    }
+};
+
+// 32 rows of K or V at the piece j0, 64 consecutive 16-byte chunks of consecutive
+// rows at a time.  (A load straight into the matrix instruction's layout, 16 rows of
+// 64 bytes, costs the cache one access for each lane instead of one for four, and was
+// what bound the walk.)  Whole pieces take a scalar base and one 32-bit offset for
+// all loads; at a sequence's end, and for narrower heads, addresses are kept inside
+// and what is beyond becomes 0.
+template <int DP> struct Piece {
+    static constexpr int CH = DP / 8, N = 32 * CH / 64;
+    const uint16_t *base;
+    int64_t token;
+    uint32_t off;          // bytes
+    int lane, dim, last;   // last: row that may be read at most
+    __device__ Piece(const Side &x, int b, int g, int lane, int dim, int kl)
+        : base(x.at(b, 0, g)), token(x.token), lane(lane), dim(dim), last(kl - 1) {
+        off = (uint32_t)((lane / CH) * token * 2 + (lane % CH) * 16);
+    }
+    __device__ void load(s16x8 (&f)[N], int j0, int end) const {
+        if (j0 + 32 <= end && dim == DP) {
+            const uint16_t *row = base + j0 * token;
+#pragma unroll
+            for (int n = 0; n < N; ++n, row += token * (64 / CH))
+                f[n] = *reinterpret_cast<const s16x8 *>(reinterpret_cast<const char *>(row) + off);
+            return;
+        }
+        const int d = lane % CH * 8;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int j = j0 + n * (64 / CH) + lane / CH;
+            const s16x8 x = load8(base + min(j, last) * token + (d < dim ? d : 0));
+            f[n] = j < end && d < dim ? x : s16x8{};
+        }
+    }
+};
+
 struct RowPlan {
     int32_t nq, span, parts;   // queries and heads of a workgroup, workgroups of one query's heads
     int32_t tiles;     // per batch element and key head
@@ -147,7 +228,7 @@ struct RowPlan {
 // the lists, the rows' figures, the bias table.
 template <int DP, int MT> constexpr int attend_out_bytes() { return 4 * 16 * MT * (DP + 4) * 4; }
 inline size_t attend_lds(int dp, int mt, int nblocks, int most, int table) {
-    const size_t v = 4 * 32 * (size_t)dp * 2, o = 4 * 16 * (size_t)mt * (dp + 4) * 4;
+    const size_t v = 4 * 2 * 32 * (size_t)dp * 2, o = 4 * 16 * (size_t)mt * (dp + 4) * 4;
     return (v > o ? v : o) + 8 * (size_t)((nblocks + 31) / 32) + 8 * (size_t)most + 4 * 16 * (size_t)mt * 2 * 4 + 16 + 4 * (size_t)table;
 }
 
@@ -155,7 +236,7 @@ template <class T, int DP, int MT, bool BIAS>
 __global__ __launch_bounds__(256, 2) void k_attend(AttnShape s, RowPlan plan, Side q, Side k, Side v,
                                                 const int32_t *__restrict__ blocks, SideOut out, float *__restrict__ lse) {
     constexpr int R = 16 * MT, KS = DP / 32, DT = DP / 16, VL = 32 * DP * 2 / 1024, CH = DP / 8;
-    constexpr int AREA = attend_out_bytes<DP, MT>() > 4 * 32 * DP * 2 ? attend_out_bytes<DP, MT>() : 4 * 32 * DP * 2;
+    constexpr int AREA = attend_out_bytes<DP, MT>() > 4 * 2 * 32 * DP * 2 ? attend_out_bytes<DP, MT>() : 4 * 2 * 32 * DP * 2;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float *sums = reinterpret_cast<float *>(lds);                       // [4][R][DP + 4]
     float *stat = reinterpret_cast<float *>(lds + AREA);                // [4][R][2]
@@ -178,7 +259,8 @@ __global__ __launch_bounds__(256, 2) void k_attend(AttnShape s, RowPlan plan, Si
     if (i0 >= ql) return;
     const int nq = min(plan.nq, ql - (int)i0), rows = (nq - 1) * plan.span + min(plan.span, s.group - h0);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, col = lane & 15, quad = lane >> 4;
-    char *tile = lds + wave * 32 * DP * 2;
+    const Tile<DP> tile(lds + wave * 2 * Tile<DP>::BYTES, lane);   // K, then V
+    constexpr int KT = 0, VT = Tile<DP>::BYTES;
 
     if (BIAS)
         for (int e = tid; e < s.num_buckets * s.group; e += 256)
@@ -201,12 +283,18 @@ __global__ __launch_bounds__(256, 2) void k_attend(AttnShape s, RowPlan plan, Si
         for (int ks = 0; ks < KS; ++ks) {
             const int d = 32 * ks + 8 * quad;
             qf[m][ks] = there && d < s.dim ? load8(row + d) : s16x8{};
+            if (s.scale < 0.0f) qf[m][ks] = negated(qf[m][ks]);
         }
     }
     const int per_block = s.block / 32;
     const int share = (found + plan.splits - 1) / plan.splits;
-    const int u0 = min(found, split * share) * per_block, u1 = min(found, (split + 1) * share) * per_block;
-    const float c = BIAS ? s.scale : s.scale * LOG2E;
+    const int first = min(found, split * share), stop = min(found, (split + 1) * share);
+    // scores in units of log 2 where there is no bias; with one in its own units, so
+    // that a bias of the type's lowest value stays finite
+    const float c = fmaxf(fabsf(BIAS ? s.scale : s.scale * LOG2E), 1e-38f);
+    const float unit = BIAS ? LOG2E : 1.0f;
+    const int sure = s.causal ? min(kl, (int)i0 + kl - ql + 1) : kl;   // keys that every row may read
+    const Piece<DP> kp(k, b, g, lane, s.dim, kl), vp(v, b, g, lane, s.dim, kl);
 
     // turn 0: all queries together.  Zeros of P times infinities of V make NaN
     // in rows that do not read them: if anything in the result is not finite, each
@@ -223,108 +311,103 @@ __global__ __launch_bounds__(256, 2) void k_attend(AttnShape s, RowPlan plan, Si
 #pragma unroll
             for (int t = 0; t < DT; ++t) o[m][t] = f32x4{};
         }
-        s16x8 kf[2][KS], vf[VL];
-        auto at = [&](int u) { return __builtin_amdgcn_readfirstlane(ids[u / per_block]) * s.block + (u % per_block) * 32; };
-        auto chose = [&](int u) { return (uint32_t)__builtin_amdgcn_readfirstlane(masks[u / per_block]) & only; };
-        auto next = [&](int u) {   // the next piece of this wave that anyone here reads
-            while (u < u1 && !chose(u)) u += 4;
-            return u;
+        s16x8 kr[VL], vr[VL];
+        Walk at(first * per_block + wave, per_block);
+        auto skip = [&]() {   // to the next piece that anyone here reads
+            while (turn > 0 && at.step < stop && !(masks[at.step] & only)) at.on();
         };
-        auto fetch_k = [&](int u) {
-            const int j0 = at(u);
-#pragma unroll
-            for (int sub = 0; sub < 2; ++sub) {
-                const uint16_t *row = k.at(b, min(j0 + 16 * sub + col, kl - 1), g);
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    const int d = 32 * ks + 8 * quad;
-                    kf[sub][ks] = d < s.dim ? load8(row + d) : s16x8{};
-                }
-            }
-        };
-        auto fetch_v = [&](int u) {
-            const int j0 = at(u);
-            const int ch = lane % CH;
-#pragma unroll
-            for (int n = 0; n < VL; ++n) {
-                const int j = j0 + n * (64 / CH) + lane / CH;
-                vf[n] = j < vend && ch * 8 < s.dim ? load8(v.at(b, j, g) + ch * 8) : s16x8{};
-            }
-        };
-        int u = next(u0 + wave);
-        if (u < u1) {
-            fetch_k(u);
-            fetch_v(u);
+        skip();
+        int j0 = 0;
+        uint32_t mask = 0;
+        if (at.step < stop) {
+            j0 = __builtin_amdgcn_readfirstlane(ids[at.step]) * s.block + at.part * 32;
+            mask = __builtin_amdgcn_readfirstlane(masks[at.step]) & only;
+            kp.load(kr, j0, kl);
+            vp.load(vr, j0, vend);
         }
-        while (u < u1) {
-            const int j0 = at(u);
-            const uint32_t mask = chose(u);
-#pragma unroll
-            for (int n = 0; n < VL; ++n)
-                *reinterpret_cast<s16x8 *>(Tile<DP>::chunk(tile, n * (64 / CH) + lane / CH, lane % CH)) = vf[n];
+        while (at.step < stop) {
+            at.on();
+            skip();
+            const bool more = at.step < stop;
+            const int id = more ? ids[at.step] : 0;
+            const uint32_t chose = more ? masks[at.step] : 0;
+            tile.fill(kr, KT);
+            tile.fill(vr, VT);
             f32x4 x[MT][2];
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int sub = 0; sub < 2; ++sub) {
 #pragma unroll
-                for (int sub = 0; sub < 2; ++sub) {
-                    f32x4 acc{};
+                for (int m = 0; m < MT; ++m) x[m][sub] = f32x4{};
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) acc = Mma<T>::run(kf[sub][ks], qf[m][ks], acc);
-                    x[m][sub] = acc;
+                for (int ks = 0; ks < KS; ++ks) {
+                    const s16x8 kf = tile.natural(KT, 16 * sub, ks);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) x[m][sub] = Mma<T>::run(kf, qf[m][ks], x[m][sub]);
                 }
-            const int un = next(u + 4);
-            if (un < u1) {
-                fetch_k(un);
-                fetch_v(un);
             }
+            const int jn = __builtin_amdgcn_readfirstlane(id) * s.block + at.part * 32;
+            const uint32_t maskn = __builtin_amdgcn_readfirstlane(chose) & only;
+            if (more) {
+                kp.load(kr, jn, kl);
+                vp.load(vr, jn, vend);
+            }
+            const bool whole = j0 + 32 <= sure;
             s16x8 pf[MT];
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                const int lim = (mask >> qi[m] & 1u) ? end[m] - j0 - 4 * quad : INT32_MIN;
-                float y[8], big = -INFINITY;
+                const bool sel = mask >> qi[m] & 1u;
+                float y[8], big;
 #pragma unroll
                 for (int sub = 0; sub < 2; ++sub) {
                     uint32_t bucket = 0;
                     if (BIAS) __builtin_memcpy(&bucket, s.map + ((int64_t)j0 + 16 * sub + 4 * quad - pos[m] + s.k_len - 1), 4);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float t = x[m][sub][e] * c;
-                        if (BIAS) t += table[(bucket >> (8 * e) & 255) * s.group + hr[m]];
-                        t = 16 * sub + e < lim ? t : -INFINITY;
-                        y[4 * sub + e] = t;
-                        big = fmaxf(big, t);
+                        y[4 * sub + e] = x[m][sub][e];
+                        if (BIAS) y[4 * sub + e] = __builtin_fmaf(x[m][sub][e], c, table[(bucket >> (8 * e) & 255) * s.group + hr[m]]);
                     }
                 }
-                big = fmaxf(big, __shfl_xor(big, 16));
-                big = fmaxf(big, __shfl_xor(big, 32));
-                const float was = top[m], now = fmaxf(was, big), base = now == -INFINITY ? 0.0f : now;
-                if (__any(now > was)) {
-                    const float f = BIAS ? __builtin_amdgcn_exp2f((was - base) * LOG2E) : __builtin_amdgcn_exp2f(was - base);
+                if (!whole) {
+                    const int lim = end[m] - j0 - 4 * quad;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = 16 * (e / 4) + e % 4 < lim ? y[e] : -INFINITY;
+                }
+                big = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
+                big = quad_max(big);
+                if (!BIAS) big *= c;
+                big = sel ? big : -INFINITY;
+                // the maximum is moved only where it grew by so much that exponentials would
+                // get large (2^8): that is the first piece and hardly ever another
+                if (__any(big > top[m] + 8.0f / unit)) {
+                    const float now = fmaxf(top[m], big);
+                    const float f = __builtin_amdgcn_exp2f((top[m] - (now == -INFINITY ? 0.0f : now)) * unit);
                     sum[m] *= f;
 #pragma unroll
                     for (int t = 0; t < DT; ++t) o[m][t] *= f;
                     top[m] = now;
                 }
+                // a row that did not choose the block: exp(x - inf) = 0
+                const float shift = sel ? (top[m] == -INFINITY ? 0.0f : top[m]) : INFINITY;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    y[e] = BIAS ? __builtin_amdgcn_exp2f((y[e] - base) * LOG2E) : __builtin_amdgcn_exp2f(y[e] - base);
+                    y[e] = __builtin_amdgcn_exp2f(BIAS ? (y[e] - shift) * LOG2E : __builtin_fmaf(y[e], c, -shift));
                     sum[m] += y[e];
                 }
                 pf[m] = Mma<T>::pack(y);
             }
 #pragma unroll
             for (int t = 0; t < DT; ++t) {
-                const s16x8 vt = Tile<DP>::transposed(tile, 0, t, lane);
+                const s16x8 vf = tile.transposed(VT, t);
 #pragma unroll
-                for (int m = 0; m < MT; ++m) o[m][t] = Mma<T>::run(vt, pf[m], o[m][t]);
+                for (int m = 0; m < MT; ++m) o[m][t] = Mma<T>::run(vf, pf[m], o[m][t]);
             }
-            u = un;
+            j0 = jn;
+            mask = maskn;
         }
         // the waves meet
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            sum[m] += __shfl_xor(sum[m], 16);
-            sum[m] += __shfl_xor(sum[m], 32);
+            sum[m] = quad_sum(sum[m]);
             if (quad == 0) {
                 stat[(wave * R + m * 16 + col) * 2] = top[m];
                 stat[(wave * R + m * 16 + col) * 2 + 1] = sum[m];
@@ -332,7 +415,6 @@ __global__ __launch_bounds__(256, 2) void k_attend(AttnShape s, RowPlan plan, Si
         }
         if (tid == 0) scratch[1] = 0;
         __syncthreads();
-        const float unit = BIAS ? LOG2E : 1.0f;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             float all = -INFINITY;

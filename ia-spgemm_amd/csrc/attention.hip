@@ -134,9 +134,13 @@ ias_status bucket_map(const ias_attention *a, dev::AttnShape &s, uint8_t *map) {
 // How the walks share out the rows.  16 rows fill one matrix tile; 32 let more
 // queries share a walk and each fragment of K and V feed two tiles.  Few rows
 // (single tokens) are split along the walk until about every CU has two workgroups,
-// two blocks of keys each at least.
+// two blocks of keys each at least.  The chip holds two waves a SIMD, 2048, of these
+// kernels: a workgroup has as many waves as it takes to fill it, since a walk of one
+// wave has no end where waves wait for each other (8192 tokens, 8192 tiles, one block
+// of keys each: 148, 90 and 65 us with 4, 2 and 1 waves; 16 blocks 406, 343, 324 us;
+// 2048 tiles with their gradients: 417, 342, 364 us).
 struct Rows {
-    int mt, dp;
+    int mt, dp, waves;
     dev::RowPlan plan{};
     int64_t tiles, part, stat;   // all tiles; floats of the splits' results
     explicit Rows(const ias_attention *a, bool small = false) {
@@ -146,10 +150,13 @@ struct Rows {
         plan.span = std::min(group, 16 * mt);
         plan.parts = (int32_t)ceil_div(group, plan.span);
         plan.nq = plan.parts > 1 ? 1 : (int32_t)std::max<int64_t>(1, std::min<int64_t>(16 * mt / group, a->q_len));
+        // the union's list takes 8 bytes of LDS an entry
+        if (std::min<int64_t>((int64_t)plan.nq * a->keep, ceil_div(a->k_len, a->block)) > 2048) plan.nq = std::max(1, 2048 / a->keep);
         plan.tiles = (int32_t)ceil_div(a->q_len, plan.nq) * plan.parts;
         plan.most = (int32_t)std::max<int64_t>(1, std::min<int64_t>((int64_t)plan.nq * a->keep, ceil_div(a->k_len, a->block)));
         tiles = a->batch * a->k_heads * plan.tiles;
         plan.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({ceil_div(512, std::max<int64_t>(1, tiles)), ceil_div(plan.most, 2), 64}));
+        waves = plan.splits > 1 || tiles < 512 ? 4 : tiles < 4096 ? 2 : 1;
         part = plan.splits > 1 ? tiles * plan.splits * 16 * mt * dp : 0;
         stat = plan.splits > 1 ? tiles * plan.splits * 16 * mt * 2 : 0;
     }
@@ -241,19 +248,27 @@ ias_status select(const ias_attention *a, const ias_heads *q, const void *summar
     return select_rows<T, DP, 4>(a, s, p, 256, q, summary, blocks);
 }
 
-template <class T, int DP, int MT>
-ias_status attend_rows(const ias_attention *a, const dev::AttnShape &s, const ias_heads *q, const ias_heads *k,
+template <class T, int DP, int MT, int W>
+ias_status attend_waves(const ias_attention *a, const dev::AttnShape &s, const ias_heads *q, const ias_heads *k,
                        const ias_heads *v, const int32_t *blocks, const ias_heads *out, float *lse, const Rows &r) {
     const int64_t grid = ceil_div(r.tiles * r.plan.splits, 8) * 8;
-    const size_t lds = dev::attend_lds(DP, MT, s.nblocks, r.plan.most, s.num_buckets * s.group);
+    const size_t lds = dev::attend_lds(DP, MT, W, s.nblocks, r.plan.most, s.num_buckets * r.plan.span);
     if (a->table)
-        IAS_TRY(launch(dev::k_attend<T, DP, MT, true>, grid, 256, lds, a->stream, s, r.plan, side(q), side(k), side(v), blocks, side_out(out), lse));
+        IAS_TRY(launch(dev::k_attend<T, DP, MT, W, true>, grid, 64 * W, lds, a->stream, s, r.plan, side(q), side(k), side(v), blocks, side_out(out), lse));
     else
-        IAS_TRY(launch(dev::k_attend<T, DP, MT, false>, grid, 256, lds, a->stream, s, r.plan, side(q), side(k), side(v), blocks, side_out(out), lse));
+        IAS_TRY(launch(dev::k_attend<T, DP, MT, W, false>, grid, 64 * W, lds, a->stream, s, r.plan, side(q), side(k), side(v), blocks, side_out(out), lse));
     if (r.plan.splits > 1)
         IAS_TRY(launch(dev::k_attend_join<T>, r.tiles * r.plan.nq * r.plan.span, 64, 0, a->stream, s, r.plan, DP, 16 * MT,
                        a->table ? dev::LOG2E : 1.0f, side_out(out), lse));
     return IAS_SUCCESS;
+}
+
+template <class T, int DP, int MT>
+ias_status attend_rows(const ias_attention *a, const dev::AttnShape &s, const ias_heads *q, const ias_heads *k,
+                       const ias_heads *v, const int32_t *blocks, const ias_heads *out, float *lse, const Rows &r) {
+    return r.waves == 4   ? attend_waves<T, DP, MT, 4>(a, s, q, k, v, blocks, out, lse, r)
+           : r.waves == 2 ? attend_waves<T, DP, MT, 2>(a, s, q, k, v, blocks, out, lse, r)
+                          : attend_waves<T, DP, MT, 1>(a, s, q, k, v, blocks, out, lse, r);
 }
 
 template <class T>
@@ -267,18 +282,27 @@ ias_status attend(const ias_attention *a, const ias_heads *q, const ias_heads *k
     return r.mt == 1 ? attend_rows<T, 128, 1>(a, s, q, k, v, blocks, out, lse, r) : attend_rows<T, 128, 2>(a, s, q, k, v, blocks, out, lse, r);
 }
 
-template <class T, int DP, int MT>
-ias_status grad_rows(const ias_attention *a, const dev::AttnShape &s, const dev::GradPlan &p, const ias_heads *dout, const ias_heads *q,
-                     const ias_heads *k, const ias_heads *v, const ias_heads *out, const float *lse, const int32_t *blocks,
-                     const ias_heads *dq) {
+template <class T, int DP, int MT, int W>
+ias_status grad_waves(const ias_attention *a, const dev::AttnShape &s, const dev::GradPlan &p, const ias_heads *dout, const ias_heads *q,
+                      const ias_heads *k, const ias_heads *v, const ias_heads *out, const float *lse, const int32_t *blocks,
+                      const ias_heads *dq) {
     const int64_t tiles = a->batch * a->k_heads * p.tiles, grid = ceil_div(tiles, 8) * 8;
-    const size_t lds = dev::grad_q_lds(DP, MT, s.nblocks, p.most, s.group, s.num_buckets, p.sums);
-    const int32_t area = (int32_t)dev::grad_q_lds(DP, MT, 0, 0, s.group, s.num_buckets, p.sums) - 16 - 4 * s.group * s.num_buckets;
+    const int32_t area = dev::grad_q_area(DP, MT, W, s.num_buckets, p.sums);
+    const size_t lds = dev::grad_q_lds(area, s.nblocks, p.most, p.span, s.num_buckets);
     if (a->table)
-        return launch(dev::k_grad_q<T, DP, MT, true>, grid, 256, lds, a->stream, s, p, area, side(dout), side(q), side(k), side(v), side(out), lse,
+        return launch(dev::k_grad_q<T, DP, MT, W, true>, grid, 64 * W, lds, a->stream, s, p, area, side(dout), side(q), side(k), side(v), side(out), lse,
                       blocks, side_out(dq));
-    return launch(dev::k_grad_q<T, DP, MT, false>, grid, 256, lds, a->stream, s, p, area, side(dout), side(q), side(k), side(v), side(out), lse, blocks,
+    return launch(dev::k_grad_q<T, DP, MT, W, false>, grid, 64 * W, lds, a->stream, s, p, area, side(dout), side(q), side(k), side(v), side(out), lse, blocks,
                   side_out(dq));
+}
+
+template <class T, int DP, int MT>
+ias_status grad_rows(const ias_attention *a, const dev::AttnShape &s, const dev::GradPlan &p, int waves, const ias_heads *dout,
+                     const ias_heads *q, const ias_heads *k, const ias_heads *v, const ias_heads *out, const float *lse,
+                     const int32_t *blocks, const ias_heads *dq) {
+    return waves == 4   ? grad_waves<T, DP, MT, 4>(a, s, p, dout, q, k, v, out, lse, blocks, dq)
+           : waves == 2 ? grad_waves<T, DP, MT, 2>(a, s, p, dout, q, k, v, out, lse, blocks, dq)
+                        : grad_waves<T, DP, MT, 1>(a, s, p, dout, q, k, v, out, lse, blocks, dq);
 }
 
 template <class T, int DP>
@@ -292,8 +316,8 @@ ias_status grad_all(const ias_attention *a, const ias_heads *dout, const ias_hea
     const int64_t bh = a->batch * a->k_heads;
     if (bh > 0 && a->q_len > 0) {
         const int mt = w.rows.mt;
-        if (mt == 1) IAS_TRY((grad_rows<T, DP, 1>(a, s, p, dout, q, k, v, out, lse, blocks, dq)));
-        else IAS_TRY((grad_rows<T, DP, 2>(a, s, p, dout, q, k, v, out, lse, blocks, dq)));
+        if (mt == 1) IAS_TRY((grad_rows<T, DP, 1>(a, s, p, w.rows.waves, dout, q, k, v, out, lse, blocks, dq)));
+        else IAS_TRY((grad_rows<T, DP, 2>(a, s, p, w.rows.waves, dout, q, k, v, out, lse, blocks, dq)));
     }
     if (w.k.entries > 0) {
         IAS_TRY(launch(dev::k_clear, ceil_div(w.k.entries, 256), 256, 0, a->stream, w.k.entries, w.count));

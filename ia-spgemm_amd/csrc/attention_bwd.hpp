@@ -22,19 +22,22 @@ struct GradPlan {
 
 // LDS of k_grad_q: the waves' K and V tiles and the lanes' sums by bucket, over which
 // the end's sums are laid; the lists; the bias table.
-inline size_t grad_q_lds(int dp, int mt, int nblocks, int most, int group, int buckets, bool sums) {
-    const size_t v = 4 * 2 * 32 * (size_t)dp * 2 + (sums ? (size_t)mt * buckets * 256 * 4 : 0), o = 4 * 16 * (size_t)mt * (dp + 4) * 4;
-    return (v > o ? v : o) + 8 * (size_t)((nblocks + 31) / 32) + 8 * (size_t)most + 16 + 4 * (size_t)group * buckets;
+inline int grad_q_area(int dp, int mt, int waves, int buckets, bool sums) {
+    const int v = waves * 2 * 32 * dp * 2 + (sums ? mt * buckets * 64 * waves * 4 : 0), o = walk_area(dp, mt, waves);
+    return v > o ? v : o;
+}
+inline size_t grad_q_lds(int area, int nblocks, int most, int span, int buckets) {
+    return area + 8 * (size_t)((nblocks + 31) / 32) + 8 * (size_t)most + 16 + 4 * (size_t)span * buckets;
 }
 
-template <class T, int DP, int MT, bool BIAS>
-__global__ __launch_bounds__(256, 2) void k_grad_q(AttnShape s, GradPlan plan, int32_t area, Side dout, Side q, Side k,
+template <class T, int DP, int MT, int W, bool BIAS>
+__global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan, int32_t area, Side dout, Side q, Side k,
                                                                  Side v, Side out, const float *__restrict__ lse,
                                                                  const int32_t *__restrict__ blocks, SideOut dq) {
-    constexpr int R = 16 * MT, KS = DP / 32, DT = DP / 16, CH = DP / 8;
+    constexpr int THREADS = 64 * W, R = 16 * MT, KS = DP / 32, DT = DP / 16, CH = DP / 8;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    float *sums = reinterpret_cast<float *>(lds);                           // [4][R][DP + 4], at the end
-    float *hist = reinterpret_cast<float *>(lds + 4 * 2 * 32 * DP * 2);       // [MT][buckets][256]
+    float *sums = reinterpret_cast<float *>(lds);                           // [W][R][DP + 4], at the end
+    float *hist = reinterpret_cast<float *>(lds + W * 2 * Tile<DP>::BYTES);   // [MT][buckets][64 W]
     int32_t *scratch = reinterpret_cast<int32_t *>(lds + area);             // total, flag
     int32_t *ids = scratch + 4;
     uint32_t *masks = reinterpret_cast<uint32_t *>(ids + plan.most);
@@ -52,7 +55,7 @@ __global__ __launch_bounds__(256, 2) void k_grad_q(AttnShape s, GradPlan plan, i
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, col = lane & 15, quad = lane >> 4;
     if (i0 >= ql) {
         if (BIAS && plan.sums)
-            for (int e = tid; e < plan.span * s.num_buckets; e += 256) plan.sums[tile_id * plan.span * s.num_buckets + e] = 0.0f;
+            for (int e = tid; e < plan.span * s.num_buckets; e += THREADS) plan.sums[tile_id * plan.span * s.num_buckets + e] = 0.0f;
         return;
     }
     const int nq = min(plan.nq, ql - (int)i0), rows = (nq - 1) * plan.span + min(plan.span, s.group - h0);
@@ -60,10 +63,10 @@ __global__ __launch_bounds__(256, 2) void k_grad_q(AttnShape s, GradPlan plan, i
     constexpr int KT = 0, VT = Tile<DP>::BYTES;
 
     if (BIAS) {
-        for (int e = tid; e < s.num_buckets * s.group; e += 256)
-            table[e] = T::up(s.table[(e / s.group) * s.q_heads + g * s.group + e % s.group]);
+        for (int e = tid; e < s.num_buckets * plan.span; e += THREADS)
+            if (h0 + e % plan.span < s.group) table[e] = T::up(s.table[(e / plan.span) * s.q_heads + g * s.group + h0 + e % plan.span]);
         if (plan.sums)
-            for (int e = tid; e < MT * s.num_buckets * 256; e += 256) hist[e] = 0.0f;
+            for (int e = tid; e < MT * s.num_buckets * THREADS; e += THREADS) hist[e] = 0.0f;
     }
     const int found = __builtin_amdgcn_readfirstlane(block_union(s, blocks, b, g, i0, nq, ql, kl, words, ids, masks, scratch));
 
@@ -114,7 +117,7 @@ __global__ __launch_bounds__(256, 2) void k_grad_q(AttnShape s, GradPlan plan, i
 #pragma unroll
             for (int t = 0; t < DT; ++t) o[m][t] = f32x4{};
         s16x8 kr[Piece<DP>::N], vr[Piece<DP>::N];
-        Walk at(wave, per_block);
+        Walk<W> at(wave, per_block);
         auto skip = [&]() {
             while (turn > 0 && at.step < found && !(masks[at.step] & only)) at.on();
         };
@@ -171,7 +174,7 @@ __global__ __launch_bounds__(256, 2) void k_grad_q(AttnShape s, GradPlan plan, i
                     for (int e = 0; e < 4; ++e) {
                         float p;
                         if (BIAS)
-                            p = __builtin_amdgcn_exp2f((__builtin_fmaf(x[m][sub][e], c, table[(bucket[sub] >> (8 * e) & 255) * s.group + hr[m]]) - off) * LOG2E);
+                            p = __builtin_amdgcn_exp2f((__builtin_fmaf(x[m][sub][e], c, table[(bucket[sub] >> (8 * e) & 255) * plan.span + hr[m] - h0]) - off) * LOG2E);
                         else
                             p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[m][sub][e], c, -off));
                         y[4 * sub + e] = p * (dp[m][sub][e] - delta[m]);
@@ -186,7 +189,7 @@ __global__ __launch_bounds__(256, 2) void k_grad_q(AttnShape s, GradPlan plan, i
                     // Each lane has a column of its own, so plain sums do, in the walk's order (an
                     // atomic LDS add takes some 200 cycles a wave).  Far keys share a bucket, mostly
                     // for a whole wave: then their sum goes in at once.
-                    float *mine = hist + m * s.num_buckets * 256 + tid;
+                    float *mine = hist + m * s.num_buckets * THREADS + tid;
                     if (!sel)
 #pragma unroll
                         for (int e = 0; e < 8; ++e) y[e] = 0.0f;
@@ -194,10 +197,10 @@ __global__ __launch_bounds__(256, 2) void k_grad_q(AttnShape s, GradPlan plan, i
                     for (int sub = 0; sub < 2; ++sub) {
                         const uint32_t n = bucket[sub] & 255;
                         if (__all(bucket[sub] == n * 0x01010101u)) {
-                            mine[n * 256] += (y[4 * sub] + y[4 * sub + 1]) + (y[4 * sub + 2] + y[4 * sub + 3]);
+                            mine[n * THREADS] += (y[4 * sub] + y[4 * sub + 1]) + (y[4 * sub + 2] + y[4 * sub + 3]);
                         } else {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) mine[(bucket[sub] >> (8 * e) & 255) * 256] += y[4 * sub + e];
+                            for (int e = 0; e < 4; ++e) mine[(bucket[sub] >> (8 * e) & 255) * THREADS] += y[4 * sub + e];
                         }
                     }
                 }
@@ -215,18 +218,18 @@ __global__ __launch_bounds__(256, 2) void k_grad_q(AttnShape s, GradPlan plan, i
         if (tid == 0) scratch[1] = 0;
         __syncthreads();
         if (BIAS && plan.sums && turn == 0) {
-            // a row's 16 columns first: each 16 threads take a (bucket, 16 rows), starting
-            // at different columns so that the four of a wave lie in different banks
-            for (int e = tid / 16; e < MT * s.num_buckets; e += 16) {
+            // a row's 4 W columns first: each 16 threads take a (bucket, 16 rows), starting at
+            // different columns so that the four of a wave lie in different banks
+            for (int e = tid / 16; e < MT * s.num_buckets; e += 4 * W) {
                 float t = 0.0f;
-                for (int a = 0; a < 16; ++a) t += hist[e * 256 + (((a + e) & 15) << 4) + (tid & 15)];
-                hist[e * 256 + (tid & 15)] = t;   // read by this thread alone (column 0) up to here
+                for (int a = 0; a < 4 * W; ++a) t += hist[e * THREADS + (((a + e) & (4 * W - 1)) << 4) + (tid & 15)];
+                hist[e * THREADS + (tid & 15)] = t;   // read by this thread alone (column 0) up to here
             }
             __syncthreads();
-            for (int e = tid; e < plan.span * s.num_buckets; e += 256) {
+            for (int e = tid; e < plan.span * s.num_buckets; e += THREADS) {
                 const int h = e / s.num_buckets, n = e % s.num_buckets;
                 float t = 0.0f;
-                for (int r = h; r < rows; r += plan.span) t += hist[((r / 16) * s.num_buckets + n) * 256 + r % 16];
+                for (int r = h; r < rows; r += plan.span) t += hist[((r / 16) * s.num_buckets + n) * THREADS + r % 16];
                 plan.sums[tile_id * plan.span * s.num_buckets + e] = t;
             }
             __syncthreads();
@@ -238,13 +241,13 @@ __global__ __launch_bounds__(256, 2) void k_grad_q(AttnShape s, GradPlan plan, i
                 *reinterpret_cast<f32x4 *>(sums + (wave * R + m * 16 + col) * (DP + 4) + 16 * t + 4 * quad) = o[m][t];
         __syncthreads();
         bool fine = true;
-        for (int e = tid; e < R * CH; e += 256) {
+        for (int e = tid; e < R * CH; e += THREADS) {
             const int r = e / CH, ch = e % CH;
             if (r >= rows || ch * 8 >= s.dim) continue;
             const int rq = r / plan.span;
             if (!(only >> rq & 1u)) continue;
             float y[8] = {};
-            for (int n = 0; n < 4; ++n)
+            for (int n = 0; n < W; ++n)
 #pragma unroll
                 for (int d = 0; d < 8; ++d) y[d] += sums[(n * R + r) * (DP + 4) + ch * 8 + d];
 #pragma unroll

@@ -172,12 +172,12 @@ __device__ inline float quad_sum(float x) {
 
 __device__ inline s16x8 negated(s16x8 x) { return x ^ (short)0x8000; }
 
-// A wave's way along the union: pieces of 32 keys, every fourth is its own.
-struct Walk {
+// A wave's way along the union: pieces of 32 keys, every W-th is its own.
+template <int W> struct Walk {
     int step, part, per;   // block of the union, piece of the block, pieces of a block
     __device__ Walk(int start, int per_block) : step(start / per_block), part(start % per_block), per(per_block) {}
     __device__ void on() {
-        for (part += 4; part >= per; part -= per) ++step;
+        for (part += W; part >= per; part -= per) ++step;
     }
 };
 
@@ -226,21 +226,22 @@ struct RowPlan {
 
 // LDS of k_attend: the end's sums (the waves' V tiles lie in the same place),
 // the lists, the rows' figures, the bias table.
-template <int DP, int MT> constexpr int attend_out_bytes() { return 4 * 16 * MT * (DP + 4) * 4; }
-inline size_t attend_lds(int dp, int mt, int nblocks, int most, int table) {
-    const size_t v = 4 * 2 * 32 * (size_t)dp * 2, o = 4 * 16 * (size_t)mt * (dp + 4) * 4;
-    return (v > o ? v : o) + 8 * (size_t)((nblocks + 31) / 32) + 8 * (size_t)most + 4 * 16 * (size_t)mt * 2 * 4 + 16 + 4 * (size_t)table;
+constexpr int walk_area(int dp, int mt, int waves) {
+    return waves * (2 * 32 * dp * 2 > 16 * mt * (dp + 4) * 4 ? 2 * 32 * dp * 2 : 16 * mt * (dp + 4) * 4);
+}
+inline size_t attend_lds(int dp, int mt, int waves, int nblocks, int most, int table) {
+    return walk_area(dp, mt, waves) + 8 * (size_t)((nblocks + 31) / 32) + 8 * (size_t)most + waves * 16 * (size_t)mt * 2 * 4 + 16 + 4 * (size_t)table;
 }
 
-template <class T, int DP, int MT, bool BIAS>
-__global__ __launch_bounds__(256, 2) void k_attend(AttnShape s, RowPlan plan, Side q, Side k, Side v,
+template <class T, int DP, int MT, int W, bool BIAS>
+__global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan, Side q, Side k, Side v,
                                                 const int32_t *__restrict__ blocks, SideOut out, float *__restrict__ lse) {
-    constexpr int R = 16 * MT, KS = DP / 32, DT = DP / 16, VL = 32 * DP * 2 / 1024, CH = DP / 8;
-    constexpr int AREA = attend_out_bytes<DP, MT>() > 4 * 2 * 32 * DP * 2 ? attend_out_bytes<DP, MT>() : 4 * 2 * 32 * DP * 2;
+    constexpr int R = 16 * MT, KS = DP / 32, DT = DP / 16, VL = Tile<DP>::N, CH = DP / 8;
+    constexpr int AREA = walk_area(DP, MT, W);
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    float *sums = reinterpret_cast<float *>(lds);                       // [4][R][DP + 4]
-    float *stat = reinterpret_cast<float *>(lds + AREA);                // [4][R][2]
-    int32_t *scratch = reinterpret_cast<int32_t *>(stat + 4 * R * 2);   // total, flag
+    float *sums = reinterpret_cast<float *>(lds);                       // [W][R][DP + 4]
+    float *stat = reinterpret_cast<float *>(lds + AREA);                // [W][R][2]
+    int32_t *scratch = reinterpret_cast<int32_t *>(stat + W * R * 2);   // total, flag
     int32_t *ids = scratch + 4;
     uint32_t *masks = reinterpret_cast<uint32_t *>(ids + plan.most);
     uint32_t *words = masks + plan.most;
@@ -263,8 +264,8 @@ __global__ __launch_bounds__(256, 2) void k_attend(AttnShape s, RowPlan plan, Si
     constexpr int KT = 0, VT = Tile<DP>::BYTES;
 
     if (BIAS)
-        for (int e = tid; e < s.num_buckets * s.group; e += 256)
-            table[e] = T::up(s.table[(e / s.group) * s.q_heads + g * s.group + e % s.group]);
+        for (int e = tid; e < s.num_buckets * plan.span; e += 64 * W)
+            if (h0 + e % plan.span < s.group) table[e] = T::up(s.table[(e / plan.span) * s.q_heads + g * s.group + h0 + e % plan.span]);
     const int found = __builtin_amdgcn_readfirstlane(block_union(s, blocks, b, g, i0, nq, ql, kl, words, ids, masks, scratch));
 
     // this lane's rows
@@ -312,7 +313,7 @@ __global__ __launch_bounds__(256, 2) void k_attend(AttnShape s, RowPlan plan, Si
             for (int t = 0; t < DT; ++t) o[m][t] = f32x4{};
         }
         s16x8 kr[VL], vr[VL];
-        Walk at(first * per_block + wave, per_block);
+        Walk<W> at(first * per_block + wave, per_block);
         auto skip = [&]() {   // to the next piece that anyone here reads
             while (turn > 0 && at.step < stop && !(masks[at.step] & only)) at.on();
         };
@@ -364,7 +365,7 @@ __global__ __launch_bounds__(256, 2) void k_attend(AttnShape s, RowPlan plan, Si
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         y[4 * sub + e] = x[m][sub][e];
-                        if (BIAS) y[4 * sub + e] = __builtin_fmaf(x[m][sub][e], c, table[(bucket >> (8 * e) & 255) * s.group + hr[m]]);
+                        if (BIAS) y[4 * sub + e] = __builtin_fmaf(x[m][sub][e], c, table[(bucket >> (8 * e) & 255) * plan.span + hr[m] - h0]);
                     }
                 }
                 if (!whole) {
@@ -418,7 +419,7 @@ __global__ __launch_bounds__(256, 2) void k_attend(AttnShape s, RowPlan plan, Si
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             float all = -INFINITY;
-            for (int n = 0; n < 4; ++n) all = fmaxf(all, stat[(n * R + m * 16 + col) * 2]);
+            for (int n = 0; n < W; ++n) all = fmaxf(all, stat[(n * R + m * 16 + col) * 2]);
             const float f = top[m] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((top[m] - all) * unit);
 #pragma unroll
             for (int t = 0; t < DT; ++t) {
@@ -429,14 +430,14 @@ __global__ __launch_bounds__(256, 2) void k_attend(AttnShape s, RowPlan plan, Si
         }
         __syncthreads();
         bool fine = true;
-        for (int e = tid; e < R * CH; e += 256) {
+        for (int e = tid; e < R * CH; e += 64 * W) {
             const int r = e / CH, ch = e % CH;
             if (r >= rows || ch * 8 >= s.dim) continue;
             const int rq = r / plan.span;
             if (!(only >> rq & 1u)) continue;
             float all = -INFINITY, l = 0.0f, y[8] = {};
-            for (int n = 0; n < 4; ++n) all = fmaxf(all, stat[(n * R + r) * 2]);
-            for (int n = 0; n < 4; ++n) {
+            for (int n = 0; n < W; ++n) all = fmaxf(all, stat[(n * R + r) * 2]);
+            for (int n = 0; n < W; ++n) {
                 const float m = stat[(n * R + r) * 2], x = stat[(n * R + r) * 2 + 1];
                 if (m != -INFINITY || x != x) l += x * __builtin_amdgcn_exp2f((m - all) * unit);
 #pragma unroll

@@ -115,6 +115,19 @@ def test_forward_and_gradients(A, c):
 
 
 @gpu
+@pytest.mark.parametrize("c", [
+    # the longest lists and tables that a workgroup holds
+    case(sq=40, sk=19200, hq=1, hkv=1, d=128, keep=256, nb=32),
+    case("fp16", sq=9, sk=16390, hq=64, hkv=1, d=128, keep=256, nb=64),
+    # many short walks (one wave each), and a few (two)
+    case(b=2, sq=2100, sk=130, hq=8, hkv=4, d=64, keep=2, nb=8),
+    case("fp16", b=3, sq=500, sk=500, hq=8, hkv=8, d=128, keep=6, q_lens=[500, 499, 3], k_lens=[400, 499, 500]),
+], ids=names)
+def test_limits_and_shares(A, c):
+    check(A, c, make(c, 14))
+
+
+@gpu
 @pytest.mark.parametrize("layout", ["packed", "bhsd"])
 def test_strides(A, layout):
     c = case(b=2, sq=90, sk=200, hq=4, hkv=2, d=64, nb=8)
@@ -422,7 +435,9 @@ def test_addresses_and_strides_are_refused():
         for bad, status in ((None, INVALID), (ias.Heads(None, 1024, 256, 64), INVALID),
                             (ias.Heads((1 << 20) + 8, 1024, 256, 64), UNSUPPORTED),
                             (ias.Heads(1 << 20, 1024, 258, 64), UNSUPPORTED),
-                            (ias.Heads(1 << 20, 1024, 256, 60), UNSUPPORTED)):
+                            (ias.Heads(1 << 20, 1024, 256, 60), UNSUPPORTED),
+                            (ias.Heads(1 << 20, 1 << 30, (1 << 24) + 8, 64), UNSUPPORTED),
+                            (ias.Heads(1 << 20, 1 << 30, -256, 64), UNSUPPORTED)):
             assert _call("grad", heads={n: bad}) == status, n
     # nothing to do is done without an address
     assert _call("attend", q_len=0, blocks=None, heads={n: ias.Heads(None, 0, 0, 0) for n in ("q", "out")}) == 0

@@ -8,6 +8,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace ias {
 namespace {
@@ -53,43 +54,123 @@ __device__ inline int bucket_of(int64_t d, const int32_t *edges, int nb) {
     return lo;
 }
 
+constexpr int V = 8;         // consecutive values of a thread of k_rel_bias
+constexpr int HEADS = 16;    // heads of a workgroup
+constexpr int E = 2;         // neighbouring diagonals of a thread of k_rel_bias_grad
+constexpr int SPAN = 256 * E;
+
+// out[h][i][j] = table[bucket(j - i - shift)][h].  A thread has 8 consecutive values
+// of one matrix (counted through its rows) and writes them for 16 heads: their
+// buckets are found once, by one search and steps from edge to edge, and a head costs
+// 8 reads of the table in LDS and one 16-byte store (32 for f32).  Bound by the
+// stores: 2048 x 2048, 16 heads, bf16, 134 MB.
 template <class T>
 __global__ __launch_bounds__(256) void k_rel_bias(int32_t heads, int64_t q_len, int64_t k_len, int32_t nb,
                                                   const T *__restrict__ table, const int32_t *__restrict__ edges,
                                                   T *__restrict__ out) {
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (e >= q_len * k_len) return;
-    const int64_t i = e / k_len, j = e % k_len;
-    const int n = bucket_of(j - i - (k_len - q_len), edges, nb);
-    for (int h = 0; h < heads; ++h) out[h * q_len * k_len + e] = table[n * heads + h];
-}
-
-// Rows of one head, each lane's sums by bucket in its own column of LDS.
-template <class T>
-__global__ __launch_bounds__(64) void k_rel_bias_grad(int64_t batch, int32_t heads, int64_t q_len, int64_t k_len,
-                                                      int32_t nb, const T *__restrict__ grad, int64_t sb, int64_t sh,
-                                                      int64_t sr, const int32_t *__restrict__ edges,
-                                                      int32_t per, float *__restrict__ part) {
-    extern __shared__ float hist[];   // nb x 64
+    typedef uint32_t Packed __attribute__((ext_vector_type(sizeof(T) * V / 4), aligned(sizeof(T))));
+    __shared__ T ts[64 * HEADS];
     __shared__ int32_t es[64];
-    const int lane = threadIdx.x, h = blockIdx.x % heads;
-    const int64_t chunk = blockIdx.x / heads, rows = batch * q_len;
-    if (lane < nb - 1) es[lane] = edges[lane];
-    for (int n = 0; n < nb; ++n) hist[n * 64 + lane] = 0.0f;
+    const int h0 = blockIdx.y * HEADS, hn = min(HEADS, heads - h0);
+    for (int e = threadIdx.x; e < nb * HEADS; e += 256)
+        if (e % HEADS < hn) ts[e] = table[(e / HEADS) * heads + h0 + e % HEADS];
+    if ((int)threadIdx.x < nb - 1) es[threadIdx.x] = edges[threadIdx.x];
     __syncthreads();
-    for (int64_t r = chunk * per; r < min(rows, (chunk + 1) * per); ++r) {
-        const int64_t b = r / q_len, i = r % q_len;
-        const T *x = grad + b * sb + h * sh + i * sr;
-        for (int64_t j = lane; j < k_len; j += 64) hist[bucket_of(j - i - (k_len - q_len), es, nb) * 64 + lane] += up(x[j]);
+    const int64_t size = q_len * k_len, e0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
+    if (e0 >= size) return;
+    const int64_t i = e0 / k_len;
+    int64_t j = e0 - i * k_len, d = j - i - (k_len - q_len);
+    int at[V], n = bucket_of(d, es, nb);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        at[v] = n * HEADS;
+        if (++j < k_len) {
+            ++d;
+            while (n < nb - 1 && es[n] <= d) ++n;
+        } else {   // on to the next row
+            j = 0;
+            d -= k_len;
+            n = bucket_of(d, es, nb);
+        }
     }
-    __syncthreads();
-    if (lane < nb) {
-        float t = 0.0f;
-        for (int n = 0; n < 64; ++n) t += hist[lane * 64 + n];
-        part[(chunk * heads + h) * nb + lane] = t;
+    for (int h = 0; h < hn; ++h) {
+        alignas(16) T y[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) y[v] = ts[at[v] + h];
+        T *to = out + (h0 + h) * size + e0;
+        if (e0 + V <= size) {
+            *reinterpret_cast<Packed *>(to) = *reinterpret_cast<Packed *>(y);   // vector stores, whatever their alignment
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (e0 + v < size) to[v] = y[v];
+        }
     }
 }
 
+// Sums over diagonals.  A thread has 2 neighbouring diagonals and goes down some rows
+// of every batch element, its loads moving one to the right with each row: the sums
+// stay in registers, and buckets matter only at the end, where each is one stretch of
+// the workgroup's 512 diagonals.  part: [chunk][head][bucket].  Bound by the read of
+// the gradient.
+template <class T>
+__global__ __launch_bounds__(256) void k_rel_bias_grad(int64_t batch, int32_t heads, int64_t q_len, int64_t k_len,
+                                                       int32_t nb, const T *__restrict__ grad, int64_t sb, int64_t sh,
+                                                       int64_t sr, const int32_t *__restrict__ edges, int32_t spans,
+                                                       int32_t rows, float *__restrict__ part) {
+    __shared__ float sums[SPAN];
+    __shared__ int32_t es[64];
+    const int tid = threadIdx.x, h = blockIdx.x % heads;
+    const int64_t chunk = blockIdx.x / heads;
+    const int64_t r0 = chunk / spans * rows, r1 = min(q_len, r0 + rows);
+    // column of the thread's first diagonal in row i: c0 + i
+    const int64_t first = chunk % spans * SPAN - (q_len - 1), c0 = first + tid * E;
+    if (tid < nb - 1) es[tid] = edges[tid];
+    float acc[E] = {};
+    // rows where both columns are there, and those beside them where one is
+    const int64_t ia = max(r0, -c0), ib = min(r1, k_len - E + 1 - c0);
+    for (int64_t b = 0; b < batch; ++b) {
+        const T *x = grad + b * sb + h * sh + c0;
+        int64_t i = ia;
+        auto rows_down = [&](auto some) {   // rows whose loads are in flight together
+            constexpr int U = decltype(some)::value;
+            for (; i + U <= ib; i += U) {
+                T y[U][E];
+#pragma unroll
+                for (int u = 0; u < U; ++u) __builtin_memcpy(y[u], x + (i + u) * (sr + 1), sizeof y[u]);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[e] += up(y[u][e]);
+            }
+        };
+        rows_down(std::integral_constant<int, 8>{});
+        rows_down(std::integral_constant<int, 2>{});
+        rows_down(std::integral_constant<int, 1>{});
+        for (int side = 0; side < 2; ++side) {
+            const int64_t from = side ? max(r0, max(ia, ib)) : max(r0, -c0 - (E - 1)), to = side ? min(r1, k_len - c0) : min(min(r1, ia), k_len - c0);
+            for (int64_t n = from; n < to; ++n)
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (c0 + n + e >= 0 && c0 + n + e < k_len) acc[e] += up(x[n * (sr + 1) + e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) sums[tid * E + e] = acc[e];
+    __syncthreads();
+    // bucket n is the stretch of diagonals from edge n - 1 to edge n
+    const int lane = tid % 64;
+    const int64_t d0 = first - (k_len - q_len);   // distance of the first diagonal
+    for (int n = tid / 64; n < nb; n += 4) {
+        const int64_t lo = n == 0 ? 0 : max((int64_t)0, es[n - 1] - d0), hi = n == nb - 1 ? SPAN : min((int64_t)SPAN, es[n] - d0);
+        float t = 0.0f;
+        for (int64_t k = lo + lane; k < hi; k += 64) t += sums[k];
+        for (int d = 32; d; d >>= 1) t += __shfl_xor(t, d);
+        if (lane == 0) part[(chunk * heads + h) * nb + n] = t;
+    }
+}
+
+// dtable[n][h]: one wave for each, in a fixed order.
 template <class T>
 __global__ __launch_bounds__(64) void k_rel_bias_sum(int64_t chunks, int32_t heads, int32_t nb,
                                                      const float *__restrict__ part, T *__restrict__ dtable) {
@@ -112,14 +193,25 @@ ias_status check_bias(int32_t dtype, int64_t batch, int32_t heads, int64_t q_len
         REFUSE(IAS_ERROR_INVALID_ARGUMENT, "batch %lld, heads %d, q_len %lld, k_len %lld, device %d", (long long)batch, heads,
                (long long)q_len, (long long)k_len, device);
     if (nb < 1 || nb > 64) REFUSE(IAS_ERROR_UNSUPPORTED, "%d buckets: 1 to 64", nb);
-    if (batch > INT32_MAX || q_len > INT32_MAX / 2 || k_len > INT32_MAX / 2 ||
-        (q_len > 0 && batch * heads > INT64_MAX / 16 / q_len / std::max<int64_t>(1, k_len)))
+    if (batch > INT32_MAX || heads > 1 << 20 || q_len > 1 << 24 || k_len > 1 << 24 ||
+        (q_len > 0 && k_len > (1ll << 41) / q_len) || (q_len > 0 && batch * heads > INT64_MAX / 16 / q_len / std::max<int64_t>(1, k_len)))
         REFUSE(IAS_ERROR_OVERFLOW, "batch x heads x q_len x k_len is too large");
     return IAS_SUCCESS;
 }
 
-constexpr int ROWS = 16;   // rows of a workgroup of the gradient
-int64_t chunks_of(int64_t batch, int64_t q_len) { return ceil_div(batch * q_len, ROWS); }
+// How the gradient is shared out: spans of 512 diagonals, and so many rows that
+// about 4096 workgroups are there (half of them hold corners outside the matrix), 16
+// at least (each ends in sums of its own).
+struct Chunks {
+    int64_t spans = 0, rows = 1, all = 0;
+    Chunks(int64_t batch, int32_t heads, int64_t q_len, int64_t k_len) {
+        if (batch == 0 || heads == 0 || q_len == 0 || k_len == 0) return;
+        spans = ceil_div(q_len + k_len - 1, SPAN);
+        rows = std::max<int64_t>(16, ceil_div(q_len * spans * heads, 4096));
+        rows = std::max(rows, ceil_div(q_len * spans * heads, INT32_MAX / 2));
+        all = spans * ceil_div(q_len, rows);
+    }
+};
 
 ias_status launched() {
     HIPC(hipGetLastError());
@@ -129,21 +221,21 @@ ias_status launched() {
 template <class T>
 ias_status bias(int32_t heads, int64_t q_len, int64_t k_len, int32_t nb, const void *table, const int32_t *edges,
                 void *out, hipStream_t st) {
-    const int64_t grid = ceil_div(q_len * k_len, 256);
-    k_rel_bias<T><<<dim3((unsigned)grid), 256, 0, st>>>(heads, q_len, k_len, nb, (const T *)table, edges, (T *)out);
+    const dim3 grid((unsigned)ceil_div(q_len * k_len, 256 * V), (unsigned)ceil_div(heads, HEADS));
+    k_rel_bias<T><<<grid, 256, 0, st>>>(heads, q_len, k_len, nb, (const T *)table, edges, (T *)out);
     return launched();
 }
 
 template <class T>
 ias_status bias_grad(int64_t batch, int32_t heads, int64_t q_len, int64_t k_len, int32_t nb, const void *grad,
                      int64_t sb, int64_t sh, int64_t sr, const int32_t *edges, void *dtable, float *part, hipStream_t st) {
-    const int64_t chunks = k_len > 0 ? chunks_of(batch, q_len) : 0;
-    if (chunks * heads > 0) {
-        k_rel_bias_grad<T><<<dim3((unsigned)(chunks * heads)), 64, (size_t)nb * 256, st>>>(batch, heads, q_len, k_len, nb, (const T *)grad,
-                                                                                           sb, sh, sr, edges, ROWS, part);
+    const Chunks c(batch, heads, q_len, k_len);
+    if (c.all > 0) {
+        k_rel_bias_grad<T><<<dim3((unsigned)(c.all * heads)), 256, 0, st>>>(batch, heads, q_len, k_len, nb, (const T *)grad, sb, sh, sr, edges,
+                                                                            (int32_t)c.spans, (int32_t)c.rows, part);
         IAS_TRY(launched());
     }
-    k_rel_bias_sum<T><<<dim3((unsigned)(heads * nb)), 64, 0, st>>>(chunks, heads, nb, part, (T *)dtable);
+    k_rel_bias_sum<T><<<dim3((unsigned)(heads * nb)), 64, 0, st>>>(c.all, heads, nb, part, (T *)dtable);
     return launched();
 }
 
@@ -169,7 +261,7 @@ extern "C" ias_status ias_rel_bias_grad_workspace(int64_t batch, int32_t heads, 
                                                   int32_t num_buckets, int64_t *bytes) {
     IAS_TRY(check_bias(IAS_DTYPE_F32, batch, heads, q_len, k_len, num_buckets, 0));
     if (!bytes) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "no bytes");
-    *bytes = chunks_of(batch, q_len) * heads * num_buckets * (int64_t)sizeof(float);
+    *bytes = Chunks(batch, heads, q_len, k_len).all * heads * num_buckets * (int64_t)sizeof(float);
     return IAS_SUCCESS;
 }
 

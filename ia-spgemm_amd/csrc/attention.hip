@@ -9,6 +9,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 namespace ias {
@@ -211,10 +212,14 @@ ias_status check_workspace(const void *p, int64_t have, int64_t need) {
     return IAS_SUCCESS;
 }
 
-// A launch with `lds` bytes of dynamic LDS; more than 64 KB are asked for.
-template <class K, class... P>
-ias_status launch(K kernel, int64_t grid, int threads, size_t lds, void *stream, P... args) {
-    if (lds > 64 * 1024) HIPC(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+// A launch with `lds` bytes of dynamic LDS; more than 64 KB are asked for once a device.
+template <auto kernel, class... P>
+ias_status launch(int device, int64_t grid, int threads, size_t lds, void *stream, P... args) {
+    static std::atomic<bool> asked[64];
+    if (lds > 64 * 1024 && !(device < 64 && asked[device].load(std::memory_order_relaxed))) {
+        HIPC(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        if (device < 64) asked[device].store(true, std::memory_order_relaxed);
+    }
     kernel<<<dim3((unsigned)grid), threads, lds, (hipStream_t)stream>>>(args...);
     return launched();
 }
@@ -223,7 +228,7 @@ template <class T, int DP, int MT>
 ias_status select_rows(const ias_attention *a, const dev::AttnShape &s, const dev::SelectPlan &p, int threads, const ias_heads *q,
                        const void *summary, int32_t *blocks) {
     const int64_t grid = ceil_div(a->batch * a->k_heads * p.tiles, 8) * 8;
-    return launch(dev::k_block_select<T, DP, MT>, grid, threads, dev::select_lds(p.nq, p.stride, threads / 64), a->stream, s, p, side(q),
+    return launch<dev::k_block_select<T, DP, MT>>(a->device, grid, threads, dev::select_lds(p.nq, p.stride, threads / 64), a->stream, s, p, side(q),
                   static_cast<const uint16_t *>(summary), blocks);
 }
 
@@ -254,12 +259,12 @@ ias_status attend_waves(const ias_attention *a, const dev::AttnShape &s, const i
     const int64_t grid = ceil_div(r.tiles * r.plan.splits, 8) * 8;
     const size_t lds = dev::attend_lds(DP, MT, W, s.nblocks, r.plan.most, s.num_buckets * r.plan.span);
     if (a->table)
-        IAS_TRY(launch(dev::k_attend<T, DP, MT, W, true>, grid, 64 * W, lds, a->stream, s, r.plan, side(q), side(k), side(v), blocks, side_out(out), lse));
+        IAS_TRY((launch<dev::k_attend<T, DP, MT, W, true>>(a->device, grid, 64 * W, lds, a->stream, s, r.plan, side(q), side(k), side(v), blocks, side_out(out), lse)));
     else
-        IAS_TRY(launch(dev::k_attend<T, DP, MT, W, false>, grid, 64 * W, lds, a->stream, s, r.plan, side(q), side(k), side(v), blocks, side_out(out), lse));
+        IAS_TRY((launch<dev::k_attend<T, DP, MT, W, false>>(a->device, grid, 64 * W, lds, a->stream, s, r.plan, side(q), side(k), side(v), blocks, side_out(out), lse)));
     if (r.plan.splits > 1)
-        IAS_TRY(launch(dev::k_attend_join<T>, r.tiles * r.plan.nq * r.plan.span, 64, 0, a->stream, s, r.plan, DP, 16 * MT,
-                       a->table ? dev::LOG2E : 1.0f, side_out(out), lse));
+        IAS_TRY((launch<dev::k_attend_join<T>>(a->device, r.tiles * r.plan.nq * r.plan.span, 64, 0, a->stream, s, r.plan, DP, 16 * MT,
+                       a->table ? dev::LOG2E : 1.0f, side_out(out), lse)));
     return IAS_SUCCESS;
 }
 
@@ -290,9 +295,9 @@ ias_status grad_waves(const ias_attention *a, const dev::AttnShape &s, const dev
     const int32_t area = dev::grad_q_area(DP, MT, W, s.num_buckets, p.sums);
     const size_t lds = dev::grad_q_lds(area, s.nblocks, p.most, p.span, s.num_buckets);
     if (a->table)
-        return launch(dev::k_grad_q<T, DP, MT, W, true>, grid, 64 * W, lds, a->stream, s, p, area, side(dout), side(q), side(k), side(v), side(out), lse,
+        return launch<dev::k_grad_q<T, DP, MT, W, true>>(a->device, grid, 64 * W, lds, a->stream, s, p, area, side(dout), side(q), side(k), side(v), side(out), lse,
                       blocks, side_out(dq));
-    return launch(dev::k_grad_q<T, DP, MT, W, false>, grid, 64 * W, lds, a->stream, s, p, area, side(dout), side(q), side(k), side(v), side(out), lse, blocks,
+    return launch<dev::k_grad_q<T, DP, MT, W, false>>(a->device, grid, 64 * W, lds, a->stream, s, p, area, side(dout), side(q), side(k), side(v), side(out), lse, blocks,
                   side_out(dq));
 }
 
@@ -320,22 +325,22 @@ ias_status grad_all(const ias_attention *a, const ias_heads *dout, const ias_hea
         else IAS_TRY((grad_rows<T, DP, 2>(a, s, p, w.rows.waves, dout, q, k, v, out, lse, blocks, dq)));
     }
     if (w.k.entries > 0) {
-        IAS_TRY(launch(dev::k_clear, ceil_div(w.k.entries, 256), 256, 0, a->stream, w.k.entries, w.count));
+        IAS_TRY((launch<dev::k_clear>(a->device, ceil_div(w.k.entries, 256), 256, 0, a->stream, w.k.entries, w.count)));
         if (a->q_len > 0)
-            IAS_TRY(launch(dev::k_invert, bh * w.k.nw, 256, 4 * (size_t)s.nblocks, a->stream, s, w.k.nw, blocks, w.bits, w.count));
-        IAS_TRY(launch(dev::k_items, 1, 1024, 0, a->stream, w.k.entries, w.k.per, w.count, w.first));
+            IAS_TRY((launch<dev::k_invert>(a->device, bh * w.k.nw, 256, 4 * (size_t)s.nblocks, a->stream, s, w.k.nw, blocks, w.bits, w.count)));
+        IAS_TRY((launch<dev::k_items>(a->device, 1, 1024, 0, a->stream, w.k.entries, w.k.per, w.count, w.first)));
         const size_t lds = 4 * 32 * (size_t)DP * 2 + 2 * 5 * 32 * 4 + 4 * (size_t)w.k.per + 32 + 4 * (size_t)s.group * s.num_buckets;
         const int64_t grid = ceil_div(w.items * w.k.subs, 8) * 8;
         if (a->q_len > 0) {
             if (a->table)
-                IAS_TRY(launch(dev::k_grad_kv<T, DP, true>, grid, 256, lds, a->stream, s, w.k, side(dout), side(q), side(k), side(v), lse, side_out(dk), side_out(dv)));
+                IAS_TRY((launch<dev::k_grad_kv<T, DP, true>>(a->device, grid, 256, lds, a->stream, s, w.k, side(dout), side(q), side(k), side(v), lse, side_out(dk), side_out(dv))));
             else
-                IAS_TRY(launch(dev::k_grad_kv<T, DP, false>, grid, 256, lds, a->stream, s, w.k, side(dout), side(q), side(k), side(v), lse, side_out(dk), side_out(dv)));
+                IAS_TRY((launch<dev::k_grad_kv<T, DP, false>>(a->device, grid, 256, lds, a->stream, s, w.k, side(dout), side(q), side(k), side(v), lse, side_out(dk), side_out(dv))));
         }
-        IAS_TRY(launch(dev::k_grad_kv_join<T>, w.k.entries * w.k.subs, 256, 0, a->stream, s, w.k, DP, side_out(dk), side_out(dv)));
+        IAS_TRY((launch<dev::k_grad_kv_join<T>>(a->device, w.k.entries * w.k.subs, 256, 0, a->stream, s, w.k, DP, side_out(dk), side_out(dv))));
     }
     if (dtable)
-        IAS_TRY(launch(dev::k_grad_table<T>, (int64_t)a->q_heads * a->num_buckets, 256, 0, a->stream, s, p, static_cast<uint16_t *>(dtable)));
+        IAS_TRY((launch<dev::k_grad_table<T>>(a->device, (int64_t)a->q_heads * a->num_buckets, 256, 0, a->stream, s, p, static_cast<uint16_t *>(dtable))));
     return IAS_SUCCESS;
 }
 

@@ -475,10 +475,12 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan,
     }
 }
 
-// Joins the splits of a tile: one wave for each row.
+// Joins the splits of a tile: one wave for each row, a lane for each split's figures
+// and then for two channels.
 template <class T>
 __global__ __launch_bounds__(64) void k_attend_join(AttnShape s, RowPlan plan, int32_t dp, int32_t tile_rows, float unit,
                                                     SideOut out, float *__restrict__ lse) {
+    __shared__ float weight[64];
     int64_t w = blockIdx.x;
     const int r = (int)(w % (plan.nq * plan.span));
     w /= plan.nq * plan.span;
@@ -486,18 +488,38 @@ __global__ __launch_bounds__(64) void k_attend_join(AttnShape s, RowPlan plan, i
     const int hh = (int)(w % plan.tiles % plan.parts) * plan.span + r % plan.span;
     w /= plan.tiles;
     const int g = (int)(w % s.k_heads), b = (int)(w / s.k_heads), lane = threadIdx.x;
+    const int64_t first = tile_id * plan.splits * tile_rows + r;   // splits: at most 64
+    const bool on = lane < plan.splits;
+    const float m = on ? plan.stat[(first + (int64_t)lane * tile_rows) * 2] : -INFINITY;
+    const float x = on ? plan.stat[(first + (int64_t)lane * tile_rows) * 2 + 1] : 0.0f;
+    float y[2] = {};
+    const float *from = plan.part + first * dp + 2 * lane;
+    const int64_t step = (int64_t)tile_rows * dp;
+    float all = m;
+    for (int d = 32; d; d >>= 1) all = fmaxf(all, __shfl_xor(all, d));
+    // a split that read nothing for the row weighs nothing; NaN goes on
+    const float f = m == -INFINITY && x == x ? 0.0f : __builtin_amdgcn_exp2f((m - all) * unit);
+    float l = x * f;
+    for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
+    weight[lane] = f;
+    __syncthreads();
     if (i >= s.ql(b) || hh >= s.group) return;
-    float all = -INFINITY, l = 0.0f, y[2] = {};
-    for (int n = 0; n < plan.splits; ++n) all = fmaxf(all, plan.stat[((tile_id * plan.splits + n) * tile_rows + r) * 2]);
-    for (int n = 0; n < plan.splits; ++n) {
-        const int64_t at = (tile_id * plan.splits + n) * tile_rows + r;
-        const float m = plan.stat[at * 2], x = plan.stat[at * 2 + 1];
-        if (m == -INFINITY && !(x != x)) continue;
-        const float f = __builtin_amdgcn_exp2f((m - all) * unit);
-        l += x * f;
-        for (int u = 0; u < 2; ++u)
-            if (2 * lane + u < s.dim) y[u] += plan.part[at * dp + 2 * lane + u] * f;
-    }
+    if (2 * lane < s.dim)
+        for (int n0 = 0; n0 < plan.splits; n0 += 8) {
+            float z[8][2];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const float *at = from + min(n0 + n, plan.splits - 1) * step;
+                z[n][0] = at[0];
+                z[n][1] = at[1];
+            }
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                if (n0 + n < plan.splits && weight[n0 + n] != 0.0f) {
+                    y[0] += z[n][0] * weight[n0 + n];
+                    y[1] += z[n][1] * weight[n0 + n];
+                }
+        }
     const int64_t h = (int64_t)g * s.group + hh;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (2 * lane < s.dim) {

@@ -69,13 +69,19 @@ __device__ double exact_score(const AttnShape &s, const Side &q, const uint16_t 
     const bool on = d < s.dim;
     const s16x8 m = on ? load8(mean + (int64_t)c * s.dim + d) : s16x8{};
     double best = -INFINITY;
-    for (int h = 0; h < s.group; ++h) {
-        const s16x8 x = on ? load8(q.at(b, i, (int64_t)g * s.group + h) + d) : s16x8{};
-        double t = 0.0;
+    for (int h0 = 0; h0 < s.group; h0 += 4) {
+        s16x8 x[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) t += (double)T::up((uint16_t)x[e]) * (double)T::up((uint16_t)m[e]);
-        for (int n = 8; n; n >>= 1) t += __shfl_xor(t, n);
-        if (t > best) best = t;
+        for (int n = 0; n < 4; ++n)
+            x[n] = on ? load8(q.at(b, i, (int64_t)g * s.group + min(h0 + n, s.group - 1)) + d) : s16x8{};
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            double t = 0.0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t += (double)T::up((uint16_t)x[n][e]) * (double)T::up((uint16_t)m[e]);
+            for (int k = 8; k; k >>= 1) t += __shfl_xor(t, k);
+            if (t > best) best = t;
+        }
     }
     return best;
 }
@@ -183,7 +189,8 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 256) void k_block_select(AttnShape
     }
 
     constexpr int HELD = 8;   // 64-block pieces of the keys in registers; more are read from LDS
-    uint32_t *taken = mnorm + 1 + wave * 2 * ((plan.stride + 31) / 32), *open = taken + (plan.stride + 31) / 32;
+    const int words = (plan.stride + 31) / 32;
+    uint32_t *taken = mnorm + 1 + wave * 2 * words, *open = taken + words;
     for (int qi = wave; qi < nq; qi += waves) {
         const int i = i0 + qi, seen = blocks_seen(p0 + qi);
         int32_t *row = blocks + ((((int64_t)b * s.k_heads + g) * s.q_len) + i) * s.keep;
@@ -216,8 +223,29 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 256) void k_block_select(AttnShape
         };
         // the largest key that at least `left` candidates have
         auto place = [&]() {
-            uint32_t at = 0;
-            for (int bit = 31; bit >= 0; --bit) {
+            uint32_t high = 0, low = 0xffffffffu;
+#pragma unroll
+            for (int n = 0; n < HELD; ++n) {
+                high = max(high, held[n]);
+                if (held[n]) low = min(low, held[n]);
+            }
+            for (int n = HELD; n < pieces; ++n) {
+                const int c = n * 64 + lane;
+                const uint32_t k = c >= lo && c < hi ? key[c] : 0;
+                high = max(high, k);
+                if (k) low = min(low, k);
+            }
+            for (int d = 32; d; d >>= 1) {
+                high = max(high, (uint32_t)__shfl_xor((int)high, d));
+                low = min(low, (uint32_t)__shfl_xor((int)low, d));
+            }
+            high = __builtin_amdgcn_readfirstlane(high);
+            low = __builtin_amdgcn_readfirstlane(low);
+            if (high == low) return high;
+            // all keys agree above this bit
+            const int top = 31 - __clz(high ^ low);
+            uint32_t at = high >> top >> 1 << top << 1;
+            for (int bit = top; bit >= 0; --bit) {
                 const uint32_t up = at | 1u << bit;
                 const int n = count(up);
                 if (n >= left) at = up;
@@ -272,7 +300,43 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 256) void k_block_select(AttnShape
             opened = split(0xffffffffu, 0xffffffffu, true);
             opened = 0;
         }
-        // the open ones by their 64-bit scores: high half, then the low one's halves
+        // the open ones by their 64-bit scores.  Up to 64, as nearly always: candidate n's
+        // score to lane n, and its place is the number of those before it.
+        if (opened > left && left > 0 && opened <= 64) {
+            unsigned long long mine = 0;
+            int where = 0, n = 0;
+            for (int p = 0; p < pieces; ++p) {
+                unsigned long long on = (unsigned long long)(2 * p + 1 < words ? open[2 * p + 1] : 0) << 32 | open[2 * p];
+                while (on) {
+                    int c[4];
+                    const int n0 = n;
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        c[d] = on ? p * 64 + __ffsll(on) - 1 : -1;
+                        n += on != 0;
+                        on &= on - 1;
+                    }
+                    const int group = lane / 16, own = group == 0 ? c[0] : group == 1 ? c[1] : group == 2 ? c[2] : c[3];
+                    const unsigned long long k = order_key(exact_score<T>(s, q, mean, b, i, g, max(own, 0), lane));
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        const unsigned long long kd = __shfl(k, 16 * d);
+                        if (lane == n0 + d && c[d] >= 0) {
+                            mine = kd;
+                            where = c[d];
+                        }
+                    }
+                }
+            }
+            int before = 0;
+            for (int d = 0; d < opened; ++d) {
+                const unsigned long long k = __shfl(mine, d);
+                before += k > mine || (k == mine && d < lane);
+            }
+            if (lane < opened && before < left) atomicOr(&taken[where >> 5], 1u << (where & 31));
+            left = 0;
+        }
+        // more: high half, then the low one's halves
         for (int level = 0; level < 3 && opened > left && left > 0; ++level) {
             for (int n = 0; n < pieces; ++n) {
                 const uint32_t low = open[2 * n], high = 2 * n + 1 < (plan.stride + 31) / 32 ? open[2 * n + 1] : 0;

@@ -33,40 +33,38 @@ def _device(t: torch.Tensor) -> int:
 
 
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return torch.cuda.current_stream(t.device.index).cuda_stream
 
 
 def _heads(t: torch.Tensor, shape, dtype, device, name: str) -> Heads:
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} is {tuple(t.shape)}, not {tuple(shape)}")
     if t.dtype != dtype or t.device != device:
         raise ValueError(f"{name} is {t.dtype} on {t.device}, not {dtype} on {device}")
-    if t.stride(3) != 1 and t.numel():
+    s = t.stride()
+    if s[3] != 1 and t.numel():
         raise ValueError(f"{name}: the last dimension has to be contiguous")
-    return Heads(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+    return Heads(t.data_ptr(), s[0], s[1], s[2])
 
 
 def _plain(t: Optional[torch.Tensor], shape, dtype, device, name: str) -> Optional[int]:
     """Address of a contiguous tensor of that shape and type."""
     if t is None:
         return None
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device or not t.is_contiguous():
+    if t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} has to be a contiguous {dtype} {tuple(shape)} on {device}, not {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
 def _attention(like: torch.Tensor, batch, q_len, k_len, q_heads, k_heads, dim, block, keep, causal, scale, q_lens,
                k_lens, table=None, edges=None) -> Attention:
-    _device(like)
-    if like.dtype not in _DTYPE:
+    device, dtype = _device(like), _DTYPE.get(like.dtype)
+    if dtype is None:
         raise ValueError(f"{like.dtype} is not supported")
-    a = Attention()
-    a.dtype, a.device, a.stream = _DTYPE[like.dtype], _device(like), _stream(like)
-    a.batch, a.q_len, a.k_len, a.q_heads, a.k_heads, a.head_dim = batch, q_len, k_len, q_heads, k_heads, dim
-    a.block, a.keep, a.causal = block, keep, int(bool(causal))
-    a.scale = float(scale) if scale is not None else (dim ** -0.5 if dim else 1.0)
-    a.q_lens = _plain(q_lens, (batch,), torch.int32, like.device, "q_lens")
-    a.k_lens = _plain(k_lens, (batch,), torch.int32, like.device, "k_lens")
+    a = Attention(dtype, device, _stream(like), batch, q_len, k_len, q_heads, k_heads, dim, block, keep, 1 if causal else 0,
+                  float(scale) if scale is not None else (dim ** -0.5 if dim else 1.0), 0,
+                  None if q_lens is None else _plain(q_lens, (batch,), torch.int32, like.device, "q_lens"),
+                  None if k_lens is None else _plain(k_lens, (batch,), torch.int32, like.device, "k_lens"))
     if (table is None) != (edges is None):
         raise ValueError("table and edges go together")
     if table is not None:
@@ -131,10 +129,14 @@ def _shapes(q, k, blocks, block, causal, scale, q_lens, k_lens, table, edges):
 
 
 def _workspace(a: Attention, like: torch.Tensor, backward: bool):
-    f, g = C.c_int64(0), C.c_int64(0)
-    check(lib.ias_block_attention_workspace(C.byref(a), C.byref(f), C.byref(g)), "ias_block_attention_workspace")
-    n = g.value if backward else f.value
-    return torch.empty(n, dtype=torch.uint8, device=like.device), n
+    n = C.c_int64(0)
+    check(lib.ias_block_attention_workspace(C.byref(a), None if backward else C.byref(n), C.byref(n) if backward else None),
+          "ias_block_attention_workspace")
+    return (torch.empty(n.value, dtype=torch.uint8, device=like.device) if n.value else None), n.value
+
+
+def _address(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, blocks: torch.Tensor, *, block: int = 64,
@@ -152,7 +154,7 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, blocks: t
     ws, n = _workspace(a, q, False)
     h = [_heads(t, s, q.dtype, q.device, x) for t, s, x in ((q, qs, "q"), (k, ks, "k"), (v, ks, "v"), (out, qs, "out"))]
     check(lib.ias_block_attention(C.byref(a), C.byref(h[0]), C.byref(h[1]), C.byref(h[2]), pb, C.byref(h[3]),
-                                  lse.data_ptr(), ws.data_ptr(), n), "ias_block_attention")
+                                  lse.data_ptr(), _address(ws), n), "ias_block_attention")
     return out, lse
 
 
@@ -173,7 +175,7 @@ def block_attention_grad(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v
         (dv, ks, "dv"))]
     p = [C.byref(x) for x in h]
     check(lib.ias_block_attention_grad(C.byref(a), p[0], p[1], p[2], p[3], p[4], pl, pb, p[5], p[6], p[7],
-                                       None if dtable is None else dtable.data_ptr(), ws.data_ptr(), n),
+                                       _address(dtable), _address(ws), n),
           "ias_block_attention_grad")
     return dq, dk, dv, dtable
 

@@ -472,3 +472,27 @@ def test_tensors_of_the_host_are_refused():
         attention.block_summary(q)
     with pytest.raises(ValueError):
         attention.rel_bias(torch.zeros(3, 2), torch.zeros(2, dtype=torch.int32), 4, 4)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["near", "same", "zero", "huge", "tiny"])
+@pytest.mark.parametrize("m", [70, 600])
+def test_select_where_scores_are_close(A, kind, m):
+    """Order by 64 bits where fp32 sums do not tell the scores apart, overflow or vanish."""
+    gen = torch.Generator(device="cuda").manual_seed(15)
+    b, n, hq, hkv, d, keep = 2, 9, 6, 2, 64, 20
+    q = torch.randn(b, n, hq, d, device="cuda", generator=gen).to(torch.bfloat16)
+    base = torch.randn(1, 1, 1, d, device="cuda", generator=gen).to(torch.bfloat16)
+    s = base.expand(b, hkv, m, d).clone()
+    if kind == "near":    # one channel differs by its last place: scores a few 2^-16 of the sum apart
+        at = torch.randint(0, d, (b, hkv, m), device="cuda", generator=gen)
+        step = torch.randint(-1, 2, (b, hkv, m), device="cuda", generator=gen).to(torch.int16)
+        s.view(torch.int16).scatter_add_(3, at[..., None], step[..., None])
+    elif kind == "zero":
+        q[:, ::2] = 0
+        s = torch.randn(b, hkv, m, d, device="cuda", generator=gen).to(torch.bfloat16)
+    elif kind in ("huge", "tiny"):
+        s = torch.randn(b, hkv, m, d, device="cuda", generator=gen).to(torch.bfloat16)
+        s, q = (x * (2.0 ** (100 if kind == "huge" else -100)) for x in (s, q))
+    got = A.block_select(q, s, keep, k_len=m * 64, first=1, local=1)
+    assert torch.equal(got.cpu(), ref.select(q, s, keep, m * 64, 64, True, 1, 1, None, None))

@@ -95,6 +95,8 @@ dev::AttnShape shape_of(const ias_attention *a) {
     s.q_len = a->q_len; s.k_len = a->k_len;
     s.batch = (int32_t)a->batch; s.q_heads = a->q_heads; s.k_heads = a->k_heads;
     s.group = a->q_heads / a->k_heads;
+    s.inverse = (uint32_t)ceil_div(65536, s.group);
+    s.inverse_keep = a->keep > 1 ? (uint32_t)ceil_div(1ll << 32, a->keep) : 0;
     s.dim = a->head_dim; s.block = a->block; s.keep = a->keep; s.causal = a->causal != 0;
     s.nblocks = (int32_t)ceil_div(a->k_len, a->block);
     s.scale = a->scale;
@@ -150,6 +152,7 @@ struct Rows {
         dp = a->head_dim > 64 ? 128 : 64;
         plan.span = std::min(group, 16 * mt);
         plan.parts = (int32_t)ceil_div(group, plan.span);
+        plan.inverse = (uint32_t)ceil_div(65536, plan.span);
         plan.nq = plan.parts > 1 ? 1 : (int32_t)std::max<int64_t>(1, std::min<int64_t>(16 * mt / group, a->q_len));
         // the union's list takes 8 bytes of LDS an entry
         if (std::min<int64_t>((int64_t)plan.nq * a->keep, ceil_div(a->k_len, a->block)) > 2048) plan.nq = std::max(1, 2048 / a->keep);
@@ -186,7 +189,7 @@ struct Backward {
     int64_t items;      // at most
     explicit Backward(const ias_attention *a, Space &w) : rows(a, a->table && a->num_buckets > 32) {
         const int64_t group = a->q_heads / a->k_heads, bh = a->batch * a->k_heads, nblocks = ceil_div(a->k_len, a->block);
-        q.nq = rows.plan.nq; q.span = rows.plan.span; q.parts = rows.plan.parts;
+        q.nq = rows.plan.nq; q.span = rows.plan.span; q.parts = rows.plan.parts; q.inverse = rows.plan.inverse;
         q.tiles = rows.plan.tiles; q.most = rows.plan.most;
         map = a->table ? w.part<uint8_t>(map_size(a)) : nullptr;
         q.delta = w.part<float>(a->batch * a->q_heads * a->q_len);

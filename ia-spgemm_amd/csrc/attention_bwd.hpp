@@ -16,8 +16,10 @@ namespace dev {
 // ------------------------------------------------------------------ dq
 struct GradPlan {
     int32_t nq, span, parts, tiles, most;   // as RowPlan
+    uint32_t inverse;
     float *delta;                           // [batch][q_heads][q_len]
     float *sums;                            // [tile][span][num_buckets], null: no dtable
+    __device__ int per_span(int r) const { return (int)((uint32_t)r * inverse >> 16); }
 };
 
 // LDS of k_grad_q: the waves' K and V tiles and the lanes' sums by bucket, over which
@@ -78,8 +80,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
     for (int m = 0; m < MT; ++m) {
         const int r = m * 16 + col;
         const bool there = r < rows;
-        qi[m] = there ? r / plan.span : 0;
-        hr[m] = h0 + (there ? r % plan.span : 0);
+        qi[m] = there ? plan.per_span(r) : 0;
+        hr[m] = h0 + (there ? r - qi[m] * plan.span : 0);
         pos[m] = (int)i0 + qi[m] + kl - ql;
         end[m] = !there ? 0 : s.causal ? min(kl, pos[m] + 1) : kl;
         const int64_t h = (int64_t)g * s.group + hr[m], at = ((int64_t)b * s.q_heads + h) * s.q_len + i0 + qi[m];
@@ -244,7 +246,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
         for (int e = tid; e < R * CH; e += THREADS) {
             const int r = e / CH, ch = e % CH;
             if (r >= rows || ch * 8 >= s.dim) continue;
-            const int rq = r / plan.span;
+            const int rq = plan.per_span(r);
             if (!(only >> rq & 1u)) continue;
             float y[8] = {};
             for (int n = 0; n < W; ++n)
@@ -255,7 +257,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
                 fine = fine && fabsf(y[d]) < INFINITY;
                 y[d] *= s.scale;
             }
-            *reinterpret_cast<s16x8 *>(dq.at(b, i0 + rq, (int64_t)g * s.group + h0 + r % plan.span) + ch * 8) = Mma<T>::pack(y);
+            *reinterpret_cast<s16x8 *>(dq.at(b, i0 + rq, (int64_t)g * s.group + h0 + r - rq * plan.span) + ch * 8) = Mma<T>::pack(y);
         }
         if (turn == 0) {
             if (!fine) scratch[1] = 1;
@@ -299,7 +301,7 @@ __global__ __launch_bounds__(256) inline void k_invert(AttnShape s, int32_t nw, 
     __syncthreads();
     const int n = max(0, min(32, ql - i0)) * s.keep;
     for (int e = threadIdx.x; e < n; e += 256) {
-        const int i = i0 + e / s.keep, c = blocks[(bh * s.q_len + i0) * s.keep + e];
+        const int i = i0 + s.per_keep(e), c = blocks[(bh * s.q_len + i0) * s.keep + e];
         const int end = s.causal ? min(kl, i + kl - ql + 1) : kl;
         if (c >= 0 && c < s.nblocks && (int64_t)c * s.block < end) atomicOr(&word[c], 1u << (i - i0));
     }

@@ -120,7 +120,7 @@ __device__ inline int block_union(const AttnShape &s, const int32_t *__restrict_
     const int64_t row0 = ((int64_t)b * s.k_heads + g) * s.q_len + i0;
     const int n = nq * s.keep;
     for (int e = tid; e < n; e += blockDim.x) {
-        const int qi = e / s.keep, c = blocks[row0 * s.keep + e];
+        const int qi = s.per_keep(e), c = blocks[row0 * s.keep + e];
         const int end = s.causal ? min(kl, (int)(i0 + qi) + kl - ql + 1) : kl;
         if (c >= 0 && c < s.nblocks && (int64_t)c * s.block < end) atomicOr(&words[c >> 5], 1u << (c & 31));
     }
@@ -144,7 +144,7 @@ __device__ inline int block_union(const AttnShape &s, const int32_t *__restrict_
     for (int k = tid; k < found; k += blockDim.x) masks[k] = 0;
     __syncthreads();
     for (int e = tid; e < n; e += blockDim.x) {
-        const int qi = e / s.keep, c = blocks[row0 * s.keep + e];
+        const int qi = s.per_keep(e), c = blocks[row0 * s.keep + e];
         const int end = s.causal ? min(kl, (int)(i0 + qi) + kl - ql + 1) : kl;
         if (c >= 0 && c < s.nblocks && (int64_t)c * s.block < end) {
             const int k = before[c >> 5] + __popc(words[c >> 5] & ((1u << (c & 31)) - 1));
@@ -217,11 +217,13 @@ template <int DP> struct Piece {
 
 struct RowPlan {
     int32_t nq, span, parts;   // queries and heads of a workgroup, workgroups of one query's heads
+    uint32_t inverse;          // ceil(2^16 / span)
     int32_t tiles;     // per batch element and key head
     int32_t splits;    // workgroups that share a tile's walk
     int32_t most;      // bound on the blocks of a union
     float *part;       // splits > 1: [tile][split][16 MT rows][DP] sums
     float *stat;       //             [tile][split][16 MT rows][2] maximum and sum
+    __device__ int per_span(int r) const { return (int)((uint32_t)r * inverse >> 16); }   // r / span, r < 64
 };
 
 // LDS of k_attend: the end's sums (the waves' V tiles lie in the same place),
@@ -275,8 +277,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan,
     for (int m = 0; m < MT; ++m) {
         const int r = m * 16 + col;
         const bool there = r < rows;
-        qi[m] = there ? r / plan.span : 0;
-        hr[m] = h0 + (there ? r % plan.span : 0);
+        qi[m] = there ? plan.per_span(r) : 0;
+        hr[m] = h0 + (there ? r - qi[m] * plan.span : 0);
         pos[m] = (int)i0 + qi[m] + kl - ql;
         end[m] = !there ? 0 : s.causal ? min(kl, pos[m] + 1) : kl;
         const uint16_t *row = q.at(b, i0 + qi[m], (int64_t)g * s.group + hr[m]);
@@ -433,7 +435,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan,
         for (int e = tid; e < R * CH; e += 64 * W) {
             const int r = e / CH, ch = e % CH;
             if (r >= rows || ch * 8 >= s.dim) continue;
-            const int rq = r / plan.span;
+            const int rq = plan.per_span(r);
             if (!(only >> rq & 1u)) continue;
             float all = -INFINITY, l = 0.0f, y[8] = {};
             for (int n = 0; n < W; ++n) all = fmaxf(all, stat[(n * R + r) * 2]);
@@ -456,7 +458,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan,
                 float z[8];
 #pragma unroll
                 for (int d = 0; d < 8; ++d) z[d] = y[d] * inv;
-                const int64_t h = (int64_t)g * s.group + h0 + r % plan.span;
+                const int64_t h = (int64_t)g * s.group + h0 + r - rq * plan.span;
                 *reinterpret_cast<s16x8 *>(out.at(b, i0 + rq, h) + ch * 8) = Mma<T>::pack(z);
                 if (lse && ch == 0)
                     lse[((int64_t)b * s.q_heads + h) * s.q_len + i0 + rq] =

@@ -24,10 +24,15 @@ struct SideOut {
 struct AttnShape {
     int64_t q_len, k_len;
     int32_t batch, q_heads, k_heads, group, dim, block, keep, causal, nblocks, num_buckets;
+    uint32_t inverse, inverse_keep;   // ceil(2^16 / group), ceil(2^32 / keep) (0 for keep = 1)
     float scale;
     const int32_t *q_lens, *k_lens;
     const uint16_t *table;
     const uint8_t *map;       // bucket of each distance, map[d + k_len - 1]
+    // r / group for r < 64 (group <= 64: the inverse is off by less than 2^-16)
+    __device__ int per_group(int r) const { return (int)((uint32_t)r * inverse >> 16); }
+    // e / keep for e < 2^14 (keep <= 256)
+    __device__ int per_keep(int e) const { return inverse_keep ? (int)__umulhi((uint32_t)e, inverse_keep) : e; }
     __device__ int32_t ql(int b) const {
         return q_lens ? min(max(q_lens[b], 0), (int32_t)q_len) : (int32_t)q_len;
     }

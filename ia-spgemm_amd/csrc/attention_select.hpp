@@ -86,6 +86,245 @@ __device__ double exact_score(const AttnShape &s, const Side &q, const uint16_t 
     return best;
 }
 
+// One of 64 lanes' maximum / minimum in all of them.
+template <class F> __device__ inline uint32_t wave_reduce(uint32_t x, F f) {
+    x = f(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0xb1, 0xf, 0xf, false));    // lanes 1 apart
+    x = f(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x4e, 0xf, 0xf, false));    // 2
+    x = f(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x141, 0xf, 0xf, false));   // mirrored in 8
+    x = f(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x140, 0xf, 0xf, false));   // in 16
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = f(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return __builtin_amdgcn_readfirstlane(f(b[0], b[1]));
+}
+
+// What a wave needs to pick one query's blocks.  off: twice the bound of the scores'
+// errors, infinite where there is none.  keep < seen here, so the first and the local
+// blocks do not meet.
+struct Pick {
+    const AttnShape &s;
+    const SelectPlan &plan;
+    const Side &q;
+    const uint16_t *mean;
+    int b, i, g, seen, lane;
+    uint32_t *key;
+    float off;
+    int32_t *row;
+};
+
+// Up to 64 NP blocks: keys in registers, sets of blocks in masks.  False, and nothing
+// written, if more than 64 candidates are too close to call (equal blocks, say).
+template <class T, int NP> __device__ bool pick_held(const Pick &p) {
+    const int lane = p.lane, lo = p.plan.first, hi = p.seen - p.plan.local;
+    int left = p.s.keep - p.plan.first - p.plan.local;
+    uint32_t held[NP];
+    unsigned long long taken[NP], open[NP];
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+        const int c = n * 64 + lane;
+        const bool free = c >= lo && c < hi;
+        held[n] = free ? p.key[c] : 0;
+        taken[n] = __ballot(c < p.seen && !free);
+        open[n] = 0;
+    }
+    if (left > 0) {
+        auto count = [&](uint32_t least) {
+            int t = 0;
+#pragma unroll
+            for (int n = 0; n < NP; ++n) t += __popcll(__ballot(held[n] >= least));
+            return t;
+        };
+        uint32_t from = 1, over = 0xffffffffu;
+        if (p.off < INFINITY) {
+            // the key in the last place: bits from the top, below those that all keys share
+            uint32_t high = 0, low = 0xffffffffu;
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                high = max(high, held[n]);
+                low = min(low, held[n] ? held[n] : 0xffffffffu);
+            }
+            high = wave_reduce(high, [](uint32_t x, uint32_t y) { return max(x, y); });
+            low = wave_reduce(low, [](uint32_t x, uint32_t y) { return min(x, y); });
+            uint32_t at = high;
+            if (high != low) {
+                const int top = 31 - __clz(high ^ low);
+                at = high >> top >> 1 << top << 1;
+                for (int bit = top; bit >= 0; --bit) {
+                    const int n = count(at | 1u << bit);
+                    if (n >= left) at |= 1u << bit;
+                    if (n == left) {   // these and no others: the smallest of their keys
+                        uint32_t least = 0xffffffffu;
+#pragma unroll
+                        for (int m = 0; m < NP; ++m) least = min(least, held[m] >= at ? held[m] : 0xffffffffu);
+                        at = wave_reduce(least, [](uint32_t x, uint32_t y) { return min(x, y); });
+                        break;
+                    }
+                }
+            }
+            const float last = of_key(at);
+            from = order_key(last - p.off);
+            over = order_key(last + p.off);
+        }
+        int opened = 0;
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const unsigned long long up = __ballot(held[n] > over);
+            open[n] = __ballot(held[n] >= from) & ~up;
+            taken[n] |= up;
+            left -= __popcll(up);
+            opened += __popcll(open[n]);
+        }
+        if (opened > left) {
+            if (opened > 64) return false;
+            // candidate n's 64-bit score to lane n; its place is the number of those before it
+            unsigned long long mine = 0;
+            int where = 0, n = 0;
+#pragma unroll
+            for (int m = 0; m < NP; ++m)
+                for (unsigned long long on = open[m]; on;) {
+                    int c[4];
+                    const int n0 = n;
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        c[d] = on ? m * 64 + __ffsll(on) - 1 : -1;
+                        n += on != 0;
+                        on &= on - 1;
+                    }
+                    const int group = lane / 16, own = group == 0 ? c[0] : group == 1 ? c[1] : group == 2 ? c[2] : c[3];
+                    const unsigned long long k = order_key(exact_score<T>(p.s, p.q, p.mean, p.b, p.i, p.g, max(own, 0), lane));
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        const unsigned long long kd = __shfl(k, 16 * d);
+                        if (lane == n0 + d && c[d] >= 0) {
+                            mine = kd;
+                            where = c[d];
+                        }
+                    }
+                }
+            int before = 0;
+            for (int d = 0; d < opened; ++d) {
+                const unsigned long long k = __shfl(mine, d);
+                before += k > mine || (k == mine && d < lane);
+            }
+            for (unsigned long long on = __ballot(lane < opened && before < left); on; on &= on - 1) {
+                const int c = __shfl(where, __ffsll(on) - 1);
+#pragma unroll
+                for (int m = 0; m < NP; ++m)
+                    if (c / 64 == m) taken[m] |= 1ull << (c & 63);
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < NP; ++n) taken[n] |= open[n];
+        }
+    }
+    int n = 0;
+#pragma unroll
+    for (int m = 0; m < NP; ++m) {
+        if (taken[m] >> lane & 1) p.row[n + __popcll(taken[m] & ((1ull << lane) - 1))] = m * 64 + lane;
+        n += __popcll(taken[m]);
+    }
+    for (int t = n + lane; t < p.s.keep; t += 64) p.row[t] = -1;
+    return true;
+}
+
+// Any number of blocks: keys and sets in LDS (taken, open: a bit for each block).
+template <class T> __device__ void pick_any(const Pick &p, uint32_t *taken, uint32_t *open) {
+    const AttnShape &s = p.s;
+    const SelectPlan &plan = p.plan;
+    const Side &q = p.q;
+    const uint16_t *mean = p.mean;
+    const int b = p.b, i = p.i, g = p.g, seen = p.seen, lane = p.lane, col = lane & 15;
+    uint32_t *key = p.key;
+    int32_t *row = p.row;
+    const float off = p.off;
+    const int words = (plan.stride + 31) / 32, pieces = (seen + 63) / 64;
+    const int lo = plan.first, hi = seen - plan.local;
+    int left = s.keep - plan.first - plan.local;
+    auto count = [&](uint32_t least) {   // candidates with a key of at least that (least > 0)
+        int t = 0;
+        for (int n = 0; n < pieces; ++n) {
+            const int c = n * 64 + lane;
+            t += __popcll(__ballot(c < hi && c >= lo && key[c] >= least));
+        }
+        return t;
+    };
+    // the largest key that at least `left` candidates have
+    auto place = [&]() {
+        uint32_t at = 0;
+        for (int bit = 31; bit >= 0; --bit)
+            if (count(at | 1u << bit) >= left) at |= 1u << bit;
+        return at;
+    };
+    // marks what is above `over` as taken and what is in [from, over] as open; returns how many are open
+    auto split = [&](uint32_t from, uint32_t over, bool start) {
+        int opened = 0, sure = 0;
+        for (int n = 0; n < pieces; ++n) {
+            const int c = n * 64 + lane;
+            const uint32_t k = c >= lo && c < hi ? key[c] : 0;
+            const unsigned long long up = __ballot(k > over), on = __ballot(k >= from && k <= over && k > 0);
+            const unsigned long long forced = __ballot(start && c < seen && (c < lo || c >= hi));
+            sure += __popcll(up);
+            opened += __popcll(on);
+            if (lane < 2) {
+                const uint32_t u = (uint32_t)((up | forced) >> (32 * lane)), o = (uint32_t)(on >> (32 * lane));
+                if (n * 2 + lane < words) {
+                    taken[n * 2 + lane] = start ? u : taken[n * 2 + lane] | u;
+                    open[n * 2 + lane] = o;
+                }
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        left -= sure;
+        return opened;
+    };
+    int opened;
+    if (left > 0) {
+        if (off < INFINITY) {
+            const float last = of_key(place());
+            opened = split(order_key(last - off), order_key(last + off), true);
+        } else {
+            opened = split(1, 0xffffffffu, true);
+        }
+    } else {
+        opened = split(0xffffffffu, 0xffffffffu, true);
+        opened = 0;
+    }
+    // the open ones by their 64-bit scores: high half, then the low one's halves
+    for (int level = 0; level < 3 && opened > left && left > 0; ++level) {
+        for (int n = 0; n < pieces; ++n) {
+            const uint32_t low = open[2 * n], high = 2 * n + 1 < words ? open[2 * n + 1] : 0;
+            unsigned long long on = (unsigned long long)high << 32 | low;
+            if (n * 64 + lane >= lo && n * 64 + lane < hi && !(on >> lane & 1)) key[n * 64 + lane] = 0;
+            while (on) {
+                int mine = -1;
+                for (int d = 0; d < 4 && on; ++d, on &= on - 1)
+                    if (lane / 16 == d) mine = __ffsll(on) - 1;
+                const double x = exact_score<T>(s, q, mean, b, i, g, n * 64 + max(mine, 0), lane);
+                const unsigned long long k = order_key(x);
+                const uint32_t part = level == 0 ? (uint32_t)(k >> 32) : level == 1 ? (uint32_t)(k >> 16 & 0xffff) + 1 : (uint32_t)(k & 0xffff) + 1;
+                if (mine >= 0 && col == 0) key[n * 64 + mine] = part;
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const uint32_t last = place();
+        opened = split(last, last, false);
+    }
+    // taken, and of the open ones the first
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    int n = 0;
+    for (int m = 0; m < pieces; ++m) {
+        const int c = m * 64 + lane;
+        const bool in = c < seen && (taken[c / 32] >> (c & 31) & 1), may = left > 0 && c < seen && (open[c / 32] >> (c & 31) & 1);
+        const unsigned long long maybe = __ballot(may);
+        const bool on = in || (may && __popcll(maybe & ((1ull << lane) - 1)) < left);
+        left -= min(left, __popcll(maybe));
+        const unsigned long long got = __ballot(on);
+        if (on) row[n + __popcll(got & ((1ull << lane) - 1))] = c;
+        n += __popcll(got);
+    }
+    for (int t = n + lane; t < s.keep; t += 64) row[t] = -1;
+}
+
 template <class T, int DP, int MT>
 __global__ __launch_bounds__(MT == 1 ? 1024 : 256) void k_block_select(AttnShape s, SelectPlan plan, Side q, const uint16_t *__restrict__ summary,
                                                        int32_t *__restrict__ blocks) {
@@ -114,7 +353,7 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 256) void k_block_select(AttnShape
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             const int r = m * 16 + col;
-            const uint16_t *row = q.at(b, i0 + (r < rows ? r / s.group : 0), (int64_t)g * s.group + (r < rows ? r % s.group : 0));
+            const uint16_t *row = q.at(b, i0 + (r < rows ? s.per_group(r) : 0), (int64_t)g * s.group + (r < rows ? r - s.per_group(r) * s.group : 0));
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const int d = 32 * ks + 8 * quad;
@@ -123,7 +362,7 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 256) void k_block_select(AttnShape
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int rr = m * 16 + 4 * quad + e;
-                qrow[m][e] = rr < rows ? rr / s.group : -1;
+                qrow[m][e] = rr < rows ? s.per_group(rr) : -1;
             }
         }
         __syncthreads();
@@ -188,7 +427,6 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 256) void k_block_select(AttnShape
         __syncthreads();
     }
 
-    constexpr int HELD = 8;   // 64-block pieces of the keys in registers; more are read from LDS
     const int words = (plan.stride + 31) / 32;
     uint32_t *taken = mnorm + 1 + wave * 2 * words, *open = taken + words;
     for (int qi = wave; qi < nq; qi += waves) {
@@ -198,179 +436,11 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 256) void k_block_select(AttnShape
             for (int t = lane; t < s.keep; t += 64) row[t] = t < seen ? t : -1;
             continue;
         }
-        uint32_t *key = keys + qi * plan.stride;
-        // first + local <= keep < seen: the two do not meet
-        const int lo = plan.first, hi = seen - plan.local, pieces = (seen + 63) / 64;
-        int left = s.keep - plan.first - plan.local;
-        uint32_t held[HELD];
-        auto load = [&]() {
-#pragma unroll
-            for (int n = 0; n < HELD; ++n) {
-                const int c = n * 64 + lane;
-                held[n] = c >= lo && c < hi ? key[c] : 0;
-            }
-        };
-        auto count = [&](uint32_t least) {   // candidates with a key of at least that (least > 0)
-            int t = 0;
-#pragma unroll
-            for (int n = 0; n < HELD; ++n)
-                if (n < pieces) t += __popcll(__ballot(held[n] >= least));
-            for (int n = HELD; n < pieces; ++n) {
-                const int c = n * 64 + lane;
-                t += __popcll(__ballot(c < hi && c >= lo && key[c] >= least));
-            }
-            return t;
-        };
-        // the largest key that at least `left` candidates have
-        auto place = [&]() {
-            uint32_t high = 0, low = 0xffffffffu;
-#pragma unroll
-            for (int n = 0; n < HELD; ++n) {
-                high = max(high, held[n]);
-                if (held[n]) low = min(low, held[n]);
-            }
-            for (int n = HELD; n < pieces; ++n) {
-                const int c = n * 64 + lane;
-                const uint32_t k = c >= lo && c < hi ? key[c] : 0;
-                high = max(high, k);
-                if (k) low = min(low, k);
-            }
-            for (int d = 32; d; d >>= 1) {
-                high = max(high, (uint32_t)__shfl_xor((int)high, d));
-                low = min(low, (uint32_t)__shfl_xor((int)low, d));
-            }
-            high = __builtin_amdgcn_readfirstlane(high);
-            low = __builtin_amdgcn_readfirstlane(low);
-            if (high == low) return high;
-            // all keys agree above this bit
-            const int top = 31 - __clz(high ^ low);
-            uint32_t at = high >> top >> 1 << top << 1;
-            for (int bit = top; bit >= 0; --bit) {
-                const uint32_t up = at | 1u << bit;
-                const int n = count(up);
-                if (n >= left) at = up;
-                if (n == left) {   // these and no others: their smallest key
-                    uint32_t least = 0xffffffffu;
-#pragma unroll
-                    for (int m = 0; m < HELD; ++m)
-                        if (held[m] >= up) least = min(least, held[m]);
-                    for (int m = HELD; m < pieces; ++m) {
-                        const int c = m * 64 + lane;
-                        if (c >= lo && c < hi && key[c] >= up) least = min(least, key[c]);
-                    }
-                    for (int d = 32; d; d >>= 1) least = min(least, (uint32_t)__shfl_xor((int)least, d));
-                    return least;
-                }
-            }
-            return at;
-        };
-        // marks what is above `over` as taken and what is in [from, over] as open; returns how many are open
-        auto split = [&](uint32_t from, uint32_t over, bool start) {
-            int opened = 0, sure = 0;
-            for (int n = 0; n < pieces; ++n) {
-                const int c = n * 64 + lane;
-                const uint32_t k = c >= lo && c < hi ? key[c] : 0;
-                const unsigned long long up = __ballot(k > over), on = __ballot(k >= from && k <= over && k > 0);
-                const unsigned long long forced = __ballot(start && c < seen && (c < lo || c >= hi));
-                sure += __popcll(up);
-                opened += __popcll(on);
-                if (lane < 2) {
-                    const uint32_t u = (uint32_t)((up | forced) >> (32 * lane)), o = (uint32_t)(on >> (32 * lane));
-                    if (n * 2 + lane < (plan.stride + 31) / 32) {
-                        taken[n * 2 + lane] = start ? u : taken[n * 2 + lane] | u;
-                        open[n * 2 + lane] = o;
-                    }
-                }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            left -= sure;
-            return opened;
-        };
-        int opened;
-        if (left > 0) {
-            load();
-            const float qq = __uint_as_float(qnorm[qi]), mm = __uint_as_float(*mnorm);
-            if (qq > 1e-30f && qq < 1e30f && mm > 1e-30f && mm < 1e30f) {
-                const float off = 2.0f * 1.6e-5f * sqrtf(qq) * sqrtf(mm), last = of_key(place());
-                opened = split(order_key(last - off), order_key(last + off), true);
-            } else {
-                opened = split(1, 0xffffffffu, true);
-            }
-        } else {
-            opened = split(0xffffffffu, 0xffffffffu, true);
-            opened = 0;
-        }
-        // the open ones by their 64-bit scores.  Up to 64, as nearly always: candidate n's
-        // score to lane n, and its place is the number of those before it.
-        if (opened > left && left > 0 && opened <= 64) {
-            unsigned long long mine = 0;
-            int where = 0, n = 0;
-            for (int p = 0; p < pieces; ++p) {
-                unsigned long long on = (unsigned long long)(2 * p + 1 < words ? open[2 * p + 1] : 0) << 32 | open[2 * p];
-                while (on) {
-                    int c[4];
-                    const int n0 = n;
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) {
-                        c[d] = on ? p * 64 + __ffsll(on) - 1 : -1;
-                        n += on != 0;
-                        on &= on - 1;
-                    }
-                    const int group = lane / 16, own = group == 0 ? c[0] : group == 1 ? c[1] : group == 2 ? c[2] : c[3];
-                    const unsigned long long k = order_key(exact_score<T>(s, q, mean, b, i, g, max(own, 0), lane));
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) {
-                        const unsigned long long kd = __shfl(k, 16 * d);
-                        if (lane == n0 + d && c[d] >= 0) {
-                            mine = kd;
-                            where = c[d];
-                        }
-                    }
-                }
-            }
-            int before = 0;
-            for (int d = 0; d < opened; ++d) {
-                const unsigned long long k = __shfl(mine, d);
-                before += k > mine || (k == mine && d < lane);
-            }
-            if (lane < opened && before < left) atomicOr(&taken[where >> 5], 1u << (where & 31));
-            left = 0;
-        }
-        // more: high half, then the low one's halves
-        for (int level = 0; level < 3 && opened > left && left > 0; ++level) {
-            for (int n = 0; n < pieces; ++n) {
-                const uint32_t low = open[2 * n], high = 2 * n + 1 < (plan.stride + 31) / 32 ? open[2 * n + 1] : 0;
-                unsigned long long on = (unsigned long long)high << 32 | low;
-                if (n * 64 + lane >= lo && n * 64 + lane < hi && !(on >> lane & 1)) key[n * 64 + lane] = 0;
-                while (on) {
-                    int mine = -1;
-                    for (int d = 0; d < 4 && on; ++d, on &= on - 1)
-                        if (lane / 16 == d) mine = __ffsll(on) - 1;
-                    const double x = exact_score<T>(s, q, mean, b, i, g, n * 64 + max(mine, 0), lane);
-                    const unsigned long long k = order_key(x);
-                    const uint32_t part = level == 0 ? (uint32_t)(k >> 32) : level == 1 ? (uint32_t)(k >> 16 & 0xffff) + 1 : (uint32_t)(k & 0xffff) + 1;
-                    if (mine >= 0 && col == 0) key[n * 64 + mine] = part;
-                }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            load();
-            const uint32_t last = place();
-            opened = split(last, last, false);
-        }
-        // taken, and of the open ones the first
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        int n = 0;
-        for (int m = 0; m < pieces; ++m) {
-            const int c = m * 64 + lane;
-            const bool in = c < seen && (taken[c / 32] >> (c & 31) & 1), may = left > 0 && c < seen && (open[c / 32] >> (c & 31) & 1);
-            const unsigned long long maybe = __ballot(may);
-            const bool on = in || (may && __popcll(maybe & ((1ull << lane) - 1)) < left);
-            left -= min(left, __popcll(maybe));
-            const unsigned long long got = __ballot(on);
-            if (on) row[n + __popcll(got & ((1ull << lane) - 1))] = c;
-            n += __popcll(got);
-        }
-        for (int t = n + lane; t < s.keep; t += 64) row[t] = -1;
+        const float qq = __uint_as_float(__builtin_amdgcn_readfirstlane(qnorm[qi])), mm = __uint_as_float(__builtin_amdgcn_readfirstlane(*mnorm));
+        const bool tame = qq > 1e-30f && qq < 1e30f && mm > 1e-30f && mm < 1e30f;
+        const Pick p{s, plan, q, mean, b, i, g, seen, lane, keys + qi * plan.stride, tame ? 2.0f * 1.6e-5f * sqrtf(qq) * sqrtf(mm) : INFINITY, row};
+        const bool done = seen <= 64 ? pick_held<T, 1>(p) : seen <= 128 ? pick_held<T, 2>(p) : seen <= 512 ? pick_held<T, 8>(p) : false;
+        if (!done) pick_any<T>(p, taken, open);
     }
 }
 

@@ -177,8 +177,11 @@ struct Forward {
 };
 // The backward pass: k_grad_q's rows (as the forward's; with the bias's gradient
 // the lanes' sums by bucket take 1 KB of LDS for each bucket and 16 rows, so 32 rows
-// only up to 32 buckets), and the items of k_grad_kv: about 2048 rows each, which
-// keeps the f32 results of blocks that many queries chose small beside their work.
+// only up to 32 buckets), and the items of k_grad_kv: 256 to 1024 rows each, about
+// 1024 items where there are few rows.  An item of a block that many queries chose
+// writes 64 KB of f32 results, so small ones cost more to join than they even out
+// (8192 tokens, 16/2 heads of 128, both kernels: 421, 382 and 415 us with 768, 1024
+// and 2048 rows).
 struct Backward {
     uint8_t *map;
     Rows rows;
@@ -195,7 +198,8 @@ struct Backward {
         q.delta = w.part<float>(a->batch * a->q_heads * a->q_len);
         q.sums = a->table ? w.part<float>(bh * q.tiles * q.span * a->num_buckets) : nullptr;
         k.nw = (int32_t)ceil_div(a->q_len, 32);
-        k.per = (int32_t)std::max<int64_t>(32, 2048 / group);
+        const int64_t rows_all = a->batch * a->q_heads * a->q_len * std::min<int64_t>(a->keep, nblocks);
+        k.per = (int32_t)(std::min<int64_t>(1024, std::max<int64_t>(256, rows_all / 1024)) / group);
         k.subs = a->block / 64;
         k.entries = bh * nblocks;
         items = k.entries + bh * a->q_len * std::min<int64_t>(a->keep, nblocks) / k.per;
@@ -340,7 +344,7 @@ ias_status grad_all(const ias_attention *a, const ias_heads *dout, const ias_hea
             else
                 IAS_TRY((launch<dev::k_grad_kv<T, DP, false>>(a->device, grid, 256, lds, a->stream, s, w.k, side(dout), side(q), side(k), side(v), lse, side_out(dk), side_out(dv))));
         }
-        IAS_TRY((launch<dev::k_grad_kv_join<T>>(a->device, w.k.entries * w.k.subs, 256, 0, a->stream, s, w.k, DP, side_out(dk), side_out(dv))));
+        IAS_TRY((launch<dev::k_grad_kv_join<T>>(a->device, w.k.entries * w.k.subs * 4, 256, 0, a->stream, s, w.k, DP, side_out(dk), side_out(dv))));
     }
     if (dtable)
         IAS_TRY((launch<dev::k_grad_table<T>>(a->device, (int64_t)a->q_heads * a->num_buckets, 256, 0, a->stream, s, p, static_cast<uint16_t *>(dtable))));

@@ -358,7 +358,7 @@ struct KeyPlan {
 // P and dS are rounded to the inputs' type for these products (half a step of
 // each), sums are fp32.
 template <class T, int DP, bool BIAS>
-__global__ __launch_bounds__(256, 2) void k_grad_kv(AttnShape s, KeyPlan plan, Side dout, Side q, Side k, Side v,
+__global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(AttnShape s, KeyPlan plan, Side dout, Side q, Side k, Side v,
                                                     const float *__restrict__ lse, SideOut dk, SideOut dv) {
     constexpr int KS = DP / 32, DT = DP / 16, CH = DP / 8, TILE = 32 * DP * 2, LD = 32 * CH / 256;
     extern __shared__ __attribute__((aligned(16))) char lds[];   // [2][Q, dO] tiles
@@ -421,160 +421,210 @@ __global__ __launch_bounds__(256, 2) void k_grad_kv(AttnShape s, KeyPlan plan, S
     const int rows = nqueries * s.group;
     const float cs = BIAS ? s.scale : s.scale * LOG2E;
 
-    // turn 0: 32 rows at a time.  If anything in the result is not finite (zeros of P and dS
-    // times a row's infinities), once more with one row at a time, added only to the keys that it reads.
-    for (int turn = 0; turn < 2; ++turn) {
-        const int step = turn == 0 ? 32 : 1;
-        f32x4 ak[DT], av[DT];
+    f32x4 ak[DT], av[DT];
 #pragma unroll
-        for (int t = 0; t < DT; ++t) ak[t] = av[t] = f32x4{};
-        s16x8 qn[LD], dn[LD];
-        float fn[5];
-        auto fetch = [&](int r0) {
+    for (int t = 0; t < DT; ++t) ak[t] = av[t] = f32x4{};
+    s16x8 qn[LD], dn[LD];
+    float fn[5];
+    auto fetch = [&](int r0) {
 #pragma unroll
-            for (int n = 0; n < LD; ++n) {
-                const int e = n * 256 + tid, r = r0 + e / CH, ch = e % CH;
-                const bool on = e / CH < step && r < rows && ch * 8 < s.dim;
-                const int i = on ? list[r / s.group] : 0;
-                const int64_t h = (int64_t)g * s.group + r % s.group;
-                qn[n] = on ? load8(q.at(b, i, h) + ch * 8) : s16x8{};
-                dn[n] = on ? load8(dout.at(b, i, h) + ch * 8) : s16x8{};
+        for (int n = 0; n < LD; ++n) {
+            const int r = r0 + (n * 256 + tid) / CH, ch = tid % CH;
+            const bool on = r < rows && ch * 8 < s.dim;
+            const int rr = min(r, rows - 1), i = list[rr / s.group], d = ch * 8 < s.dim ? ch * 8 : 0;
+            const int64_t h = (int64_t)g * s.group + rr % s.group;
+            const s16x8 x = load8(q.at(b, i, h) + d), y = load8(dout.at(b, i, h) + d);
+            qn[n] = on ? x : s16x8{};
+            dn[n] = on ? y : s16x8{};
+        }
+        if (tid < 32) {
+            const int r = r0 + tid;
+            const bool on = r < rows;
+            const int rr = min(r, rows - 1), i = list[rr / s.group], p = i + kl - ql;
+            const int64_t at = ((int64_t)b * s.q_heads + (int64_t)g * s.group + rr % s.group) * s.q_len + i;
+            const float l = on ? lse[at] : -INFINITY;
+            fn[0] = l == -INFINITY ? INFINITY : BIAS ? l : l * LOG2E;
+            fn[1] = plan.delta[at];
+            fn[2] = __int_as_float(!on ? 0 : s.causal ? min(kl, p + 1) : kl);
+            fn[3] = __int_as_float(p);
+            fn[4] = __int_as_float(rr % s.group);
+        }
+    };
+    auto put = [&](int buf) {
+#pragma unroll
+        for (int n = 0; n < LD; ++n) {
+            const int e = n * 256 + tid;
+            char *to = lds + buf * 2 * TILE + Tile<DP>::chunk(e / CH, e % CH);
+            *reinterpret_cast<s16x8 *>(to) = qn[n];
+            *reinterpret_cast<s16x8 *>(to + TILE) = dn[n];
+        }
+        if (tid < 32)
+#pragma unroll
+            for (int f = 0; f < 5; ++f) fig[(buf * 5 + f) * 32 + tid] = fn[f];
+    };
+    fetch(0);
+    int buf = 0;
+    for (int r0 = 0; r0 < rows; r0 += 32, buf ^= 1) {
+        put(buf);
+        __syncthreads();
+        if (r0 + 32 < rows) fetch(r0 + 32);
+        const int qt = buf * 2 * TILE, dt = qt + TILE;
+        const float *f = fig + buf * 5 * 32;
+        float p[8], ds[8];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            __builtin_amdgcn_sched_barrier(0);
+            f32x4 x{}, dp{};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                x = Mma<T>::run(tile.natural(qt, 16 * m, ks), kf[ks], x);
+                dp = Mma<T>::run(tile.natural(dt, 16 * m, ks), vf[ks], dp);
             }
-            if (tid < 32) {
-                const int r = r0 + tid;
-                const bool on = tid < step && r < rows;
-                const int i = on ? list[r / s.group] : 0, p = i + kl - ql;
-                const int64_t at = ((int64_t)b * s.q_heads + (int64_t)g * s.group + r % s.group) * s.q_len + i;
-                const float l = on ? lse[at] : -INFINITY;
-                fn[0] = l == -INFINITY ? INFINITY : BIAS ? l : l * LOG2E;
-                fn[1] = on ? plan.delta[at] : 0.0f;
-                fn[2] = __int_as_float(!on ? 0 : s.causal ? min(kl, p + 1) : kl);
-                fn[3] = __int_as_float(p);
-                fn[4] = __int_as_float(on ? r % s.group : 0);
-            }
-        };
-        auto put = [&](int buf) {
+            const int at = 16 * m + 4 * quad;
+            const f32x4 shift = *reinterpret_cast<const f32x4 *>(f + at), delta = *reinterpret_cast<const f32x4 *>(f + 32 + at);
+            const f32x4 end = *reinterpret_cast<const f32x4 *>(f + 64 + at);
 #pragma unroll
-            for (int n = 0; n < LD; ++n) {
-                const int e = n * 256 + tid;
-                char *to = lds + buf * 2 * TILE + Tile<DP>::chunk(e / CH, e % CH);
-                *reinterpret_cast<s16x8 *>(to) = qn[n];
-                *reinterpret_cast<s16x8 *>(to + TILE) = dn[n];
-            }
-            if (tid < 32)
-#pragma unroll
-                for (int f = 0; f < 5; ++f) fig[(buf * 5 + f) * 32 + tid] = fn[f];
-        };
-        fetch(0);
-        int buf = 0;
-        for (int r0 = 0; r0 < rows; r0 += step, buf ^= 1) {
-            put(buf);
-            __syncthreads();
-            if (r0 + step < rows) fetch(r0 + step);
-            const int qt = buf * 2 * TILE, dt = qt + TILE;
-            const float *f = fig + buf * 5 * 32;
-            float p[8], ds[8];
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                __builtin_amdgcn_sched_barrier(0);
-                f32x4 x{}, dp{};
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    x = Mma<T>::run(tile.natural(qt, 16 * m, ks), kf[ks], x);
-                    dp = Mma<T>::run(tile.natural(dt, 16 * m, ks), vf[ks], dp);
-                }
-                const int at = 16 * m + 4 * quad;
-                const f32x4 shift = *reinterpret_cast<const f32x4 *>(f + at), delta = *reinterpret_cast<const f32x4 *>(f + 32 + at);
-                const f32x4 end = *reinterpret_cast<const f32x4 *>(f + 64 + at);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float t = x[e] * cs;
-                    if (BIAS) {
-                        const int pos = __float_as_int(f[96 + at + e]), hr = __float_as_int(f[128 + at + e]);
-                        t += table[s.map[(int64_t)key - pos + s.k_len - 1] * s.group + hr];
-                    }
-                    const bool on = key < __float_as_int(end[e]);
-                    const float y = BIAS ? __builtin_amdgcn_exp2f((t - shift[e]) * LOG2E) : __builtin_amdgcn_exp2f(t - shift[e]);
-                    p[4 * m + e] = on ? y : 0.0f;
-                    ds[4 * m + e] = on ? y * (dp[e] - delta[e]) : 0.0f;
-                }
-            }
-            const s16x8 pf = Mma<T>::pack(p), sf = Mma<T>::pack(ds);
-            const int last = __float_as_int(f[64]) - (j0 + 16 * wave + 4 * quad);   // one row: the keys below are its own
-#pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                if (t % 2 == 0) __builtin_amdgcn_sched_barrier(0);   // else every fragment is read ahead and spilled
-                const s16x8 dtr = tile.transposed(dt, t), qtr = tile.transposed(qt, t);
-                if (turn == 0) {
-                    av[t] = Mma<T>::run(pf, dtr, av[t]);
-                    ak[t] = Mma<T>::run(sf, qtr, ak[t]);
+            for (int e = 0; e < 4; ++e) {
+                float y;
+                if (BIAS) {
+                    const int pos = __float_as_int(f[96 + at + e]), hr = __float_as_int(f[128 + at + e]);
+                    y = __builtin_amdgcn_exp2f((__builtin_fmaf(x[e], cs, table[s.map[(int64_t)key - pos + s.k_len - 1] * s.group + hr]) - shift[e]) * LOG2E);
                 } else {
-                    const f32x4 y = Mma<T>::run(pf, dtr, f32x4{}), z = Mma<T>::run(sf, qtr, f32x4{});
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        av[t][e] = e < last ? av[t][e] + y[e] : av[t][e];
-                        ak[t][e] = e < last ? ak[t][e] + z[e] : ak[t][e];
-                    }
+                    y = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], cs, -shift[e]));
                 }
+                const bool on = key < __float_as_int(end[e]);
+                p[4 * m + e] = on ? y : 0.0f;
+                ds[4 * m + e] = on ? y * (dp[e] - delta[e]) : 0.0f;
             }
         }
-        if (tid == 0) scratch[0] = 0;
-        __syncthreads();
-        bool fine = true;
+        const s16x8 pf = Mma<T>::pack(p), sf = Mma<T>::pack(ds);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            __builtin_amdgcn_sched_barrier(0);   // one row's addresses at a time
-            const int n = 16 * wave + 4 * quad + e, j = j0 + n;
-            uint16_t *tk = dk.at(b, min(j, kl - 1), g) + col, *tv = dv.at(b, min(j, kl - 1), g) + col;
-            float *to = plan.part + (((int64_t)item * plan.subs + sub) * 2 * 64 + n) * DP + col;
+        for (int t = 0; t < DT; ++t) {
+            if (t % 2 == 0) __builtin_amdgcn_sched_barrier(0);   // else every fragment is read ahead and spilled
+            av[t] = Mma<T>::run(pf, tile.transposed(dt, t), av[t]);
+            ak[t] = Mma<T>::run(sf, tile.transposed(qt, t), ak[t]);
+        }
+    }
+    if (tid == 0) scratch[0] = 0;
+    __syncthreads();
+    const bool alone = items == 1;
+    float *const parts = plan.part + ((int64_t)item * plan.subs + sub) * 2 * 64 * DP;
+    bool fine = true;
 #pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                if (16 * t + col >= s.dim) continue;
-                fine = fine && fabsf(ak[t][e]) < INFINITY && fabsf(av[t][e]) < INFINITY;
-                if (items > 1) {
-                    to[16 * t] = ak[t][e];
-                    to[64 * DP + 16 * t] = av[t][e];
-                } else if (j < kl) {
-                    tk[16 * t] = T::down(ak[t][e] * s.scale);
-                    tv[16 * t] = T::down(av[t][e]);
-                }
+    for (int e = 0; e < 4; ++e) {
+        __builtin_amdgcn_sched_barrier(0);   // one row's addresses at a time
+        const int n = 16 * wave + 4 * quad + e, j = j0 + n;
+        uint16_t *tk = dk.at(b, min(j, kl - 1), g) + col, *tv = dv.at(b, min(j, kl - 1), g) + col;
+        float *to = parts + n * DP + col;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+            if (16 * t + col >= s.dim) continue;
+            fine = fine && fabsf(ak[t][e]) < INFINITY && fabsf(av[t][e]) < INFINITY;
+            if (!alone) {
+                to[16 * t] = ak[t][e];
+                to[64 * DP + 16 * t] = av[t][e];
+            } else if (j < kl) {
+                tk[16 * t] = T::down(ak[t][e] * s.scale);
+                tv[16 * t] = T::down(av[t][e]);
             }
         }
-        if (turn == 0) {
-            if (!fine) scratch[0] = 1;
-            __syncthreads();
-            if (scratch[0] == 0) break;
+    }
+    if (!fine) scratch[0] = 1;
+    __syncthreads();
+    if (scratch[0] == 0) return;
+
+    // Something is not finite.  Zeros of P and dS times a row's infinities make NaN in keys that
+    // the row does not read, so once more without products of what is masked: four threads for a
+    // key, a quarter of the channels each, the rows one by one.
+    constexpr int C = DP / 4;
+    const int n = tid / 4, j = j0 + n, d0 = tid % 4 * C;
+    float bk[C], bv[C];
+#pragma unroll
+    for (int d = 0; d < C; ++d) bk[d] = bv[d] = 0.0f;
+    if (j < kl) {
+        const uint16_t *kr = k.at(b, j, g), *vr = v.at(b, j, g);
+        for (int r = 0; r < rows; ++r) {
+            const int i = list[r / s.group], pos = i + kl - ql, hr = r % s.group;
+            const int64_t h = (int64_t)g * s.group + hr, at = ((int64_t)b * s.q_heads + h) * s.q_len + i;
+            const float l = lse[at];
+            if ((s.causal && j > pos) || l == -INFINITY) continue;
+            const uint16_t *qr = q.at(b, i, h), *dr = dout.at(b, i, h);
+            float x = 0.0f, dp = 0.0f;
+#pragma unroll
+            for (int d = 0; d < C; ++d)
+                if (d0 + d < s.dim) {
+                    x = __builtin_fmaf(T::up(qr[d0 + d]), T::up(kr[d0 + d]), x);
+                    dp = __builtin_fmaf(T::up(dr[d0 + d]), T::up(vr[d0 + d]), dp);
+                }
+            for (int m = 1; m < 4; m <<= 1) {
+                x += __shfl_xor(x, m);
+                dp += __shfl_xor(dp, m);
+            }
+            x *= s.scale;
+            if (BIAS) x += table[s.map[(int64_t)j - pos + s.k_len - 1] * s.group + hr];
+            const float p = __builtin_amdgcn_exp2f((x - l) * LOG2E), ds = p * (dp - plan.delta[at]);
+#pragma unroll
+            for (int d = 0; d < C; ++d)
+                if (d0 + d < s.dim) {
+                    bv[d] = __builtin_fmaf(p, T::up(dr[d0 + d]), bv[d]);
+                    bk[d] = __builtin_fmaf(ds, T::up(qr[d0 + d]), bk[d]);
+                }
         }
-        __syncthreads();
+#pragma unroll
+        for (int d = 0; d < C; ++d) {
+            if (d0 + d >= s.dim) continue;
+            if (!alone) {
+                parts[n * DP + d0 + d] = bk[d];
+                parts[(64 + n) * DP + d0 + d] = bv[d];
+            } else {
+                dk.at(b, j, g)[d0 + d] = T::down(bk[d] * s.scale);
+                dv.at(b, j, g)[d0 + d] = T::down(bv[d]);
+            }
+        }
     }
 }
 
-// dk and dv of the blocks that no query or more than one item read.
+// dk and dv of the blocks that no query or more than one item read: a thread for 8
+// channels of a key, 16 keys a workgroup.
 template <class T>
 __global__ __launch_bounds__(256) void k_grad_kv_join(AttnShape s, KeyPlan plan, int32_t dp, SideOut dk, SideOut dv) {
-    const int sub = (int)(blockIdx.x % plan.subs);
-    const int64_t entry = blockIdx.x / plan.subs;
+    const int sub = (int)(blockIdx.x / 4 % plan.subs);
+    const int64_t entry = blockIdx.x / 4 / plan.subs;
     const int32_t first = plan.first[entry], items = plan.first[entry + 1] - first;
     if (items == 1) return;
     const int c = (int)(entry % s.nblocks), g = (int)(entry / s.nblocks % s.k_heads), b = (int)(entry / s.nblocks / s.k_heads);
-    const int kl = s.kl(b), j0 = c * s.block + sub * 64, chunks = s.dim / 8;
-    for (int e = threadIdx.x; e < 64 * chunks; e += 256) {
-        const int n = e / chunks, d = e % chunks * 8;
-        if (j0 + n >= kl) continue;
-        float x[8] = {}, y[8] = {};
-        for (int t = 0; t < items; ++t) {
-            const float *from = plan.part + ((((int64_t)first + t) * plan.subs + sub) * 2 * 64 + n) * dp + d;
+    const int n = blockIdx.x % 4 * 16 + threadIdx.x / 16, d = threadIdx.x % 16 * 8, j = c * s.block + sub * 64 + n;
+    if (j >= s.kl(b) || d >= s.dim) return;
+    const f32x4 *from = reinterpret_cast<const f32x4 *>(plan.part + (((int64_t)first * plan.subs + sub) * 2 * 64 + n) * dp + d);
+    const int64_t step = (int64_t)plan.subs * 2 * 64 * dp / 4, other = 64 * dp / 4;
+    f32x4 x[2] = {}, y[2] = {};
+    for (int t0 = 0; t0 < items; t0 += 4) {
+        f32x4 z[4][4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] += from[i];
-                y[i] += from[64 * dp + i];
-            }
+        for (int t = 0; t < 4; ++t) {
+            const f32x4 *at = from + min(t0 + t, items - 1) * step;
+            z[t][0] = at[0];
+            z[t][1] = at[1];
+            z[t][2] = at[other];
+            z[t][3] = at[other + 1];
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] *= s.scale;
-        *reinterpret_cast<s16x8 *>(dk.at(b, j0 + n, g) + d) = Mma<T>::pack(x);
-        *reinterpret_cast<s16x8 *>(dv.at(b, j0 + n, g) + d) = Mma<T>::pack(y);
+        for (int t = 0; t < 4; ++t)
+            if (t0 + t < items) {
+                x[0] += z[t][0];
+                x[1] += z[t][1];
+                y[0] += z[t][2];
+                y[1] += z[t][3];
+            }
     }
+    float u[8], v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        u[i] = x[i / 4][i % 4] * s.scale;
+        v[i] = y[i / 4][i % 4];
+    }
+    *reinterpret_cast<s16x8 *>(dk.at(b, j, g) + d) = Mma<T>::pack(u);
+    *reinterpret_cast<s16x8 *>(dv.at(b, j, g) + d) = Mma<T>::pack(v);
 }
 
 }  // namespace dev

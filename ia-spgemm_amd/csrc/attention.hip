@@ -143,17 +143,17 @@ ias_status bucket_map(const ias_attention *a, dev::AttnShape &s, uint8_t *map) {
 // of keys each: 148, 90 and 65 us with 4, 2 and 1 waves; 16 blocks 406, 343, 324 us;
 // 2048 tiles with their gradients: 417, 342, 364 us).
 struct Rows {
-    int mt, dp, waves;
+    int rows, dp, waves;
     dev::RowPlan plan{};
     int64_t tiles, part, stat;   // all tiles; floats of the splits' results
-    explicit Rows(const ias_attention *a, bool small = false) {
+    explicit Rows(const ias_attention *a) {
         const int group = a->q_heads / a->k_heads;
-        mt = small || a->q_len * group <= 16 ? 1 : 2;
+        rows = a->q_len * group <= 16 ? 16 : 32;
         dp = a->head_dim > 64 ? 128 : 64;
-        plan.span = std::min(group, 16 * mt);
+        plan.span = std::min(group, rows);
         plan.parts = (int32_t)ceil_div(group, plan.span);
         plan.inverse = (uint32_t)ceil_div(65536, plan.span);
-        plan.nq = plan.parts > 1 ? 1 : (int32_t)std::max<int64_t>(1, std::min<int64_t>(16 * mt / group, a->q_len));
+        plan.nq = plan.parts > 1 ? 1 : (int32_t)std::max<int64_t>(1, std::min<int64_t>(rows / group, a->q_len));
         // the union's list takes 8 bytes of LDS an entry
         if (std::min<int64_t>((int64_t)plan.nq * a->keep, ceil_div(a->k_len, a->block)) > 2048) plan.nq = std::max(1, 2048 / a->keep);
         plan.tiles = (int32_t)ceil_div(a->q_len, plan.nq) * plan.parts;
@@ -161,8 +161,8 @@ struct Rows {
         tiles = a->batch * a->k_heads * plan.tiles;
         plan.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({ceil_div(512, std::max<int64_t>(1, tiles)), ceil_div(plan.most, 2), 64}));
         waves = plan.splits > 1 || tiles < 512 ? 4 : tiles < 4096 ? 2 : 1;
-        part = plan.splits > 1 ? tiles * plan.splits * 16 * mt * dp : 0;
-        stat = plan.splits > 1 ? tiles * plan.splits * 16 * mt * 2 : 0;
+        part = plan.splits > 1 ? tiles * plan.splits * rows * dp : 0;
+        stat = plan.splits > 1 ? tiles * plan.splits * rows * 2 : 0;
     }
 };
 
@@ -175,9 +175,7 @@ struct Forward {
         rows.plan.stat = rows.stat ? w.part<float>(rows.stat) : nullptr;
     }
 };
-// The backward pass: k_grad_q's rows (as the forward's; with the bias's gradient
-// the lanes' sums by bucket take 1 KB of LDS for each bucket and 16 rows, so 32 rows
-// only up to 32 buckets), and the items of k_grad_kv: 256 to 1024 rows each, about
+// The backward pass: k_grad_q's rows as the forward's, and the items of k_grad_kv: 256 to 1024 rows each, about
 // 1024 items where there are few rows.  An item of a block that many queries chose
 // writes 64 KB of f32 results, so small ones cost more to join than they even out
 // (8192 tokens, 16/2 heads of 128, both kernels: 421, 382 and 415 us with 768, 1024
@@ -190,7 +188,7 @@ struct Backward {
     uint32_t *bits;
     int32_t *count, *first;
     int64_t items;      // at most
-    explicit Backward(const ias_attention *a, Space &w) : rows(a, a->table && a->num_buckets > 32) {
+    explicit Backward(const ias_attention *a, Space &w) : rows(a) {
         const int64_t group = a->q_heads / a->k_heads, bh = a->batch * a->k_heads, nblocks = ceil_div(a->k_len, a->block);
         q.nq = rows.plan.nq; q.span = rows.plan.span; q.parts = rows.plan.parts; q.inverse = rows.plan.inverse;
         q.tiles = rows.plan.tiles; q.most = rows.plan.most;
@@ -260,27 +258,27 @@ ias_status select(const ias_attention *a, const ias_heads *q, const void *summar
     return select_rows<T, DP, 4>(a, s, p, 256, q, summary, blocks);
 }
 
-template <class T, int DP, int MT, int W>
+template <class T, int DP, int ROWS, int W>
 ias_status attend_waves(const ias_attention *a, const dev::AttnShape &s, const ias_heads *q, const ias_heads *k,
                        const ias_heads *v, const int32_t *blocks, const ias_heads *out, float *lse, const Rows &r) {
     const int64_t grid = ceil_div(r.tiles * r.plan.splits, 8) * 8;
-    const size_t lds = dev::attend_lds(DP, MT, W, s.nblocks, r.plan.most, s.num_buckets * r.plan.span);
+    const size_t lds = dev::attend_lds(DP, ROWS, W, s.nblocks, r.plan.most, s.num_buckets * r.plan.span);
     if (a->table)
-        IAS_TRY((launch<dev::k_attend<T, DP, MT, W, true>>(a->device, grid, 64 * W, lds, a->stream, s, r.plan, side(q), side(k), side(v), blocks, side_out(out), lse)));
+        IAS_TRY((launch<dev::k_attend<T, DP, ROWS, W, true>>(a->device, grid, 64 * W, lds, a->stream, s, r.plan, side(q), side(k), side(v), blocks, side_out(out), lse)));
     else
-        IAS_TRY((launch<dev::k_attend<T, DP, MT, W, false>>(a->device, grid, 64 * W, lds, a->stream, s, r.plan, side(q), side(k), side(v), blocks, side_out(out), lse)));
+        IAS_TRY((launch<dev::k_attend<T, DP, ROWS, W, false>>(a->device, grid, 64 * W, lds, a->stream, s, r.plan, side(q), side(k), side(v), blocks, side_out(out), lse)));
     if (r.plan.splits > 1)
-        IAS_TRY((launch<dev::k_attend_join<T>>(a->device, r.tiles * r.plan.nq * r.plan.span, 64, 0, a->stream, s, r.plan, DP, 16 * MT,
+        IAS_TRY((launch<dev::k_attend_join<T>>(a->device, r.tiles * r.plan.nq * r.plan.span, 64, 0, a->stream, s, r.plan, DP, ROWS,
                        a->table ? dev::LOG2E : 1.0f, side_out(out), lse)));
     return IAS_SUCCESS;
 }
 
-template <class T, int DP, int MT>
+template <class T, int DP, int ROWS>
 ias_status attend_rows(const ias_attention *a, const dev::AttnShape &s, const ias_heads *q, const ias_heads *k,
                        const ias_heads *v, const int32_t *blocks, const ias_heads *out, float *lse, const Rows &r) {
-    return r.waves == 4   ? attend_waves<T, DP, MT, 4>(a, s, q, k, v, blocks, out, lse, r)
-           : r.waves == 2 ? attend_waves<T, DP, MT, 2>(a, s, q, k, v, blocks, out, lse, r)
-                          : attend_waves<T, DP, MT, 1>(a, s, q, k, v, blocks, out, lse, r);
+    return r.waves == 4   ? attend_waves<T, DP, ROWS, 4>(a, s, q, k, v, blocks, out, lse, r)
+           : r.waves == 2 ? attend_waves<T, DP, ROWS, 2>(a, s, q, k, v, blocks, out, lse, r)
+                          : attend_waves<T, DP, ROWS, 1>(a, s, q, k, v, blocks, out, lse, r);
 }
 
 template <class T>
@@ -290,31 +288,31 @@ ias_status attend(const ias_attention *a, const ias_heads *q, const ias_heads *k
     if (a->table) IAS_TRY(bucket_map(a, s, f.map));
     const Rows &r = f.rows;
     if (r.dp == 64)
-        return r.mt == 1 ? attend_rows<T, 64, 1>(a, s, q, k, v, blocks, out, lse, r) : attend_rows<T, 64, 2>(a, s, q, k, v, blocks, out, lse, r);
-    return r.mt == 1 ? attend_rows<T, 128, 1>(a, s, q, k, v, blocks, out, lse, r) : attend_rows<T, 128, 2>(a, s, q, k, v, blocks, out, lse, r);
+        return r.rows == 16 ? attend_rows<T, 64, 16>(a, s, q, k, v, blocks, out, lse, r) : attend_rows<T, 64, 32>(a, s, q, k, v, blocks, out, lse, r);
+    return r.rows == 16 ? attend_rows<T, 128, 16>(a, s, q, k, v, blocks, out, lse, r) : attend_rows<T, 128, 32>(a, s, q, k, v, blocks, out, lse, r);
 }
 
-template <class T, int DP, int MT, int W>
+template <class T, int DP, int ROWS, int W>
 ias_status grad_waves(const ias_attention *a, const dev::AttnShape &s, const dev::GradPlan &p, const ias_heads *dout, const ias_heads *q,
                       const ias_heads *k, const ias_heads *v, const ias_heads *out, const float *lse, const int32_t *blocks,
                       const ias_heads *dq) {
     const int64_t tiles = a->batch * a->k_heads * p.tiles, grid = ceil_div(tiles, 8) * 8;
-    const int32_t area = dev::grad_q_area(DP, MT, W, s.num_buckets, p.sums);
+    const int32_t area = dev::grad_q_area(DP, ROWS, W, s.num_buckets, p.sums);
     const size_t lds = dev::grad_q_lds(area, s.nblocks, p.most, p.span, s.num_buckets);
     if (a->table)
-        return launch<dev::k_grad_q<T, DP, MT, W, true>>(a->device, grid, 64 * W, lds, a->stream, s, p, area, side(dout), side(q), side(k), side(v), side(out), lse,
+        return launch<dev::k_grad_q<T, DP, ROWS, W, true>>(a->device, grid, 64 * W, lds, a->stream, s, p, area, side(dout), side(q), side(k), side(v), side(out), lse,
                       blocks, side_out(dq));
-    return launch<dev::k_grad_q<T, DP, MT, W, false>>(a->device, grid, 64 * W, lds, a->stream, s, p, area, side(dout), side(q), side(k), side(v), side(out), lse, blocks,
+    return launch<dev::k_grad_q<T, DP, ROWS, W, false>>(a->device, grid, 64 * W, lds, a->stream, s, p, area, side(dout), side(q), side(k), side(v), side(out), lse, blocks,
                   side_out(dq));
 }
 
-template <class T, int DP, int MT>
+template <class T, int DP, int ROWS>
 ias_status grad_rows(const ias_attention *a, const dev::AttnShape &s, const dev::GradPlan &p, int waves, const ias_heads *dout,
                      const ias_heads *q, const ias_heads *k, const ias_heads *v, const ias_heads *out, const float *lse,
                      const int32_t *blocks, const ias_heads *dq) {
-    return waves == 4   ? grad_waves<T, DP, MT, 4>(a, s, p, dout, q, k, v, out, lse, blocks, dq)
-           : waves == 2 ? grad_waves<T, DP, MT, 2>(a, s, p, dout, q, k, v, out, lse, blocks, dq)
-                        : grad_waves<T, DP, MT, 1>(a, s, p, dout, q, k, v, out, lse, blocks, dq);
+    return waves == 4   ? grad_waves<T, DP, ROWS, 4>(a, s, p, dout, q, k, v, out, lse, blocks, dq)
+           : waves == 2 ? grad_waves<T, DP, ROWS, 2>(a, s, p, dout, q, k, v, out, lse, blocks, dq)
+                        : grad_waves<T, DP, ROWS, 1>(a, s, p, dout, q, k, v, out, lse, blocks, dq);
 }
 
 template <class T, int DP>
@@ -327,9 +325,8 @@ ias_status grad_all(const ias_attention *a, const ias_heads *dout, const ias_hea
     if (a->table) IAS_TRY(bucket_map(a, s, w.map));
     const int64_t bh = a->batch * a->k_heads;
     if (bh > 0 && a->q_len > 0) {
-        const int mt = w.rows.mt;
-        if (mt == 1) IAS_TRY((grad_rows<T, DP, 1>(a, s, p, w.rows.waves, dout, q, k, v, out, lse, blocks, dq)));
-        else IAS_TRY((grad_rows<T, DP, 2>(a, s, p, w.rows.waves, dout, q, k, v, out, lse, blocks, dq)));
+        if (w.rows.rows == 16) IAS_TRY((grad_rows<T, DP, 16>(a, s, p, w.rows.waves, dout, q, k, v, out, lse, blocks, dq)));
+        else IAS_TRY((grad_rows<T, DP, 32>(a, s, p, w.rows.waves, dout, q, k, v, out, lse, blocks, dq)));
     }
     if (w.k.entries > 0) {
         IAS_TRY((launch<dev::k_clear>(a->device, ceil_div(w.k.entries, 256), 256, 0, a->stream, w.k.entries, w.count)));

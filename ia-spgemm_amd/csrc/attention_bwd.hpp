@@ -24,22 +24,23 @@ struct GradPlan {
 
 // LDS of k_grad_q: the waves' K and V tiles and the lanes' sums by bucket, over which
 // the end's sums are laid; the lists; the bias table.
-inline int grad_q_area(int dp, int mt, int waves, int buckets, bool sums) {
-    const int v = waves * 2 * 32 * dp * 2 + (sums ? mt * buckets * 64 * waves * 4 : 0), o = walk_area(dp, mt, waves);
+inline int grad_q_area(int dp, int rows, int waves, int buckets, bool sums) {
+    const int v = waves * 2 * 32 * dp * 2 + (sums ? buckets * 64 * waves * 4 : 0), o = walk_area(dp, rows, waves);
     return v > o ? v : o;
 }
 inline size_t grad_q_lds(int area, int nblocks, int most, int span, int buckets) {
     return area + 8 * (size_t)((nblocks + 31) / 32) + 8 * (size_t)most + 16 + 4 * (size_t)span * buckets;
 }
 
-template <class T, int DP, int MT, int W, bool BIAS>
+template <class T, int DP, int ROWS, int W, bool BIAS>
 __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan, int32_t area, Side dout, Side q, Side k,
-                                                                 Side v, Side out, const float *__restrict__ lse,
-                                                                 const int32_t *__restrict__ blocks, SideOut dq) {
-    constexpr int THREADS = 64 * W, R = 16 * MT, KS = DP / 32, DT = DP / 16, CH = DP / 8;
+                                                      Side v, Side out, const float *__restrict__ lse,
+                                                      const int32_t *__restrict__ blocks, SideOut dq) {
+    typedef Form<ROWS> F;
+    constexpr int THREADS = 64 * W, CH = DP / 8, N = F::N, VL = Tile<DP>::N;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    float *sums = reinterpret_cast<float *>(lds);                           // [W][R][DP + 4], at the end
-    float *hist = reinterpret_cast<float *>(lds + W * 2 * Tile<DP>::BYTES);   // [MT][buckets][64 W]
+    float *sums = reinterpret_cast<float *>(lds);                           // [W][ROWS][DP + 4], at the end
+    float *hist = reinterpret_cast<float *>(lds + W * 2 * Tile<DP>::BYTES);   // [buckets][64 W]
     int32_t *scratch = reinterpret_cast<int32_t *>(lds + area);             // total, flag
     int32_t *ids = scratch + 4;
     uint32_t *masks = reinterpret_cast<uint32_t *>(ids + plan.most);
@@ -54,57 +55,46 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
     w /= plan.tiles;
     const int g = (int)(w % s.k_heads), b = (int)(w / s.k_heads);
     const int ql = s.ql(b), kl = s.kl(b);
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, col = lane & 15, quad = lane >> 4;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
     if (i0 >= ql) {
         if (BIAS && plan.sums)
             for (int e = tid; e < plan.span * s.num_buckets; e += THREADS) plan.sums[tile_id * plan.span * s.num_buckets + e] = 0.0f;
         return;
     }
     const int nq = min(plan.nq, ql - (int)i0), rows = (nq - 1) * plan.span + min(plan.span, s.group - h0);
-    const Tile<DP> tile(lds + wave * 2 * Tile<DP>::BYTES, lane);   // K, then V
+    const Tile<DP, ROWS> tile(lds + wave * 2 * Tile<DP>::BYTES, lane);   // K, then V
     constexpr int KT = 0, VT = Tile<DP>::BYTES;
 
     if (BIAS) {
         for (int e = tid; e < s.num_buckets * plan.span; e += THREADS)
             if (h0 + e % plan.span < s.group) table[e] = T::up(s.table[(e / plan.span) * s.q_heads + g * s.group + h0 + e % plan.span]);
         if (plan.sums)
-            for (int e = tid; e < MT * s.num_buckets * THREADS; e += THREADS) hist[e] = 0.0f;
+            for (int e = tid; e < s.num_buckets * THREADS; e += THREADS) hist[e] = 0.0f;
     }
     const int found = __builtin_amdgcn_readfirstlane(block_union(s, blocks, b, g, i0, nq, ql, kl, words, ids, masks, scratch));
 
-    s16x8 qf[MT][KS], df[MT][KS];
-    int qi[MT], end[MT], pos[MT], hr[MT];
-    float shift[MT], delta[MT];
-    const float c = fabsf(BIAS ? s.scale : s.scale * LOG2E);
+    const Row<DP, ROWS> row(lane, rows, plan.per_span(lane % ROWS), h0, plan.span, (int)i0, kl, ql, s.causal);
+    s16x8 qf[DP / F::K], df[DP / F::K];
+    float delta = 0.0f, shift;
+    {
+        const int64_t h = (int64_t)g * s.group + row.head, at = ((int64_t)b * s.q_heads + h) * s.q_len + i0 + row.query;
+        row.load(df, dout.at(b, i0 + row.query, h), s.dim);
+        row.load(qf, out.at(b, i0 + row.query, h), s.dim);
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int r = m * 16 + col;
-        const bool there = r < rows;
-        qi[m] = there ? plan.per_span(r) : 0;
-        hr[m] = h0 + (there ? r - qi[m] * plan.span : 0);
-        pos[m] = (int)i0 + qi[m] + kl - ql;
-        end[m] = !there ? 0 : s.causal ? min(kl, pos[m] + 1) : kl;
-        const int64_t h = (int64_t)g * s.group + hr[m], at = ((int64_t)b * s.q_heads + h) * s.q_len + i0 + qi[m];
-        const uint16_t *qr = q.at(b, i0 + qi[m], h), *dr = dout.at(b, i0 + qi[m], h), *orow = out.at(b, i0 + qi[m], h);
-        float t = 0.0f;
+        for (int ks = 0; ks < DP / F::K; ++ks)
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const int d = 32 * ks + 8 * quad;
-            const bool on = there && d < s.dim;
-            qf[m][ks] = on ? load8(qr + d) : s16x8{};
-            if (s.scale < 0.0f) qf[m][ks] = negated(qf[m][ks]);
-            df[m][ks] = on ? load8(dr + d) : s16x8{};
-            const s16x8 of = on ? load8(orow + d) : s16x8{};
+            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(T::up((uint16_t)df[ks][e]), T::up((uint16_t)qf[ks][e]), delta);
+        delta = row_sum<F::PARTS>(delta);
+        row.load(qf, q.at(b, i0 + row.query, h), s.dim);
+        if (s.scale < 0.0f)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) t = fmaf(T::up((uint16_t)df[m][ks][e]), T::up((uint16_t)of[e]), t);
-        }
-        t = quad_sum(t);
-        delta[m] = t;
-        const float l = there ? lse[at] : -INFINITY;
+            for (int ks = 0; ks < DP / F::K; ++ks) qf[ks] = negated(qf[ks]);
+        const float l = row.there ? lse[at] : -INFINITY;
         // a row that read nothing has lse = -inf: exp(x - inf) = 0
-        shift[m] = l == -INFINITY ? INFINITY : BIAS ? l : l * LOG2E;
-        if (wave == 0 && quad == 0 && there) plan.delta[at] = t;
+        shift = l == -INFINITY ? INFINITY : BIAS ? l : l * LOG2E;
+        if (wave == 0 && row.part == 0 && row.there) plan.delta[at] = delta;
     }
+    const float c = fabsf(BIAS ? s.scale : s.scale * LOG2E);
     const int per_block = s.block / 32;
     const int sure = s.causal ? min(kl, (int)i0 + kl - ql + 1) : kl;
     const Piece<DP> kp(k, b, g, lane, s.dim, kl), vp(v, b, g, lane, s.dim, kl);
@@ -113,12 +103,10 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
     for (int turn = 0; turn <= nq; ++turn) {
         const uint32_t only = turn == 0 ? ~0u : 1u << (turn - 1);
         const int vend = turn == 0 || !s.causal ? kl : min(kl, (int)i0 + turn - 1 + kl - ql + 1);
-        f32x4 o[MT][DT];
+        typename F::Acc o[DP / ROWS];
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int t = 0; t < DT; ++t) o[m][t] = f32x4{};
-        s16x8 kr[Piece<DP>::N], vr[Piece<DP>::N];
+        for (int t = 0; t < DP / ROWS; ++t) o[t] = typename F::Acc{};
+        s16x8 kr[VL], vr[VL];
         Walk<W> at(wave, per_block);
         auto skip = [&]() {
             while (turn > 0 && at.step < found && !(masks[at.step] & only)) at.on();
@@ -140,110 +128,92 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
             const uint32_t chose = more ? masks[at.step] : 0;
             tile.fill(kr, KT);
             tile.fill(vr, VT);
-            f32x4 x[MT][2], dp[MT][2];
-#pragma unroll
-            for (int sub = 0; sub < 2; ++sub) {
-#pragma unroll
-                for (int m = 0; m < MT; ++m) x[m][sub] = dp[m][sub] = f32x4{};
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    const s16x8 kf = tile.natural(KT, 16 * sub, ks), vf = tile.natural(VT, 16 * sub, ks);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        x[m][sub] = Mma<T>::run(kf, qf[m][ks], x[m][sub]);
-                        dp[m][sub] = Mma<T>::run(vf, df[m][ks], dp[m][sub]);
-                    }
-                }
-            }
+            float x[N], y[N];
+            scores<T, DP, ROWS>(tile, KT, qf, x);
+            scores<T, DP, ROWS>(tile, VT, df, y);
             const int jn = __builtin_amdgcn_readfirstlane(id) * s.block + at.part * 32;
             const uint32_t maskn = __builtin_amdgcn_readfirstlane(chose) & only;
             if (more) {
                 kp.load(kr, jn, vend);
                 vp.load(vr, jn, vend);
             }
-            const bool whole = j0 + 32 <= sure;
-            s16x8 sf[MT];
+            const bool sel = mask >> row.query & 1u;
+            const float off = sel ? shift : INFINITY;   // exp(x - inf) = 0
+            uint32_t bucket[N / 4];
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const bool sel = mask >> qi[m] & 1u;
-                const float off = sel ? shift[m] : INFINITY;   // exp(x - inf) = 0
-                float y[8];
-                uint32_t bucket[2] = {};
+            for (int n = 0; n < N; n += 4) {
+                if (BIAS) __builtin_memcpy(&bucket[n / 4], s.map + ((int64_t)j0 + row.key(n) + 4 * row.part - row.pos + s.k_len - 1), 4);
 #pragma unroll
-                for (int sub = 0; sub < 2; ++sub) {
-                    if (BIAS) __builtin_memcpy(&bucket[sub], s.map + ((int64_t)j0 + 16 * sub + 4 * quad - pos[m] + s.k_len - 1), 4);
+                for (int e = n; e < n + 4; ++e) {
+                    float p;
+                    if (BIAS)
+                        p = __builtin_amdgcn_exp2f((__builtin_fmaf(x[e], c, table[(bucket[n / 4] >> (8 * (e - n)) & 255) * plan.span + row.head - h0]) - off) * LOG2E);
+                    else
+                        p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], c, -off));
+                    y[e] = p * (y[e] - delta);
+                }
+            }
+            if (j0 + 32 > sure) {
+                const int lim = row.end - j0 - 4 * row.part;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float p;
-                        if (BIAS)
-                            p = __builtin_amdgcn_exp2f((__builtin_fmaf(x[m][sub][e], c, table[(bucket[sub] >> (8 * e) & 255) * plan.span + hr[m] - h0]) - off) * LOG2E);
-                        else
-                            p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[m][sub][e], c, -off));
-                        y[4 * sub + e] = p * (dp[m][sub][e] - delta[m]);
+                for (int e = 0; e < N; ++e) y[e] = row.key(e) < lim ? y[e] : 0.0f;
+            }
+            if (BIAS && plan.sums && turn == 0) {
+                // Each lane has a column of its own, so plain sums do, in the walk's order (an
+                // atomic LDS add takes some 200 cycles a wave).  Far keys share a bucket, mostly
+                // for a whole wave: then their sum goes in at once.
+                float *mine = hist + tid;
+                if (!sel)
+#pragma unroll
+                    for (int e = 0; e < N; ++e) y[e] = 0.0f;
+#pragma unroll
+                for (int n = 0; n < N; n += 4) {
+                    const uint32_t to = bucket[n / 4] & 255;
+                    if (__all(bucket[n / 4] == to * 0x01010101u)) {
+                        mine[to * THREADS] += (y[n] + y[n + 1]) + (y[n + 2] + y[n + 3]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) mine[(bucket[n / 4] >> (8 * e) & 255) * THREADS] += y[n + e];
                     }
                 }
-                if (!whole) {
-                    const int lim = end[m] - j0 - 4 * quad;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = 16 * (e / 4) + e % 4 < lim ? y[e] : 0.0f;
-                }
-                if (BIAS && plan.sums && turn == 0) {
-                    // Each lane has a column of its own, so plain sums do, in the walk's order (an
-                    // atomic LDS add takes some 200 cycles a wave).  Far keys share a bucket, mostly
-                    // for a whole wave: then their sum goes in at once.
-                    float *mine = hist + m * s.num_buckets * THREADS + tid;
-                    if (!sel)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) y[e] = 0.0f;
-#pragma unroll
-                    for (int sub = 0; sub < 2; ++sub) {
-                        const uint32_t n = bucket[sub] & 255;
-                        if (__all(bucket[sub] == n * 0x01010101u)) {
-                            mine[n * THREADS] += (y[4 * sub] + y[4 * sub + 1]) + (y[4 * sub + 2] + y[4 * sub + 3]);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) mine[(bucket[sub] >> (8 * e) & 255) * THREADS] += y[4 * sub + e];
-                        }
-                    }
-                }
-                sf[m] = Mma<T>::pack(y);
             }
-#pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                const s16x8 kf = tile.transposed(KT, t);
-#pragma unroll
-                for (int m = 0; m < MT; ++m) o[m][t] = Mma<T>::run(kf, sf[m], o[m][t]);
-            }
+            products<T, DP, ROWS>(tile, KT, y, o);
             j0 = jn;
             mask = maskn;
         }
         if (tid == 0) scratch[1] = 0;
         __syncthreads();
         if (BIAS && plan.sums && turn == 0) {
-            // a row's 4 W columns first: each 16 threads take a (bucket, 16 rows), starting at
-            // different columns so that the four of a wave lie in different banks
-            for (int e = tid / 16; e < MT * s.num_buckets; e += 4 * W) {
+            // a row's columns first: ROWS threads take a bucket, starting at different columns so
+            // that those of a wave lie in different banks
+            constexpr int COLS = THREADS / ROWS;
+            for (int n = tid / ROWS; n < s.num_buckets; n += COLS) {
                 float t = 0.0f;
-                for (int a = 0; a < 4 * W; ++a) t += hist[e * THREADS + (((a + e) & (4 * W - 1)) << 4) + (tid & 15)];
-                hist[e * THREADS + (tid & 15)] = t;   // read by this thread alone (column 0) up to here
+                for (int a = 0; a < COLS; ++a) t += hist[n * THREADS + ((a + n) & (COLS - 1)) * ROWS + tid % ROWS];
+                hist[n * THREADS + tid % ROWS] = t;   // read by this thread alone (column 0) up to here
             }
             __syncthreads();
             for (int e = tid; e < plan.span * s.num_buckets; e += THREADS) {
                 const int h = e / s.num_buckets, n = e % s.num_buckets;
                 float t = 0.0f;
-                for (int r = h; r < rows; r += plan.span) t += hist[((r / 16) * s.num_buckets + n) * THREADS + r % 16];
+                for (int r = h; r < rows; r += plan.span) t += hist[n * THREADS + r];
                 plan.sums[tile_id * plan.span * s.num_buckets + e] = t;
             }
             __syncthreads();
         }
+        const int r0 = lane % ROWS;
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int t = 0; t < DP / ROWS; ++t)
 #pragma unroll
-            for (int t = 0; t < DT; ++t)
-                *reinterpret_cast<f32x4 *>(sums + (wave * R + m * 16 + col) * (DP + 4) + 16 * t + 4 * quad) = o[m][t];
+            for (int n = 0; n < (int)(sizeof(typename F::Acc) / 4); n += 4) {
+                f32x4 z;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[e] = o[t][n + e];
+                *reinterpret_cast<f32x4 *>(sums + (wave * ROWS + r0) * (DP + 4) + ROWS * t + row.key(n) + 4 * row.part) = z;
+            }
         __syncthreads();
         bool fine = true;
-        for (int e = tid; e < R * CH; e += THREADS) {
+        for (int e = tid; e < ROWS * CH; e += THREADS) {
             const int r = e / CH, ch = e % CH;
             if (r >= rows || ch * 8 >= s.dim) continue;
             const int rq = plan.per_span(r);
@@ -251,7 +221,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
             float y[8] = {};
             for (int n = 0; n < W; ++n)
 #pragma unroll
-                for (int d = 0; d < 8; ++d) y[d] += sums[(n * R + r) * (DP + 4) + ch * 8 + d];
+                for (int d = 0; d < 8; ++d) y[d] += sums[(n * ROWS + r) * (DP + 4) + ch * 8 + d];
 #pragma unroll
             for (int d = 0; d < 8; ++d) {
                 fine = fine && fabsf(y[d]) < INFINITY;

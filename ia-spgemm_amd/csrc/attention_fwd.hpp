@@ -1,6 +1,6 @@
 // attention_fwd.hpp — block-sparse attention, forward (k_attend, k_attend_join).
 //
-// A workgroup takes up to 16 * MT rows of one key head: its query heads for a few
+// A workgroup takes up to ROWS rows of one key head: its query heads for a few
 // consecutive queries (row r is query r / span, head r % span), or some of the heads
 // of one query where there are more of them than rows.  It walks the union of the blocks that these queries chose, each block once:
 // neighbouring queries choose mostly the same blocks, and where they do not the
@@ -26,6 +26,7 @@ namespace ias {
 namespace dev {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -35,6 +36,9 @@ template <class T> struct Mma;
 template <> struct Mma<Bf16> {
     static __device__ f32x4 run(s16x8 a, s16x8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ f32x16 run(s16x8 a, s16x8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
     static __device__ s16x8 pack(const float *x) {
         bf16x8 y;
@@ -46,6 +50,9 @@ template <> struct Mma<Bf16> {
 template <> struct Mma<Fp16> {
     static __device__ f32x4 run(s16x8 a, s16x8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ f32x16 run(s16x8 a, s16x8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
     static __device__ s16x8 pack(const float *x) {
         f16x8 y;
@@ -59,14 +66,31 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 __device__ inline s16x8 load8(const uint16_t *p) { return *reinterpret_cast<const s16x8 *>(p); }
 
+// How the matrix instructions lay out 16 or 32 rows of queries by 32 keys.  The results
+// of S^T = K Q^T: a lane holds one row, of the keys 4 PARTS * (e / 4) + 4 * part + e % 4
+// for e < N, and PARTS lanes share the row.  The same, in this order and in groups of 8,
+// is what the right operand of O^T += V^T P^T asks for.
+template <int ROWS> struct Form;
+template <> struct Form<16> {
+    static constexpr int PARTS = 4, N = 8, K = 32;   // K: terms of one instruction
+    typedef f32x4 Acc;
+};
+template <> struct Form<32> {
+    static constexpr int PARTS = 2, N = 16, K = 16;
+    typedef f32x16 Acc;
+};
+
 // A tile of 32 rows by DP channels (16 bits) in LDS, 32-byte columns permuted by row:
-// column c of row r lies at c ^ mix(r).  Addresses are LDS offsets; all of one lane's
-// come from three by xor and constant offsets.
-template <int DP> struct Tile {
+// column c of row r lies at c ^ mix(r), so that the 8 rows which half a wave reads, and
+// the 4 rows by 64 bytes of a transposed read, lie in different banks.  Addresses are LDS
+// offsets; all of one lane's come from four by xor and constant offsets.
+template <int DP, int ROWS = 16> struct Tile {
     typedef __attribute__((address_space(3))) s16x8 lds8;
     typedef __attribute__((address_space(3))) s16x4 lds4;
     static constexpr int ROW = DP * 2, BYTES = 32 * ROW, CH = DP / 8, N = 32 * CH / 64, STEP = 64 / CH;
-    static __device__ uint32_t mix(int row) { return DP == 128 ? row & 7 : (row >> 1) & 3; }
+    static __device__ uint32_t mix(int row) {
+        return DP == 128 ? 2 * (row & 3) + (row >> 2 & 1) : (row & 2) + (row >> 2 & 1);
+    }
     // 16-byte chunk c of a row
     static __device__ uint32_t chunk(int row, int c) { return row * ROW + ((((uint32_t)c >> 1) ^ mix(row)) * 32) + (c & 1) * 16; }
     static __device__ uint32_t offset(const char *lds) {
@@ -77,9 +101,9 @@ template <int DP> struct Tile {
         const uint32_t base = offset(lds);
         even = base + chunk(lane / CH, lane % CH);
         odd = base + chunk(STEP + lane / CH, lane % CH);   // mix has a period of 8 rows
-        const int r = 4 * (lane >> 4) + ((lane & 15) >> 2);
-        nat = base + chunk(lane & 15, lane >> 4);
-        tr = base + r * ROW + mix(r) * 32 + (lane & 3) * 8;
+        nat = base + chunk(lane % ROWS, lane / ROWS);
+        const int r = 4 * (lane / ROWS) + ((lane & 15) >> 2), c = lane % ROWS / 16;
+        tr = base + r * ROW + (c ^ mix(r)) * 32 + (lane & 3) * 8;
     }
     // A piece that lies in registers as Piece::load leaves it; `at`: a tile's offset from the lane's.
     __device__ void fill(const s16x8 (&f)[N], int at) const {
@@ -89,16 +113,43 @@ template <int DP> struct Tile {
             else *(lds8 *)((n % 2 ? odd : even) + at + n / 2 * 8 * ROW) = f[n];
         }
     }
-    // Fragment of the tile as it is: row row0 + (lane & 15), channels 32 * ks + 8 * (lane >> 4) + 0..7.
-    __device__ s16x8 natural(int at, int row0, int ks) const { return *(lds8 *)((nat ^ (ks * 64)) + at + row0 * ROW); }
-    // Fragment of the transposed tile: channel 16 * c + (lane & 15), rows 4 * (lane >> 4) + 0..3 and 16 more.
-    __device__ s16x8 transposed(int at, int c) const {
-        const uint32_t a = (tr ^ (c * 32)) + at;
+    // Left operand from the tile as it is: row row0 + lane % ROWS, channels K * ks + 8 * (lane / ROWS) + 0..7.
+    __device__ s16x8 natural(int at, int row0, int ks) const { return *(lds8 *)((nat ^ (ks * 2 * Form<ROWS>::K)) + at + row0 * ROW); }
+    // Operand from the transposed tile: channel ROWS * c + lane % ROWS, rows row0 + 4 * (lane / ROWS) + 0..3
+    // and 4 PARTS further.
+    __device__ s16x8 transposed(int at, int c, int row0 = 0) const {
+        const uint32_t a = (tr ^ (c * 2 * ROWS)) + at + row0 * ROW;
         const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)a);
-        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(a + 16 * ROW));
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(a + 4 * Form<ROWS>::PARTS * ROW));
         return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     }
 };
+
+// x[e] for the N keys of a lane: a tile's 32 keys against the rows whose operands are q.
+template <class T, int DP, int ROWS>
+__device__ inline void scores(const Tile<DP, ROWS> &tile, int at, const s16x8 *q, float *x) {
+    typedef Form<ROWS> F;
+#pragma unroll
+    for (int sub = 0; sub < 32 / ROWS; ++sub) {
+        typename F::Acc acc{};
+#pragma unroll
+        for (int ks = 0; ks < DP / F::K; ++ks) acc = Mma<T>::run(tile.natural(at, ROWS * sub, ks), q[ks], acc);
+#pragma unroll
+        for (int e = 0; e < F::N * ROWS / 32; ++e) x[sub * (F::N * ROWS / 32) + e] = acc[e];
+    }
+}
+// o[c]: channels ROWS * c + .., += the tile's rows, transposed, times y.
+template <class T, int DP, int ROWS>
+__device__ inline void products(const Tile<DP, ROWS> &tile, int at, const float *y, typename Form<ROWS>::Acc *o) {
+    typedef Form<ROWS> F;
+    s16x8 f[F::N / 8];
+#pragma unroll
+    for (int n = 0; n < F::N / 8; ++n) f[n] = Mma<T>::pack(y + 8 * n);
+#pragma unroll
+    for (int c = 0; c < DP / ROWS; ++c)
+#pragma unroll
+        for (int n = 0; n < F::N / 8; ++n) o[c] = Mma<T>::run(tile.transposed(at, c, 16 * n), f[n], o[c]);
+}
 
 // Which part of the call a workgroup has.  Consecutive ids go to the 8 dies in
 // turn; each die gets a contiguous stretch of the work, so that the tiles of one
@@ -156,19 +207,46 @@ __device__ inline int block_union(const AttnShape &s, const int32_t *__restrict_
     return found;
 }
 
-// Maximum and sum over the four lanes that hold a row's keys (lanes 16 and 32 apart).
-__device__ inline float quad_max(float x) {
-    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+// Maximum and sum over the lanes that hold a row's keys (lanes 32, or 32 and 16 apart).
+template <int PARTS> __device__ inline float row_max(float x) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    if (PARTS == 2) return x;
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-__device__ inline float quad_sum(float x) {
-    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+template <int PARTS> __device__ inline float row_sum(float x) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    if (PARTS == 2) return x;
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
+
+// What a lane knows of its row of queries.
+template <int DP, int ROWS> struct Row {
+    typedef Form<ROWS> F;
+    int part, query, head, pos, end;   // head: of the key head's; end: keys before it may be read
+    bool there;
+    __device__ Row(int lane, int rows, int per, int h0, int span, int i0, int kl, int ql, bool causal) {
+        const int r = lane % ROWS;
+        part = lane / ROWS;
+        there = r < rows;
+        query = there ? per : 0;
+        head = h0 + (there ? r - per * span : 0);
+        pos = i0 + query + kl - ql;
+        end = !there ? 0 : causal ? min(kl, pos + 1) : kl;
+    }
+    // right operand of the scores; zeros where there is no row or channel
+    __device__ void load(s16x8 (&f)[DP / F::K], const uint16_t *row, int dim) const {
+#pragma unroll
+        for (int ks = 0; ks < DP / F::K; ++ks) {
+            const int d = F::K * ks + 8 * part;
+            f[ks] = there && d < dim ? load8(row + d) : s16x8{};
+        }
+    }
+    static __device__ int key(int e) { return 4 * F::PARTS * (e / 4) + e % 4; }   // without 4 * part
+};
 
 __device__ inline s16x8 negated(s16x8 x) { return x ^ (short)0x8000; }
 
@@ -221,29 +299,30 @@ struct RowPlan {
     int32_t tiles;     // per batch element and key head
     int32_t splits;    // workgroups that share a tile's walk
     int32_t most;      // bound on the blocks of a union
-    float *part;       // splits > 1: [tile][split][16 MT rows][DP] sums
-    float *stat;       //             [tile][split][16 MT rows][2] maximum and sum
+    float *part;       // splits > 1: [tile][split][ROWS][DP] sums
+    float *stat;       //             [tile][split][ROWS][2] maximum and sum
     __device__ int per_span(int r) const { return (int)((uint32_t)r * inverse >> 16); }   // r / span, r < 64
 };
 
 // LDS of k_attend: the end's sums (the waves' V tiles lie in the same place),
 // the lists, the rows' figures, the bias table.
-constexpr int walk_area(int dp, int mt, int waves) {
-    return waves * (2 * 32 * dp * 2 > 16 * mt * (dp + 4) * 4 ? 2 * 32 * dp * 2 : 16 * mt * (dp + 4) * 4);
+constexpr int walk_area(int dp, int rows, int waves) {
+    return waves * (2 * 32 * dp * 2 > rows * (dp + 4) * 4 ? 2 * 32 * dp * 2 : rows * (dp + 4) * 4);
 }
-inline size_t attend_lds(int dp, int mt, int waves, int nblocks, int most, int table) {
-    return walk_area(dp, mt, waves) + 8 * (size_t)((nblocks + 31) / 32) + 8 * (size_t)most + waves * 16 * (size_t)mt * 2 * 4 + 16 + 4 * (size_t)table;
+inline size_t attend_lds(int dp, int rows, int waves, int nblocks, int most, int table) {
+    return walk_area(dp, rows, waves) + 8 * (size_t)((nblocks + 31) / 32) + 8 * (size_t)most + waves * (size_t)rows * 2 * 4 + 16 + 4 * (size_t)table;
 }
 
-template <class T, int DP, int MT, int W, bool BIAS>
+template <class T, int DP, int ROWS, int W, bool BIAS>
 __global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan, Side q, Side k, Side v,
-                                                const int32_t *__restrict__ blocks, SideOut out, float *__restrict__ lse) {
-    constexpr int R = 16 * MT, KS = DP / 32, DT = DP / 16, VL = Tile<DP>::N, CH = DP / 8;
-    constexpr int AREA = walk_area(DP, MT, W);
+                                                      const int32_t *__restrict__ blocks, SideOut out, float *__restrict__ lse) {
+    typedef Form<ROWS> F;
+    constexpr int VL = Tile<DP>::N, CH = DP / 8, N = F::N;
+    constexpr int AREA = walk_area(DP, ROWS, W);
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    float *sums = reinterpret_cast<float *>(lds);                       // [W][R][DP + 4]
-    float *stat = reinterpret_cast<float *>(lds + AREA);                // [W][R][2]
-    int32_t *scratch = reinterpret_cast<int32_t *>(stat + W * R * 2);   // total, flag
+    float *sums = reinterpret_cast<float *>(lds);                       // [W][ROWS][DP + 4]
+    float *stat = reinterpret_cast<float *>(lds + AREA);                // [W][ROWS][2]
+    int32_t *scratch = reinterpret_cast<int32_t *>(stat + W * ROWS * 2);   // total, flag
     int32_t *ids = scratch + 4;
     uint32_t *masks = reinterpret_cast<uint32_t *>(ids + plan.most);
     uint32_t *words = masks + plan.most;
@@ -261,8 +340,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan,
     const int ql = s.ql(b), kl = s.kl(b);
     if (i0 >= ql) return;
     const int nq = min(plan.nq, ql - (int)i0), rows = (nq - 1) * plan.span + min(plan.span, s.group - h0);
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, col = lane & 15, quad = lane >> 4;
-    const Tile<DP> tile(lds + wave * 2 * Tile<DP>::BYTES, lane);   // K, then V
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
+    const Tile<DP, ROWS> tile(lds + wave * 2 * Tile<DP>::BYTES, lane);   // K, then V
     constexpr int KT = 0, VT = Tile<DP>::BYTES;
 
     if (BIAS)
@@ -270,25 +349,12 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan,
             if (h0 + e % plan.span < s.group) table[e] = T::up(s.table[(e / plan.span) * s.q_heads + g * s.group + h0 + e % plan.span]);
     const int found = __builtin_amdgcn_readfirstlane(block_union(s, blocks, b, g, i0, nq, ql, kl, words, ids, masks, scratch));
 
-    // this lane's rows
-    s16x8 qf[MT][KS];
-    int qi[MT], end[MT], pos[MT], hr[MT];
+    const Row<DP, ROWS> row(lane, rows, plan.per_span(lane % ROWS), h0, plan.span, (int)i0, kl, ql, s.causal);
+    s16x8 qf[DP / F::K];
+    row.load(qf, q.at(b, i0 + row.query, (int64_t)g * s.group + row.head), s.dim);
+    if (s.scale < 0.0f)
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int r = m * 16 + col;
-        const bool there = r < rows;
-        qi[m] = there ? plan.per_span(r) : 0;
-        hr[m] = h0 + (there ? r - qi[m] * plan.span : 0);
-        pos[m] = (int)i0 + qi[m] + kl - ql;
-        end[m] = !there ? 0 : s.causal ? min(kl, pos[m] + 1) : kl;
-        const uint16_t *row = q.at(b, i0 + qi[m], (int64_t)g * s.group + hr[m]);
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const int d = 32 * ks + 8 * quad;
-            qf[m][ks] = there && d < s.dim ? load8(row + d) : s16x8{};
-            if (s.scale < 0.0f) qf[m][ks] = negated(qf[m][ks]);
-        }
-    }
+        for (int ks = 0; ks < DP / F::K; ++ks) qf[ks] = negated(qf[ks]);
     const int per_block = s.block / 32;
     const int share = (found + plan.splits - 1) / plan.splits;
     const int first = min(found, split * share), stop = min(found, (split + 1) * share);
@@ -305,15 +371,10 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan,
     for (int turn = 0; turn <= nq; ++turn) {
         const uint32_t only = turn == 0 ? ~0u : 1u << (turn - 1);
         const int vend = turn == 0 || !s.causal ? kl : min(kl, (int)i0 + turn - 1 + kl - ql + 1);
-        f32x4 o[MT][DT];
-        float top[MT], sum[MT];
+        typename F::Acc o[DP / ROWS];
+        float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            top[m] = -INFINITY;
-            sum[m] = 0.0f;
-#pragma unroll
-            for (int t = 0; t < DT; ++t) o[m][t] = f32x4{};
-        }
+        for (int t = 0; t < DP / ROWS; ++t) o[t] = typename F::Acc{};
         s16x8 kr[VL], vr[VL];
         Walk<W> at(first * per_block + wave, per_block);
         auto skip = [&]() {   // to the next piece that anyone here reads
@@ -336,117 +397,98 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan,
             const uint32_t chose = more ? masks[at.step] : 0;
             tile.fill(kr, KT);
             tile.fill(vr, VT);
-            f32x4 x[MT][2];
-#pragma unroll
-            for (int sub = 0; sub < 2; ++sub) {
-#pragma unroll
-                for (int m = 0; m < MT; ++m) x[m][sub] = f32x4{};
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    const s16x8 kf = tile.natural(KT, 16 * sub, ks);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) x[m][sub] = Mma<T>::run(kf, qf[m][ks], x[m][sub]);
-                }
-            }
+            float y[N];
+            scores<T, DP, ROWS>(tile, KT, qf, y);
             const int jn = __builtin_amdgcn_readfirstlane(id) * s.block + at.part * 32;
             const uint32_t maskn = __builtin_amdgcn_readfirstlane(chose) & only;
             if (more) {
                 kp.load(kr, jn, kl);
                 vp.load(vr, jn, vend);
             }
-            const bool whole = j0 + 32 <= sure;
-            s16x8 pf[MT];
+            const bool sel = mask >> row.query & 1u;
+            if (BIAS) {
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const bool sel = mask >> qi[m] & 1u;
-                float y[8], big;
+                for (int n = 0; n < N; n += 4) {
+                    uint32_t bucket;
+                    __builtin_memcpy(&bucket, s.map + ((int64_t)j0 + row.key(n) + 4 * row.part - row.pos + s.k_len - 1), 4);
 #pragma unroll
-                for (int sub = 0; sub < 2; ++sub) {
-                    uint32_t bucket = 0;
-                    if (BIAS) __builtin_memcpy(&bucket, s.map + ((int64_t)j0 + 16 * sub + 4 * quad - pos[m] + s.k_len - 1), 4);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        y[4 * sub + e] = x[m][sub][e];
-                        if (BIAS) y[4 * sub + e] = __builtin_fmaf(x[m][sub][e], c, table[(bucket >> (8 * e) & 255) * plan.span + hr[m] - h0]);
-                    }
+                    for (int e = 0; e < 4; ++e)
+                        y[n + e] = __builtin_fmaf(y[n + e], c, table[(bucket >> (8 * e) & 255) * plan.span + row.head - h0]);
                 }
-                if (!whole) {
-                    const int lim = end[m] - j0 - 4 * quad;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = 16 * (e / 4) + e % 4 < lim ? y[e] : -INFINITY;
-                }
-                big = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
-                big = quad_max(big);
-                if (!BIAS) big *= c;
-                big = sel ? big : -INFINITY;
-                // the maximum is moved only where it grew by so much that exponentials would
-                // get large (2^8): that is the first piece and hardly ever another
-                if (__any(big > top[m] + 8.0f / unit)) {
-                    const float now = fmaxf(top[m], big);
-                    const float f = __builtin_amdgcn_exp2f((top[m] - (now == -INFINITY ? 0.0f : now)) * unit);
-                    sum[m] *= f;
-#pragma unroll
-                    for (int t = 0; t < DT; ++t) o[m][t] *= f;
-                    top[m] = now;
-                }
-                // a row that did not choose the block: exp(x - inf) = 0
-                const float shift = sel ? (top[m] == -INFINITY ? 0.0f : top[m]) : INFINITY;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    y[e] = __builtin_amdgcn_exp2f(BIAS ? (y[e] - shift) * LOG2E : __builtin_fmaf(y[e], c, -shift));
-                    sum[m] += y[e];
-                }
-                pf[m] = Mma<T>::pack(y);
             }
+            if (j0 + 32 > sure) {
+                const int lim = row.end - j0 - 4 * row.part;
 #pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                const s16x8 vf = tile.transposed(VT, t);
-#pragma unroll
-                for (int m = 0; m < MT; ++m) o[m][t] = Mma<T>::run(vf, pf[m], o[m][t]);
+                for (int e = 0; e < N; ++e) y[e] = row.key(e) < lim ? y[e] : -INFINITY;
             }
+            float big = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+#pragma unroll
+            for (int n = 4; n < N; n += 4) big = fmaxf(big, fmaxf(fmaxf(y[n], y[n + 1]), fmaxf(y[n + 2], y[n + 3])));
+            big = row_max<F::PARTS>(big);
+            if (!BIAS) big *= c;
+            big = sel ? big : -INFINITY;
+            // the maximum is moved only where it grew by so much that exponentials would
+            // get large (2^8): that is the first piece and hardly ever another
+            if (__any(big > top + 8.0f / unit)) {
+                const float now = fmaxf(top, big);
+                const float f = __builtin_amdgcn_exp2f((top - (now == -INFINITY ? 0.0f : now)) * unit);
+                sum *= f;
+#pragma unroll
+                for (int t = 0; t < DP / ROWS; ++t) o[t] *= f;
+                top = now;
+            }
+            // a row that did not choose the block: exp(x - inf) = 0
+            const float shift = sel ? (top == -INFINITY ? 0.0f : top) : INFINITY;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                y[e] = __builtin_amdgcn_exp2f(BIAS ? (y[e] - shift) * LOG2E : __builtin_fmaf(y[e], c, -shift));
+                sum += y[e];
+            }
+            products<T, DP, ROWS>(tile, VT, y, o);
             j0 = jn;
             mask = maskn;
         }
         // the waves meet
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            sum[m] = quad_sum(sum[m]);
-            if (quad == 0) {
-                stat[(wave * R + m * 16 + col) * 2] = top[m];
-                stat[(wave * R + m * 16 + col) * 2 + 1] = sum[m];
-            }
+        const int r0 = lane % ROWS;
+        sum = row_sum<F::PARTS>(sum);
+        if (row.part == 0) {
+            stat[(wave * ROWS + r0) * 2] = top;
+            stat[(wave * ROWS + r0) * 2 + 1] = sum;
         }
         if (tid == 0) scratch[1] = 0;
         __syncthreads();
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
+        {
             float all = -INFINITY;
-            for (int n = 0; n < W; ++n) all = fmaxf(all, stat[(n * R + m * 16 + col) * 2]);
-            const float f = top[m] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((top[m] - all) * unit);
+            for (int n = 0; n < W; ++n) all = fmaxf(all, stat[(n * ROWS + r0) * 2]);
+            const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((top - all) * unit);
+            const bool none = top == -INFINITY && sum == sum;   // a wave that read nothing for a row adds nothing
 #pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                float *to = sums + (wave * R + m * 16 + col) * (DP + 4) + 16 * t + 4 * quad;
-                // a wave that read nothing for a row adds nothing
-                *reinterpret_cast<f32x4 *>(to) = top[m] == -INFINITY && !(sum[m] != sum[m]) ? f32x4{} : o[m][t] * f;
-            }
+            for (int t = 0; t < DP / ROWS; ++t)
+#pragma unroll
+                for (int n = 0; n < (int)(sizeof(typename F::Acc) / 4); n += 4) {
+                    f32x4 z;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) z[e] = none ? 0.0f : o[t][n + e] * f;
+                    *reinterpret_cast<f32x4 *>(sums + (wave * ROWS + r0) * (DP + 4) + ROWS * t + row.key(n) + 4 * row.part) = z;
+                }
         }
         __syncthreads();
         bool fine = true;
-        for (int e = tid; e < R * CH; e += 64 * W) {
+        for (int e = tid; e < ROWS * CH; e += 64 * W) {
             const int r = e / CH, ch = e % CH;
             if (r >= rows || ch * 8 >= s.dim) continue;
             const int rq = plan.per_span(r);
             if (!(only >> rq & 1u)) continue;
             float all = -INFINITY, l = 0.0f, y[8] = {};
-            for (int n = 0; n < W; ++n) all = fmaxf(all, stat[(n * R + r) * 2]);
+            for (int n = 0; n < W; ++n) all = fmaxf(all, stat[(n * ROWS + r) * 2]);
             for (int n = 0; n < W; ++n) {
-                const float m = stat[(n * R + r) * 2], x = stat[(n * R + r) * 2 + 1];
+                const float m = stat[(n * ROWS + r) * 2], x = stat[(n * ROWS + r) * 2 + 1];
                 if (m != -INFINITY || x != x) l += x * __builtin_amdgcn_exp2f((m - all) * unit);
 #pragma unroll
-                for (int d = 0; d < 8; ++d) y[d] += sums[(n * R + r) * (DP + 4) + ch * 8 + d];
+                for (int d = 0; d < 8; ++d) y[d] += sums[(n * ROWS + r) * (DP + 4) + ch * 8 + d];
             }
             if (plan.splits > 1) {
-                const int64_t at = (tile_id * plan.splits + split) * R + r;
+                const int64_t at = (tile_id * plan.splits + split) * ROWS + r;
 #pragma unroll
                 for (int d = 0; d < 8; ++d) plan.part[at * DP + ch * 8 + d] = y[d];
                 if (ch == 0) {

@@ -102,6 +102,7 @@ dev::AttnShape shape_of(const ias_attention *a) {
     s.scale = a->scale;
     s.q_lens = a->q_lens; s.k_lens = a->k_lens;
     s.table = static_cast<const uint16_t *>(a->table);
+    s.edges = a->edges;
     s.num_buckets = a->table ? a->num_buckets : 0;
     return s;
 }
@@ -134,14 +135,20 @@ ias_status bucket_map(const ias_attention *a, dev::AttnShape &s, uint8_t *map) {
     return launched();
 }
 
-// How the walks share out the rows.  16 rows fill one matrix tile; 32 let more
-// queries share a walk and each fragment of K and V feed two tiles.  Few rows
-// (single tokens) are split along the walk until about every CU has two workgroups,
-// two blocks of keys each at least.  The chip holds two waves a SIMD, 2048, of these
-// kernels: a workgroup has as many waves as it takes to fill it, since a walk of one
-// wave has no end where waves wait for each other (8192 tokens, 8192 tiles, one block
-// of keys each: 148, 90 and 65 us with 4, 2 and 1 waves; 16 blocks 406, 343, 324 us;
-// 2048 tiles with their gradients: 417, 342, 364 us).
+// How the walks share out the rows.  16 rows where all fit (single tokens), else 32, so
+// that more queries share a walk and a fragment of K and V serves more rows.
+//
+// 16 rows: 8 waves share a walk, and only where it has more than 64 pieces of 32 keys
+// and the workgroups are fewer than CUs is it split, since a split costs a second
+// launch (one user, 16 blocks of 64 keys: 38 us a step with 8 splits of 4 waves, 35
+// without; 16 users, 32 blocks: 57 and 55).
+//
+// 32 rows: few are split until about every CU has two workgroups, two blocks of keys
+// each at least.  The chip holds two waves a SIMD, 2048, of these kernels: a workgroup
+// has as many waves as it takes to fill it, since a walk of one wave has no end where
+// waves wait for each other (8192 tokens, 8192 tiles, one block of keys each: 148, 90
+// and 65 us with 4, 2 and 1 waves; 16 blocks 406, 343, 324 us; 2048 tiles with their
+// gradients: 417, 342, 364 us).
 struct Rows {
     int rows, dp, waves;
     dev::RowPlan plan{};
@@ -159,8 +166,14 @@ struct Rows {
         plan.tiles = (int32_t)ceil_div(a->q_len, plan.nq) * plan.parts;
         plan.most = (int32_t)std::max<int64_t>(1, std::min<int64_t>((int64_t)plan.nq * a->keep, ceil_div(a->k_len, a->block)));
         tiles = a->batch * a->k_heads * plan.tiles;
-        plan.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({ceil_div(512, std::max<int64_t>(1, tiles)), ceil_div(plan.most, 2), 64}));
-        waves = plan.splits > 1 || tiles < 512 ? 4 : tiles < 4096 ? 2 : 1;
+        const int64_t pieces = (int64_t)plan.most * (a->block / 32), few = std::max<int64_t>(1, tiles);
+        if (rows == 16) {
+            waves = 8;
+            plan.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({ceil_div(256, few), ceil_div(pieces, 64), 64}));
+        } else {
+            plan.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({ceil_div(512, few), ceil_div(plan.most, 2), 64}));
+            waves = plan.splits > 1 || tiles < 512 ? 4 : tiles < 4096 ? 2 : 1;
+        }
         part = plan.splits > 1 ? tiles * plan.splits * rows * dp : 0;
         stat = plan.splits > 1 ? tiles * plan.splits * rows * 2 : 0;
     }
@@ -262,7 +275,7 @@ template <class T, int DP, int ROWS, int W>
 ias_status attend_waves(const ias_attention *a, const dev::AttnShape &s, const ias_heads *q, const ias_heads *k,
                        const ias_heads *v, const int32_t *blocks, const ias_heads *out, float *lse, const Rows &r) {
     const int64_t grid = ceil_div(r.tiles * r.plan.splits, 8) * 8;
-    const size_t lds = dev::attend_lds(DP, ROWS, W, s.nblocks, r.plan.most, s.num_buckets * r.plan.span);
+    const size_t lds = dev::attend_lds(DP, ROWS, W, s.nblocks, r.plan.most, s.num_buckets * (r.plan.span + 1));
     if (a->table)
         IAS_TRY((launch<dev::k_attend<T, DP, ROWS, W, true>>(a->device, grid, 64 * W, lds, a->stream, s, r.plan, side(q), side(k), side(v), blocks, side_out(out), lse)));
     else
@@ -276,17 +289,19 @@ ias_status attend_waves(const ias_attention *a, const dev::AttnShape &s, const i
 template <class T, int DP, int ROWS>
 ias_status attend_rows(const ias_attention *a, const dev::AttnShape &s, const ias_heads *q, const ias_heads *k,
                        const ias_heads *v, const int32_t *blocks, const ias_heads *out, float *lse, const Rows &r) {
-    return r.waves == 4   ? attend_waves<T, DP, ROWS, 4>(a, s, q, k, v, blocks, out, lse, r)
-           : r.waves == 2 ? attend_waves<T, DP, ROWS, 2>(a, s, q, k, v, blocks, out, lse, r)
-                          : attend_waves<T, DP, ROWS, 1>(a, s, q, k, v, blocks, out, lse, r);
+    if constexpr (ROWS == 16) return attend_waves<T, DP, ROWS, 8>(a, s, q, k, v, blocks, out, lse, r);
+    else
+        return r.waves == 4   ? attend_waves<T, DP, ROWS, 4>(a, s, q, k, v, blocks, out, lse, r)
+               : r.waves == 2 ? attend_waves<T, DP, ROWS, 2>(a, s, q, k, v, blocks, out, lse, r)
+                              : attend_waves<T, DP, ROWS, 1>(a, s, q, k, v, blocks, out, lse, r);
 }
 
 template <class T>
 ias_status attend(const ias_attention *a, const ias_heads *q, const ias_heads *k, const ias_heads *v,
                   const int32_t *blocks, const ias_heads *out, float *lse, const Forward &f) {
     dev::AttnShape s = shape_of(a);
-    if (a->table) IAS_TRY(bucket_map(a, s, f.map));
     const Rows &r = f.rows;
+    if (a->table && r.rows == 32) IAS_TRY(bucket_map(a, s, f.map));
     if (r.dp == 64)
         return r.rows == 16 ? attend_rows<T, 64, 16>(a, s, q, k, v, blocks, out, lse, r) : attend_rows<T, 64, 32>(a, s, q, k, v, blocks, out, lse, r);
     return r.rows == 16 ? attend_rows<T, 128, 16>(a, s, q, k, v, blocks, out, lse, r) : attend_rows<T, 128, 32>(a, s, q, k, v, blocks, out, lse, r);
@@ -310,9 +325,11 @@ template <class T, int DP, int ROWS>
 ias_status grad_rows(const ias_attention *a, const dev::AttnShape &s, const dev::GradPlan &p, int waves, const ias_heads *dout,
                      const ias_heads *q, const ias_heads *k, const ias_heads *v, const ias_heads *out, const float *lse,
                      const int32_t *blocks, const ias_heads *dq) {
-    return waves == 4   ? grad_waves<T, DP, ROWS, 4>(a, s, p, dout, q, k, v, out, lse, blocks, dq)
-           : waves == 2 ? grad_waves<T, DP, ROWS, 2>(a, s, p, dout, q, k, v, out, lse, blocks, dq)
-                        : grad_waves<T, DP, ROWS, 1>(a, s, p, dout, q, k, v, out, lse, blocks, dq);
+    if constexpr (ROWS == 16) return grad_waves<T, DP, ROWS, 4>(a, s, p, dout, q, k, v, out, lse, blocks, dq);
+    else
+        return waves == 4   ? grad_waves<T, DP, ROWS, 4>(a, s, p, dout, q, k, v, out, lse, blocks, dq)
+               : waves == 2 ? grad_waves<T, DP, ROWS, 2>(a, s, p, dout, q, k, v, out, lse, blocks, dq)
+                            : grad_waves<T, DP, ROWS, 1>(a, s, p, dout, q, k, v, out, lse, blocks, dq);
 }
 
 template <class T, int DP>

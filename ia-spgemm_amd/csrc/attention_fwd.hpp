@@ -344,6 +344,9 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan,
     const Tile<DP, ROWS> tile(lds + wave * 2 * Tile<DP>::BYTES, lane);   // K, then V
     constexpr int KT = 0, VT = Tile<DP>::BYTES;
 
+    // single tokens search the edges and save the map's launch
+    int32_t *edges = reinterpret_cast<int32_t *>(table + s.num_buckets * plan.span);
+    if (BIAS && ROWS == 16 && tid < s.num_buckets - 1) edges[tid] = s.edges[tid];
     if (BIAS)
         for (int e = tid; e < s.num_buckets * plan.span; e += 64 * W)
             if (h0 + e % plan.span < s.group) table[e] = T::up(s.table[(e / plan.span) * s.q_heads + g * s.group + h0 + e % plan.span]);
@@ -410,7 +413,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan,
 #pragma unroll
                 for (int n = 0; n < N; n += 4) {
                     uint32_t bucket;
-                    __builtin_memcpy(&bucket, s.map + ((int64_t)j0 + row.key(n) + 4 * row.part - row.pos + s.k_len - 1), 4);
+                    if (ROWS == 16) bucket = four_buckets(j0 + row.key(n) + 4 * row.part - row.pos, edges, s.num_buckets);
+                    else __builtin_memcpy(&bucket, s.map + ((int64_t)j0 + row.key(n) + 4 * row.part - row.pos + s.k_len - 1), 4);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         y[n + e] = __builtin_fmaf(y[n + e], c, table[(bucket >> (8 * e) & 255) * plan.span + row.head - h0]);

@@ -28,6 +28,7 @@ struct AttnShape {
     float scale;
     const int32_t *q_lens, *k_lens;
     const uint16_t *table;
+    const int32_t *edges;
     const uint8_t *map;       // bucket of each distance, map[d + k_len - 1]
     // r / group for r < 64 (group <= 64: the inverse is off by less than 2^-16)
     __device__ int per_group(int r) const { return (int)((uint32_t)r * inverse >> 16); }
@@ -101,20 +102,34 @@ __global__ __launch_bounds__(256) void k_block_summary(AttnShape s, Side k, int6
     }
 }
 
-// ------------------------------------------------------------------ bucket map
-// map[d + k_len - 1] = how many edges are <= d, for every distance of a call.
-__global__ __launch_bounds__(256) void k_bucket_map(int64_t k_len, int64_t n, int32_t num_buckets,
-                                                    const int32_t *__restrict__ edges, uint8_t *__restrict__ map) {
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (e >= n) return;
-    const int64_t d = e - (k_len - 1);
+// ------------------------------------------------------------------ buckets
+// How many of the ascending edges are <= d.
+__device__ inline int bucket_of(int64_t d, const int32_t *edges, int num_buckets) {
     int lo = 0, hi = num_buckets - 1;
     while (lo < hi) {
         const int mid = (lo + hi) / 2;
         if (edges[mid] <= d) lo = mid + 1;
         else hi = mid;
     }
-    map[e] = (uint8_t)lo;
+    return lo;
+}
+// The buckets of d .. d + 3, a byte each.
+__device__ inline uint32_t four_buckets(int d, const int32_t *edges, int num_buckets) {
+    int n = bucket_of(d, edges, num_buckets);
+    uint32_t got = n;
+    for (int e = 1; e < 4; ++e) {
+        while (n < num_buckets - 1 && edges[n] <= d + e) ++n;
+        got |= (uint32_t)n << (8 * e);
+    }
+    return got;
+}
+
+// map[d + k_len - 1] = how many edges are <= d, for every distance of a call.
+__global__ __launch_bounds__(256) void k_bucket_map(int64_t k_len, int64_t n, int32_t num_buckets,
+                                                    const int32_t *__restrict__ edges, uint8_t *__restrict__ map) {
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (e >= n) return;
+    map[e] = (uint8_t)bucket_of(e - (k_len - 1), edges, num_buckets);
 }
 
 }  // namespace dev

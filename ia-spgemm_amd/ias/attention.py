@@ -32,15 +32,13 @@ def _device(t: torch.Tensor) -> int:
     return t.device.index
 
 
-def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device.index).cuda_stream
+def _stream(device: int) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def _heads(t: torch.Tensor, shape, dtype, device, name: str) -> Heads:
-    if t.shape != shape:
-        raise ValueError(f"{name} is {tuple(t.shape)}, not {tuple(shape)}")
-    if t.dtype != dtype or t.device != device:
-        raise ValueError(f"{name} is {t.dtype} on {t.device}, not {dtype} on {device}")
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} is {t.dtype} {tuple(t.shape)} on {t.device}, not {dtype} {tuple(shape)} on {device}")
     s = t.stride()
     if s[3] != 1 and t.numel():
         raise ValueError(f"{name}: the last dimension has to be contiguous")
@@ -51,7 +49,7 @@ def _plain(t: Optional[torch.Tensor], shape, dtype, device, name: str) -> Option
     """Address of a contiguous tensor of that shape and type."""
     if t is None:
         return None
-    if t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
+    if not t.is_contiguous() or t.shape != shape or t.dtype != dtype or t.device != device:
         raise ValueError(f"{name} has to be a contiguous {dtype} {tuple(shape)} on {device}, not {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
@@ -61,7 +59,7 @@ def _attention(like: torch.Tensor, batch, q_len, k_len, q_heads, k_heads, dim, b
     device, dtype = _device(like), _DTYPE.get(like.dtype)
     if dtype is None:
         raise ValueError(f"{like.dtype} is not supported")
-    a = Attention(dtype, device, _stream(like), batch, q_len, k_len, q_heads, k_heads, dim, block, keep, 1 if causal else 0,
+    a = Attention(dtype, device, _stream(device), batch, q_len, k_len, q_heads, k_heads, dim, block, keep, 1 if causal else 0,
                   float(scale) if scale is not None else (dim ** -0.5 if dim else 1.0), 0,
                   None if q_lens is None else _plain(q_lens, (batch,), torch.int32, like.device, "q_lens"),
                   None if k_lens is None else _plain(k_lens, (batch,), torch.int32, like.device, "k_lens"))
@@ -76,11 +74,11 @@ def _attention(like: torch.Tensor, batch, q_len, k_len, q_heads, k_heads, dim, b
     return a
 
 
-def _out(out, shape, like, lens, name="out"):
-    """`out`, or a new tensor: zeros where rows behind a sequence's end stay unwritten."""
-    if out is not None:
-        return out
-    return (torch.empty if lens is None else torch.zeros)(shape, dtype=like.dtype, device=like.device)
+def _new(shape, dtype, device, lens):
+    """A tensor and its description: zeros where rows behind a sequence's end stay unwritten."""
+    t = (torch.empty if lens is None else torch.zeros)(shape, dtype=dtype, device=device)
+    _, n, h, d = shape
+    return t, Heads(t.data_ptr(), n * h * d, h * d, d)
 
 
 def block_summary(k: torch.Tensor, *, block: int = 64, k_lens: Optional[torch.Tensor] = None, fresh: int = 0,
@@ -128,11 +126,11 @@ def _shapes(q, k, blocks, block, causal, scale, q_lens, k_lens, table, edges):
     return a, (b, n, hq, d), (b, nk, hkv, d), _plain(blocks, (b, hkv, n, blocks.shape[-1]), torch.int32, q.device, "blocks")
 
 
-def _workspace(a: Attention, like: torch.Tensor, backward: bool):
+def _workspace(pa, device, backward: bool):
     n = C.c_int64(0)
-    check(lib.ias_block_attention_workspace(C.byref(a), None if backward else C.byref(n), C.byref(n) if backward else None),
+    check(lib.ias_block_attention_workspace(pa, None if backward else C.byref(n), C.byref(n) if backward else None),
           "ias_block_attention_workspace")
-    return (torch.empty(n.value, dtype=torch.uint8, device=like.device) if n.value else None), n.value
+    return (torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None), n.value
 
 
 def _address(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -148,13 +146,18 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, blocks: t
     logarithm of each row's sum, (batch, q_heads, q_len) in fp32.  Rows behind
     q_lens are 0 / -inf in new tensors and left alone in a given `out`."""
     a, qs, ks, pb = _shapes(q, k, blocks, block, causal, scale, q_lens, k_lens, table, edges)
-    out = _out(out, qs, q, q_lens)
-    lse = torch.empty((qs[0], qs[2], qs[1]), dtype=torch.float32, device=q.device) if q_lens is None else \
-        torch.full((qs[0], qs[2], qs[1]), float("-inf"), dtype=torch.float32, device=q.device)
-    ws, n = _workspace(a, q, False)
-    h = [_heads(t, s, q.dtype, q.device, x) for t, s, x in ((q, qs, "q"), (k, ks, "k"), (v, ks, "v"), (out, qs, "out"))]
-    check(lib.ias_block_attention(C.byref(a), C.byref(h[0]), C.byref(h[1]), C.byref(h[2]), pb, C.byref(h[3]),
-                                  lse.data_ptr(), _address(ws), n), "ias_block_attention")
+    dtype, device = q.dtype, q.device
+    if out is None:
+        out, ho = _new(qs, dtype, device, q_lens)
+    else:
+        ho = _heads(out, qs, dtype, device, "out")
+    lse = torch.empty((qs[0], qs[2], qs[1]), dtype=torch.float32, device=device) if q_lens is None else \
+        torch.full((qs[0], qs[2], qs[1]), float("-inf"), dtype=torch.float32, device=device)
+    pa = C.byref(a)
+    ws, n = _workspace(pa, device, False)
+    check(lib.ias_block_attention(pa, C.byref(_heads(q, qs, dtype, device, "q")), C.byref(_heads(k, ks, dtype, device, "k")),
+                                  C.byref(_heads(v, ks, dtype, device, "v")), pb, C.byref(ho), lse.data_ptr(), _address(ws), n),
+          "ias_block_attention")
     return out, lse
 
 
@@ -166,15 +169,15 @@ def block_attention_grad(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v
     """(dq, dk, dv, dtable) from the forward call's arguments and results;
     dtable is None without a table."""
     a, qs, ks, pb = _shapes(q, k, blocks, block, causal, scale, q_lens, k_lens, table, edges)
-    dq, dk, dv = _out(None, qs, q, q_lens), _out(None, ks, q, k_lens), _out(None, ks, q, k_lens)
+    dtype, device = q.dtype, q.device
+    (dq, hq), (dk, hk), (dv, hv) = _new(qs, dtype, device, q_lens), _new(ks, dtype, device, k_lens), _new(ks, dtype, device, k_lens)
     dtable = None if table is None else torch.empty_like(table)
-    pl = _plain(lse, (qs[0], qs[2], qs[1]), torch.float32, q.device, "lse")
-    ws, n = _workspace(a, q, True)
-    h = [_heads(t, s, q.dtype, q.device, x) for t, s, x in (
-        (dout, qs, "dout"), (q, qs, "q"), (k, ks, "k"), (v, ks, "v"), (out, qs, "out"), (dq, qs, "dq"), (dk, ks, "dk"),
-        (dv, ks, "dv"))]
-    p = [C.byref(x) for x in h]
-    check(lib.ias_block_attention_grad(C.byref(a), p[0], p[1], p[2], p[3], p[4], pl, pb, p[5], p[6], p[7],
+    pl = _plain(lse, (qs[0], qs[2], qs[1]), torch.float32, device, "lse")
+    pa = C.byref(a)
+    ws, n = _workspace(pa, device, True)
+    p = [C.byref(_heads(t, s, dtype, device, x)) for t, s, x in (
+        (dout, qs, "dout"), (q, qs, "q"), (k, ks, "k"), (v, ks, "v"), (out, qs, "out"))]
+    check(lib.ias_block_attention_grad(pa, p[0], p[1], p[2], p[3], p[4], pl, pb, C.byref(hq), C.byref(hk), C.byref(hv),
                                        _address(dtable), _address(ws), n),
           "ias_block_attention_grad")
     return dq, dk, dv, dtable
@@ -190,7 +193,7 @@ def rel_bias(table: torch.Tensor, edges: torch.Tensor, q_len: int, k_len: int) -
     pe = _plain(edges, (edges.numel(),), torch.int32, table.device, "edges") or pt
     out = torch.empty((table.shape[1], q_len, k_len), dtype=table.dtype, device=table.device)
     check(lib.ias_rel_bias(_DTYPE[table.dtype], table.shape[1], q_len, k_len, table.shape[0], pt, pe, out.data_ptr(),
-                           device, _stream(table)), "ias_rel_bias")
+                           device, _stream(device)), "ias_rel_bias")
     return out
 
 
@@ -211,5 +214,5 @@ def rel_bias_grad(grad: torch.Tensor, edges: torch.Tensor) -> torch.Tensor:
     ws = torch.empty(need.value, dtype=torch.uint8, device=grad.device)
     check(lib.ias_rel_bias_grad(_DTYPE[grad.dtype], b, h, n, m, buckets, grad.data_ptr(), grad.stride(0), grad.stride(1),
                                 grad.stride(2), pe or out.data_ptr(), out.data_ptr(), ws.data_ptr(), need.value, device,
-                                _stream(grad)), "ias_rel_bias_grad")
+                                _stream(device)), "ias_rel_bias_grad")
     return out

@@ -199,7 +199,7 @@ struct Backward {
     dev::GradPlan q{};
     dev::KeyPlan k{};
     uint32_t *bits;
-    int32_t *count, *first;
+    int32_t *count, *first, *slot;
     int64_t items;      // at most
     explicit Backward(const ias_attention *a, Space &w) : rows(a) {
         const int64_t group = a->q_heads / a->k_heads, bh = a->batch * a->k_heads, nblocks = ceil_div(a->k_len, a->block);
@@ -209,16 +209,20 @@ struct Backward {
         q.delta = w.part<float>(a->batch * a->q_heads * a->q_len);
         q.sums = a->table ? w.part<float>(bh * q.tiles * q.span * a->num_buckets) : nullptr;
         k.nw = (int32_t)ceil_div(a->q_len, 32);
-        const int64_t rows_all = a->batch * a->q_heads * a->q_len * std::min<int64_t>(a->keep, nblocks);
-        k.per = (int32_t)(std::min<int64_t>(1024, std::max<int64_t>(256, rows_all / 1024)) / group);
         k.subs = a->block / 64;
         k.entries = bh * nblocks;
-        items = k.entries + bh * a->q_len * std::min<int64_t>(a->keep, nblocks) / k.per;
+        const int64_t chosen = bh * a->q_len * std::min<int64_t>(a->keep, nblocks);   // entries of the pattern, at most
+        // a block with two items or more has over `per` queries: at most 2 chosen / per results to join
+        const int64_t result = (int64_t)k.subs * 2 * 64 * rows.dp * 4;
+        k.per = (int32_t)(std::min<int64_t>(1024, std::max<int64_t>(256, chosen * group / 1024)) / group);
+        k.per = (int32_t)std::min<int64_t>(8192, std::max<int64_t>(k.per, ceil_div(2 * chosen * result, 1ll << 30)));
+        items = k.entries + chosen / k.per;
         k.bits = bits = w.part<uint32_t>(k.entries * k.nw);
         k.count = count = w.part<int32_t>(k.entries);
         k.first = first = w.part<int32_t>(k.entries + 1);
+        k.slot = slot = w.part<int32_t>(k.entries + 1);
         k.delta = q.delta;
-        k.part = w.part<float>(items * k.subs * 2 * 64 * rows.dp);
+        k.part = w.part<float>(2 * chosen / k.per * result / 4);
     }
 };
 
@@ -349,7 +353,7 @@ ias_status grad_all(const ias_attention *a, const ias_heads *dout, const ias_hea
         IAS_TRY((launch<dev::k_clear>(a->device, ceil_div(w.k.entries, 256), 256, 0, a->stream, w.k.entries, w.count)));
         if (a->q_len > 0)
             IAS_TRY((launch<dev::k_invert>(a->device, bh * w.k.nw, 256, 4 * (size_t)s.nblocks, a->stream, s, w.k.nw, blocks, w.bits, w.count)));
-        IAS_TRY((launch<dev::k_items>(a->device, 1, 1024, 0, a->stream, w.k.entries, w.k.per, w.count, w.first)));
+        IAS_TRY((launch<dev::k_items>(a->device, 1, 1024, 0, a->stream, w.k.entries, w.k.per, w.count, w.first, w.slot)));
         const size_t lds = 4 * 32 * (size_t)DP * 2 + 2 * 5 * 32 * 4 + 4 * (size_t)w.k.per + 32 + 4 * (size_t)s.group * s.num_buckets;
         const int64_t grid = ceil_div(w.items * w.k.subs, 8) * 8;
         if (a->q_len > 0) {

@@ -283,27 +283,42 @@ __global__ __launch_bounds__(256) inline void k_invert(AttnShape s, int32_t nw, 
     }
 }
 
-// first[e] = items of the blocks before e, an item being up to `per` queries of a block; first[n] = all.
-__global__ __launch_bounds__(1024) inline void k_items(int64_t n, int32_t per, const int32_t *__restrict__ count, int32_t *__restrict__ first) {
-    __shared__ int32_t part[1024];
+// first[e] = items of the blocks before e, an item being up to `per` queries of a block;
+// slot[e] = items before e of blocks with more than one, whose results are joined.
+// first[n], slot[n] = all.
+__global__ __launch_bounds__(1024) inline void k_items(int64_t n, int32_t per, const int32_t *__restrict__ count, int32_t *__restrict__ first,
+                                                       int32_t *__restrict__ slot) {
+    __shared__ int32_t part[2][1024];
     const int tid = threadIdx.x;
     const int64_t share = (n + 1023) / 1024, lo = min(n, tid * share), hi = min(n, lo + share);
-    int32_t sum = 0;
-    for (int64_t e = lo; e < hi; ++e) sum += (count[e] + per - 1) / per;
-    part[tid] = sum;
+    int32_t sum = 0, many = 0;
+    for (int64_t e = lo; e < hi; ++e) {
+        const int32_t items = (count[e] + per - 1) / per;
+        sum += items;
+        many += items > 1 ? items : 0;
+    }
+    part[0][tid] = sum;
+    part[1][tid] = many;
     __syncthreads();
     for (int d = 1; d < 1024; d <<= 1) {
-        const int32_t t = tid >= d ? part[tid - d] : 0;
+        const int32_t s = tid >= d ? part[0][tid - d] : 0, m = tid >= d ? part[1][tid - d] : 0;
         __syncthreads();
-        part[tid] += t;
+        part[0][tid] += s;
+        part[1][tid] += m;
         __syncthreads();
     }
-    int32_t at = part[tid] - sum;
+    int32_t at = part[0][tid] - sum, of = part[1][tid] - many;
     for (int64_t e = lo; e < hi; ++e) {
+        const int32_t items = (count[e] + per - 1) / per;
         first[e] = at;
-        at += (count[e] + per - 1) / per;
+        slot[e] = of;
+        at += items;
+        of += items > 1 ? items : 0;
     }
-    if (tid == 1023) first[n] = part[1023];
+    if (tid == 1023) {
+        first[n] = part[0][1023];
+        slot[n] = part[1][1023];
+    }
 }
 
 __global__ __launch_bounds__(256) inline void k_clear(int64_t n, int32_t *__restrict__ p) {
@@ -316,9 +331,9 @@ struct KeyPlan {
     int32_t nw, per, subs;      // words of a block's bits, queries of an item, 64-key parts of a block
     int64_t entries;            // batch x k_heads x nblocks
     const uint32_t *bits;
-    const int32_t *count, *first;
+    const int32_t *count, *first, *slot;
     const float *delta;
-    float *part;                // [item][sub][dk, dv][64][DP] of blocks with more than one item
+    float *part;                // [slot][sub][dk, dv][64][DP]: items of blocks with more than one
 };
 
 // One workgroup for an item and 64 of its block's keys; wave w has 16 of them,
@@ -478,7 +493,7 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
     if (tid == 0) scratch[0] = 0;
     __syncthreads();
     const bool alone = items == 1;
-    float *const parts = plan.part + ((int64_t)item * plan.subs + sub) * 2 * 64 * DP;
+    float *const parts = plan.part + ((int64_t)(plan.slot[entry] + part) * plan.subs + sub) * 2 * 64 * DP;   // not if alone
     bool fine = true;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -565,7 +580,7 @@ __global__ __launch_bounds__(256) void k_grad_kv_join(AttnShape s, KeyPlan plan,
     const int c = (int)(entry % s.nblocks), g = (int)(entry / s.nblocks % s.k_heads), b = (int)(entry / s.nblocks / s.k_heads);
     const int n = blockIdx.x % 4 * 16 + threadIdx.x / 16, d = threadIdx.x % 16 * 8, j = c * s.block + sub * 64 + n;
     if (j >= s.kl(b) || d >= s.dim) return;
-    const f32x4 *from = reinterpret_cast<const f32x4 *>(plan.part + (((int64_t)first * plan.subs + sub) * 2 * 64 + n) * dp + d);
+    const f32x4 *from = reinterpret_cast<const f32x4 *>(plan.part + (((int64_t)plan.slot[entry] * plan.subs + sub) * 2 * 64 + n) * dp + d);
     const int64_t step = (int64_t)plan.subs * 2 * 64 * dp / 4, other = 64 * dp / 4;
     f32x4 x[2] = {}, y[2] = {};
     for (int t0 = 0; t0 < items; t0 += 4) {

@@ -193,7 +193,7 @@ ias_status check_bias(int32_t dtype, int64_t batch, int32_t heads, int64_t q_len
         REFUSE(IAS_ERROR_INVALID_ARGUMENT, "batch %lld, heads %d, q_len %lld, k_len %lld, device %d", (long long)batch, heads,
                (long long)q_len, (long long)k_len, device);
     if (nb < 1 || nb > 64) REFUSE(IAS_ERROR_UNSUPPORTED, "%d buckets: 1 to 64", nb);
-    if (batch > INT32_MAX || heads > 1 << 20 || q_len > 1 << 24 || k_len > 1 << 24 ||
+    if (batch > INT32_MAX || heads > 1 << 16 || q_len > 1 << 24 || k_len > 1 << 24 ||
         (q_len > 0 && k_len > (1ll << 41) / q_len) || (q_len > 0 && batch * heads > INT64_MAX / 16 / q_len / std::max<int64_t>(1, k_len)))
         REFUSE(IAS_ERROR_OVERFLOW, "batch x heads x q_len x k_len is too large");
     return IAS_SUCCESS;

@@ -496,3 +496,67 @@ def test_select_where_scores_are_close(A, kind, m):
         s, q = (x * (2.0 ** (100 if kind == "huge" else -100)) for x in (s, q))
     got = A.block_select(q, s, keep, k_len=m * 64, first=1, local=1)
     assert torch.equal(got.cpu(), ref.select(q, s, keep, m * 64, 64, True, 1, 1, None, None))
+
+
+@gpu
+def test_offsets_beyond_32_bits(A):
+    """A cache of 2^20 tokens inside a wider tensor of over 2^32 bytes."""
+    n = 1 << 20
+    c = case(b=1, sq=2, sk=n, hq=2, hkv=1, d=128, keep=5, nb=6)
+    s = make(dict(c, sk=64))
+    wide = torch.zeros(1, n, 20, 128, dtype=torch.bfloat16, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(16)
+    s["k"], s["v"] = wide[:, :, 18:19], wide[:, :, 19:20]
+    for x in (s["k"], s["v"]):
+        x.copy_(torch.randn(1, n, 1, 128, device="cuda", generator=gen))
+    s["blocks"] = torch.tensor([[0, 16383, 5000, 16382, 12345], [16383, 1, 9, -1, -1]], dtype=torch.int32,
+                               device="cuda").view(1, 1, 2, 5)
+    s["edges"] = torch.tensor([-(1 << 19), -5000, -64, -3, 0], dtype=torch.int32, device="cuda")
+    check(A, c, s)
+    m = A.block_summary(s["k"])
+    got = A.block_select(s["q"], m, 5, k_len=n)
+    assert torch.equal(got.cpu(), ref.select(s["q"], m, 5, n, 64, True, 1, 1, None, None))
+
+
+@gpu
+def test_nothing_to_read_and_nobody_to_ask(A):
+    """No keys: zeros.  No queries: gradients of the keys are zeros."""
+    z = lambda *s: torch.randn(*s, device="cuda").to(torch.bfloat16)  # noqa: E731
+    blocks = torch.zeros(2, 1, 3, 4, dtype=torch.int32, device="cuda")
+    q, k = z(2, 3, 4, 64), z(2, 0, 1, 64)
+    table, edges = z(5, 4), torch.arange(-3, 1, dtype=torch.int32, device="cuda")
+    for bias in ({}, dict(table=table, edges=edges)):
+        out, lse = A.block_attention(q, k, k, blocks, **bias)
+        assert (out == 0).all() and (lse == -math.inf).all()
+        dq, dk, dv, dt = A.block_attention_grad(q, q, k, k, out, lse, blocks, **bias)
+        assert (dq == 0).all() and dk.shape == k.shape and (dt is None or (dt == 0).all())
+    m = A.block_summary(k)
+    assert m.shape == (2, 1, 0, 64) and (A.block_select(q, m, 4, k_len=0) == -1).all()
+    q, k = z(2, 0, 4, 64), z(2, 70, 1, 64)
+    out, lse = A.block_attention(q, k, k, blocks[:, :, :0].contiguous(), table=table, edges=edges)
+    assert out.shape == q.shape
+    dq, dk, dv, dt = A.block_attention_grad(q, q, k, k, out, lse, blocks[:, :, :0].contiguous(), table=table, edges=edges)
+    assert (dk == 0).all() and (dv == 0).all() and (dt == 0).all()
+    assert A.block_select(q, A.block_summary(k), 4, k_len=70).shape == (2, 1, 0, 4)
+    assert A.rel_bias(table, edges, 0, 7).shape == (4, 0, 7)
+    assert (A.rel_bias_grad(z(1, 4, 0, 7), edges) == 0).all()
+
+
+@gpu
+def test_first_call_is_captured(A):
+    """A graph whose capture is the first call of its shapes, and two graphs replayed in turn."""
+    c = case("fp16", b=1, sq=90, sk=190, hq=2, hkv=2, d=120, block=128, keep=2, nb=40)
+    s, t = make(c, 17), make(c, 18)
+    graphs, held = [], []
+    for x in (s, t):
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out, lse = A.block_attention(x["q"], x["k"], x["v"], x["blocks"], **kw(c, x))
+            held.append((out, lse) + A.block_attention_grad(x["dout"], x["q"], x["k"], x["v"], out, lse, x["blocks"], **kw(c, x)))
+        graphs.append(g)
+    for turn in range(3):
+        for g, x, h in zip(graphs, (s, t), held):
+            g.replay()
+            for a, b in zip(h, check(A, c, x)):
+                assert torch.equal(a, b)

@@ -98,6 +98,7 @@ dev::AttnShape shape_of(const ias_attention *a) {
     s.inverse = (uint32_t)ceil_div(65536, s.group);
     s.inverse_keep = a->keep > 1 ? (uint32_t)ceil_div(1ll << 32, a->keep) : 0;
     s.dim = a->head_dim; s.block = a->block; s.keep = a->keep; s.causal = a->causal != 0;
+    s.clear = a->clear != 0;
     s.nblocks = (int32_t)ceil_div(a->k_len, a->block);
     s.scale = a->scale;
     s.q_lens = a->q_lens; s.k_lens = a->k_lens;

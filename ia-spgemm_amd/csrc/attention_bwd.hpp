@@ -56,6 +56,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
     const int g = (int)(w % s.k_heads), b = (int)(w / s.k_heads);
     const int ql = s.ql(b), kl = s.kl(b);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
+    if (s.clear && i0 + plan.nq > ql)
+        clear_rows(s, b, g, h0, min(plan.span, s.group - h0), max(i0, (int64_t)ql), min(i0 + plan.nq, s.q_len), dq, nullptr);
     if (i0 >= ql) {
         if (BIAS && plan.sums)
             for (int e = tid; e < plan.span * s.num_buckets; e += THREADS) plan.sums[tile_id * plan.span * s.num_buckets + e] = 0.0f;
@@ -569,17 +571,24 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
     }
 }
 
-// dk and dv of the blocks that no query or more than one item read: a thread for 8
-// channels of a key, 16 keys a workgroup.
+// dk and dv of the blocks that no query or more than one item read, and of the keys
+// behind a sequence's end: a thread for 8 channels of a key, 16 keys a workgroup.
 template <class T>
 __global__ __launch_bounds__(256) void k_grad_kv_join(AttnShape s, KeyPlan plan, int32_t dp, SideOut dk, SideOut dv) {
     const int sub = (int)(blockIdx.x / 4 % plan.subs);
     const int64_t entry = blockIdx.x / 4 / plan.subs;
     const int32_t first = plan.first[entry], items = plan.first[entry + 1] - first;
-    if (items == 1) return;
     const int c = (int)(entry % s.nblocks), g = (int)(entry / s.nblocks % s.k_heads), b = (int)(entry / s.nblocks / s.k_heads);
     const int n = blockIdx.x % 4 * 16 + threadIdx.x / 16, d = threadIdx.x % 16 * 8, j = c * s.block + sub * 64 + n;
-    if (j >= s.kl(b) || d >= s.dim) return;
+    if (d >= s.dim) return;
+    if (j >= s.kl(b)) {
+        if (s.clear && j < s.k_len) {
+            *reinterpret_cast<s16x8 *>(dk.at(b, j, g) + d) = s16x8{};
+            *reinterpret_cast<s16x8 *>(dv.at(b, j, g) + d) = s16x8{};
+        }
+        return;
+    }
+    if (items == 1) return;
     const f32x4 *from = reinterpret_cast<const f32x4 *>(plan.part + (((int64_t)plan.slot[entry] * plan.subs + sub) * 2 * 64 + n) * dp + d);
     const int64_t step = (int64_t)plan.subs * 2 * 64 * dp / 4, other = 64 * dp / 4;
     f32x4 x[2] = {}, y[2] = {};

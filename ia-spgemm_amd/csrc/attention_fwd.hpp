@@ -313,6 +313,16 @@ inline size_t attend_lds(int dp, int rows, int waves, int nblocks, int most, int
     return walk_area(dp, rows, waves) + 8 * (size_t)((nblocks + 31) / 32) + 8 * (size_t)most + waves * (size_t)rows * 2 * 4 + 16 + 4 * (size_t)table;
 }
 
+// Zeros (and lse -inf) for the queries [from, to) of a tile, those behind a sequence's end.
+__device__ inline void clear_rows(const AttnShape &s, int b, int g, int h0, int heads, int64_t from, int64_t to, const SideOut &out, float *lse) {
+    const int chunks = s.dim / 8, each = heads * chunks;
+    for (int64_t e = threadIdx.x; e < (to - from) * each; e += blockDim.x) {
+        const int64_t i = from + e / each, h = (int64_t)g * s.group + h0 + e % each / chunks;
+        *reinterpret_cast<s16x8 *>(out.at(b, i, h) + e % chunks * 8) = s16x8{};
+        if (lse && e % chunks == 0) lse[((int64_t)b * s.q_heads + h) * s.q_len + i] = -INFINITY;
+    }
+}
+
 template <class T, int DP, int ROWS, int W, bool BIAS>
 __global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan, Side q, Side k, Side v,
                                                       const int32_t *__restrict__ blocks, SideOut out, float *__restrict__ lse) {
@@ -338,6 +348,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan,
     w /= plan.tiles;
     const int g = (int)(w % s.k_heads), b = (int)(w / s.k_heads);
     const int ql = s.ql(b), kl = s.kl(b);
+    if (s.clear && split == 0 && i0 + plan.nq > ql)
+        clear_rows(s, b, g, h0, min(plan.span, s.group - h0), max(i0, (int64_t)ql), min(i0 + plan.nq, s.q_len), out, lse);
     if (i0 >= ql) return;
     const int nq = min(plan.nq, ql - (int)i0), rows = (nq - 1) * plan.span + min(plan.span, s.group - h0);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;

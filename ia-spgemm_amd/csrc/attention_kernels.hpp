@@ -23,7 +23,7 @@ struct SideOut {
 };
 struct AttnShape {
     int64_t q_len, k_len;
-    int32_t batch, q_heads, k_heads, group, dim, block, keep, causal, nblocks, num_buckets;
+    int32_t batch, q_heads, k_heads, group, dim, block, keep, causal, nblocks, num_buckets, clear;
     uint32_t inverse, inverse_keep;   // ceil(2^16 / group), ceil(2^32 / keep) (0 for keep = 1)
     float scale;
     const int32_t *q_lens, *k_lens;

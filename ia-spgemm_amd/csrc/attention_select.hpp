@@ -337,6 +337,11 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 256) void k_block_select(AttnShape
     w /= plan.tiles;
     const int g = (int)(w % s.k_heads), b = (int)(w / s.k_heads);
     const int ql = s.ql(b), kl = s.kl(b);
+    if (s.clear && i0 + plan.nq > ql) {   // queries behind the sequence's end
+        const int64_t from = max(i0, ql), to = min((int64_t)i0 + plan.nq, s.q_len);
+        for (int64_t e = threadIdx.x; e < (to - from) * s.keep; e += blockDim.x)
+            blocks[((((int64_t)b * s.k_heads + g) * s.q_len) + from) * s.keep + e] = -1;
+    }
     if (i0 >= ql) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), waves = blockDim.x / 64;
     const int lane = tid % 64, col = lane & 15, quad = lane >> 4;

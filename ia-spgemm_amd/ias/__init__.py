@@ -101,7 +101,8 @@ class Attention(C.Structure):
                 ("q_heads", C.c_int32), ("k_heads", C.c_int32), ("head_dim", C.c_int32),
                 ("block", C.c_int32), ("keep", C.c_int32), ("causal", C.c_int32),
                 ("scale", C.c_float), ("num_buckets", C.c_int32),
-                ("q_lens", C.c_void_p), ("k_lens", C.c_void_p), ("table", C.c_void_p), ("edges", C.c_void_p)]
+                ("q_lens", C.c_void_p), ("k_lens", C.c_void_p), ("table", C.c_void_p), ("edges", C.c_void_p),
+                ("clear", C.c_int32), ("reserved", C.c_int32)]
 
 
 # every symbol include/ias.h declares (checked by tests/test_abi.py)

@@ -74,9 +74,9 @@ def _attention(like: torch.Tensor, batch, q_len, k_len, q_heads, k_heads, dim, b
     return a
 
 
-def _new(shape, dtype, device, lens):
-    """A tensor and its description: zeros where rows behind a sequence's end stay unwritten."""
-    t = (torch.empty if lens is None else torch.zeros)(shape, dtype=dtype, device=device)
+def _new(shape, dtype, device):
+    """A tensor and its description."""
+    t = torch.empty(shape, dtype=dtype, device=device)
     _, n, h, d = shape
     return t, Heads(t.data_ptr(), n * h * d, h * d, d)
 
@@ -108,9 +108,8 @@ def block_select(q: torch.Tensor, summary: torch.Tensor, keep: int, *, k_len: in
     a = _attention(q, b, n, k_len, hq, summary.shape[1], d, block, keep, causal, None, q_lens, k_lens)
     m = -(-k_len // block) if block > 0 else 0
     if out is None:
-        shape = (b, summary.shape[1], n, max(keep, 0))
-        out = torch.empty(shape, dtype=torch.int32, device=q.device) if q_lens is None else \
-            torch.full(shape, -1, dtype=torch.int32, device=q.device)
+        out = torch.empty((b, summary.shape[1], n, max(keep, 0)), dtype=torch.int32, device=q.device)
+        a.clear = 1
     check(lib.ias_block_select(C.byref(a), C.byref(_heads(q, q.shape, q.dtype, q.device, "q")),
                                _plain(summary, (b, summary.shape[1], m, d), q.dtype, q.device, "summary"), first,
                                local if causal else 0,
@@ -148,11 +147,13 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, blocks: t
     a, qs, ks, pb = _shapes(q, k, blocks, block, causal, scale, q_lens, k_lens, table, edges)
     dtype, device = q.dtype, q.device
     if out is None:
-        out, ho = _new(qs, dtype, device, q_lens)
+        out, ho = _new(qs, dtype, device)
+        a.clear = 1
     else:
         ho = _heads(out, qs, dtype, device, "out")
-    lse = torch.empty((qs[0], qs[2], qs[1]), dtype=torch.float32, device=device) if q_lens is None else \
-        torch.full((qs[0], qs[2], qs[1]), float("-inf"), dtype=torch.float32, device=device)
+    lse = torch.empty((qs[0], qs[2], qs[1]), dtype=torch.float32, device=device)
+    if not a.clear and q_lens is not None:
+        lse.fill_(float("-inf"))
     pa = C.byref(a)
     ws, n = _workspace(pa, device, False)
     check(lib.ias_block_attention(pa, C.byref(_heads(q, qs, dtype, device, "q")), C.byref(_heads(k, ks, dtype, device, "k")),
@@ -170,7 +171,8 @@ def block_attention_grad(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v
     dtable is None without a table."""
     a, qs, ks, pb = _shapes(q, k, blocks, block, causal, scale, q_lens, k_lens, table, edges)
     dtype, device = q.dtype, q.device
-    (dq, hq), (dk, hk), (dv, hv) = _new(qs, dtype, device, q_lens), _new(ks, dtype, device, k_lens), _new(ks, dtype, device, k_lens)
+    (dq, hq), (dk, hk), (dv, hv) = _new(qs, dtype, device), _new(ks, dtype, device), _new(ks, dtype, device)
+    a.clear = 1
     dtable = None if table is None else torch.empty_like(table)
     pl = _plain(lse, (qs[0], qs[2], qs[1]), torch.float32, device, "lse")
     pa = C.byref(a)

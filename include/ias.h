@@ -428,7 +428,8 @@ ias_status ias_dist_csr_mul_csr(ias_dist *dist, const ias_csr *A, const ias_csr 
  * element, NULL: all q_len / k_len; values are clamped to [0, q_len] and
  * [0, k_len]) query i stands at position i + k_lens[b] - q_lens[b], and causal
  * lets it read the keys up to that position.  Output rows at or beyond a
- * sequence's length are not written.  What a padded or masked key, or one of a
+ * sequence's length are not written, or with `clear` written as 0 (lse:
+ * -infinity, blocks: -1).  What a padded or masked key, or one of a
  * block that a query did not choose, holds (infinities and NaN too) does not
  * reach that query's results.
  *
@@ -463,6 +464,8 @@ typedef struct ias_attention {
     const int32_t *q_lens, *k_lens;
     const void    *table;
     const int32_t *edges;
+    int32_t clear;                /* rows behind a sequence's end: 0 left alone, 1 cleared */
+    int32_t reserved;
 } ias_attention;
 
 /* summary (batch x k_heads x ceil(k_len / block) x head_dim, of the call's

@@ -247,10 +247,15 @@ ias_status launch(int device, int64_t grid, int threads, size_t lds, void *strea
     return launched();
 }
 
+// Workgroups for tile_of: 8 dies, each with its share of a head's tiles or of all.
+int64_t tile_grid(int64_t heads, int64_t each) {
+    return 8 * (heads < 8 && 8 % heads == 0 ? ceil_div(each, 8 / heads) : ceil_div(heads * each, 8));
+}
+
 template <class T, int DP, int MT>
 ias_status select_rows(const ias_attention *a, const dev::AttnShape &s, const dev::SelectPlan &p, int threads, const ias_heads *q,
                        const void *summary, int32_t *blocks) {
-    const int64_t grid = ceil_div(a->batch * a->k_heads * p.tiles, 8) * 8;
+    const int64_t grid = tile_grid(a->batch * a->k_heads, p.tiles);
     return launch<dev::k_block_select<T, DP, MT>>(a->device, grid, threads, dev::select_lds(p.nq, p.stride, threads / 64), a->stream, s, p, side(q),
                   static_cast<const uint16_t *>(summary), blocks);
 }
@@ -279,7 +284,7 @@ ias_status select(const ias_attention *a, const ias_heads *q, const void *summar
 template <class T, int DP, int ROWS, int W>
 ias_status attend_waves(const ias_attention *a, const dev::AttnShape &s, const ias_heads *q, const ias_heads *k,
                        const ias_heads *v, const int32_t *blocks, const ias_heads *out, float *lse, const Rows &r) {
-    const int64_t grid = ceil_div(r.tiles * r.plan.splits, 8) * 8;
+    const int64_t grid = tile_grid(a->batch * a->k_heads, (int64_t)r.plan.tiles * r.plan.splits);
     const size_t lds = dev::attend_lds(DP, ROWS, W, s.nblocks, r.plan.most, s.num_buckets * (r.plan.span + 1));
     if (a->table)
         IAS_TRY((launch<dev::k_attend<T, DP, ROWS, W, true>>(a->device, grid, 64 * W, lds, a->stream, s, r.plan, side(q), side(k), side(v), blocks, side_out(out), lse)));
@@ -316,7 +321,7 @@ template <class T, int DP, int ROWS, int W>
 ias_status grad_waves(const ias_attention *a, const dev::AttnShape &s, const dev::GradPlan &p, const ias_heads *dout, const ias_heads *q,
                       const ias_heads *k, const ias_heads *v, const ias_heads *out, const float *lse, const int32_t *blocks,
                       const ias_heads *dq) {
-    const int64_t tiles = a->batch * a->k_heads * p.tiles, grid = ceil_div(tiles, 8) * 8;
+    const int64_t grid = tile_grid(a->batch * a->k_heads, p.tiles);
     const int32_t area = dev::grad_q_area(DP, ROWS, W, s.num_buckets, p.sums);
     const size_t lds = dev::grad_q_lds(area, s.nblocks, p.most, p.span, s.num_buckets);
     if (a->table)

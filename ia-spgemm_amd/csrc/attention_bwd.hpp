@@ -47,8 +47,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
     uint32_t *words = masks + plan.most;
     float *table = reinterpret_cast<float *>(words + 2 * ((s.nblocks + 31) / 32));
 
-    int64_t w = work_of((int64_t)s.batch * s.k_heads * plan.tiles);
-    if (w >= (int64_t)s.batch * s.k_heads * plan.tiles) return;
+    int64_t w = tile_of((int64_t)s.batch * s.k_heads, plan.tiles);
+    if (w < 0) return;
     const int64_t tile_id = w;
     const int64_t i0 = (w % plan.tiles) / plan.parts * plan.nq;
     const int h0 = (int)(w % plan.tiles % plan.parts) * plan.span;
@@ -131,8 +131,10 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
             tile.fill(kr, KT);
             tile.fill(vr, VT);
             float x[N], y[N];
+            __builtin_amdgcn_s_setprio(1);
             scores<T, DP, ROWS>(tile, KT, qf, x);
             scores<T, DP, ROWS>(tile, VT, df, y);
+            __builtin_amdgcn_s_setprio(0);
             const int jn = __builtin_amdgcn_readfirstlane(id) * s.block + at.part * 32;
             const uint32_t maskn = __builtin_amdgcn_readfirstlane(chose) & only;
             if (more) {
@@ -179,7 +181,9 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
                     }
                 }
             }
+            __builtin_amdgcn_s_setprio(1);
             products<T, DP, ROWS>(tile, KT, y, o);
+            __builtin_amdgcn_s_setprio(0);
             j0 = jn;
             mask = maskn;
         }
@@ -355,8 +359,8 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
     float *table = reinterpret_cast<float *>(scratch + 8);
 
     const int64_t total = (int64_t)plan.first[plan.entries] * plan.subs;
-    int64_t w = work_of((int64_t)gridDim.x);
-    if (w >= total) return;
+    const int64_t w = work_of(total);
+    if (w < 0) return;
     const int sub = (int)(w % plan.subs);
     const int32_t item = (int32_t)(w / plan.subs);
     int64_t lo = 0, hi = plan.entries;   // the block with first[e] <= item < first[e + 1]

@@ -331,8 +331,8 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 256) void k_block_select(AttnShape
     constexpr int KS = DP / 32;
     extern __shared__ uint32_t keys[];                       // [nq][stride], then the norms, then each wave's bits
     uint32_t *qnorm = keys + plan.nq * plan.stride, *mnorm = qnorm + plan.nq;
-    int64_t w = work_of((int64_t)s.batch * s.k_heads * plan.tiles);
-    if (w >= (int64_t)s.batch * s.k_heads * plan.tiles) return;
+    int64_t w = tile_of((int64_t)s.batch * s.k_heads, plan.tiles);
+    if (w < 0) return;
     const int i0 = (int)(w % plan.tiles) * plan.nq;
     w /= plan.tiles;
     const int g = (int)(w % s.k_heads), b = (int)(w / s.k_heads);

@@ -47,13 +47,12 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
     uint32_t *words = masks + plan.most;
     float *table = reinterpret_cast<float *>(words + 2 * ((s.nblocks + 31) / 32));
 
-    int64_t w = tile_of((int64_t)s.batch * s.k_heads, plan.tiles);
-    if (w < 0) return;
-    const int64_t tile_id = w;
-    const int64_t i0 = (w % plan.tiles) / plan.parts * plan.nq;
-    const int h0 = (int)(w % plan.tiles % plan.parts) * plan.span;
-    w /= plan.tiles;
-    const int g = (int)(w % s.k_heads), b = (int)(w / s.k_heads);
+    const Part part = tile_of(s.batch * s.k_heads, plan.tiles);
+    if (part.head < 0) return;
+    const uint32_t step = (uint32_t)part.tile / (uint32_t)plan.parts;
+    const int64_t tile_id = (int64_t)part.head * plan.tiles + part.tile, i0 = (int64_t)step * plan.nq;
+    const int h0 = (int)(part.tile - step * plan.parts) * plan.span;
+    const int b = (uint32_t)part.head / (uint32_t)s.k_heads, g = part.head - b * s.k_heads;
     const int ql = s.ql(b), kl = s.kl(b);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
     if (s.clear && i0 + plan.nq > ql)
@@ -270,8 +269,9 @@ __global__ __launch_bounds__(256) void k_grad_table(AttnShape s, GradPlan plan, 
 __global__ __launch_bounds__(256) inline void k_invert(AttnShape s, int32_t nw, const int32_t *__restrict__ blocks,
                                                        uint32_t *__restrict__ bits, int32_t *__restrict__ count) {
     extern __shared__ uint32_t word[];   // nblocks
-    const int64_t bh = blockIdx.x / nw;
-    const int q32 = (int)(blockIdx.x % nw), b = (int)(bh / s.k_heads);
+    const uint32_t head = blockIdx.x / (uint32_t)nw;
+    const int64_t bh = head;
+    const int q32 = (int)(blockIdx.x - head * nw), b = (int)(head / (uint32_t)s.k_heads);
     const int ql = s.ql(b), kl = s.kl(b), i0 = q32 * 32;
     for (int c = threadIdx.x; c < s.nblocks; c += 256) word[c] = 0;
     __syncthreads();
@@ -358,20 +358,20 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
     int32_t *scratch = list + plan.per;                           // flag, prefix of the list's words
     float *table = reinterpret_cast<float *>(scratch + 8);
 
-    const int64_t total = (int64_t)plan.first[plan.entries] * plan.subs;
-    const int64_t w = work_of(total);
+    const int32_t w = work_of((uint32_t)plan.first[plan.entries] * plan.subs);
     if (w < 0) return;
-    const int sub = (int)(w % plan.subs);
-    const int32_t item = (int32_t)(w / plan.subs);
-    int64_t lo = 0, hi = plan.entries;   // the block with first[e] <= item < first[e + 1]
+    const int32_t item = (uint32_t)w / (uint32_t)plan.subs;
+    const int sub = w - item * plan.subs;
+    uint32_t lo = 0, hi = (uint32_t)plan.entries;   // the block with first[e] <= item < first[e + 1]
     while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) / 2;
+        const uint32_t mid = (lo + hi) / 2;
         if (plan.first[mid] <= item) lo = mid;
         else hi = mid;
     }
+    const uint32_t head = lo / (uint32_t)s.nblocks;
     const int64_t entry = lo;
     const int part = item - plan.first[entry], items = plan.first[entry + 1] - plan.first[entry];
-    const int c = (int)(entry % s.nblocks), g = (int)(entry / s.nblocks % s.k_heads), b = (int)(entry / s.nblocks / s.k_heads);
+    const int c = (int)(lo - head * s.nblocks), b = head / (uint32_t)s.k_heads, g = head - b * s.k_heads;
     const int ql = s.ql(b), kl = s.kl(b), j0 = c * s.block + sub * 64;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, col = lane & 15, quad = lane >> 4;
     const int nqueries = min(plan.per, plan.count[entry] - part * plan.per);
@@ -422,8 +422,8 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
         for (int n = 0; n < LD; ++n) {
             const int r = r0 + (n * 256 + tid) / CH, ch = tid % CH;
             const bool on = r < rows && ch * 8 < s.dim;
-            const int rr = min(r, rows - 1), i = list[rr / s.group], d = ch * 8 < s.dim ? ch * 8 : 0;
-            const int64_t h = (int64_t)g * s.group + rr % s.group;
+            const int rr = min(r, rows - 1), rq = (uint32_t)rr / (uint32_t)s.group, i = list[rq], d = ch * 8 < s.dim ? ch * 8 : 0;
+            const int64_t h = (int64_t)g * s.group + rr - rq * s.group;
             const s16x8 x = load8(q.at(b, i, h) + d), y = load8(dout.at(b, i, h) + d);
             qn[n] = on ? x : s16x8{};
             dn[n] = on ? y : s16x8{};
@@ -431,14 +431,14 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
         if (tid < 32) {
             const int r = r0 + tid;
             const bool on = r < rows;
-            const int rr = min(r, rows - 1), i = list[rr / s.group], p = i + kl - ql;
-            const int64_t at = ((int64_t)b * s.q_heads + (int64_t)g * s.group + rr % s.group) * s.q_len + i;
+            const int rr = min(r, rows - 1), rq = (uint32_t)rr / (uint32_t)s.group, i = list[rq], p = i + kl - ql;
+            const int64_t at = ((int64_t)b * s.q_heads + (int64_t)g * s.group + rr - rq * s.group) * s.q_len + i;
             const float l = on ? lse[at] : -INFINITY;
             fn[0] = l == -INFINITY ? INFINITY : BIAS ? l : l * LOG2E;
             fn[1] = plan.delta[at];
             fn[2] = __int_as_float(!on ? 0 : s.causal ? min(kl, p + 1) : kl);
             fn[3] = __int_as_float(p);
-            fn[4] = __int_as_float(rr % s.group);
+            fn[4] = __int_as_float(rr - rq * s.group);
         }
     };
     auto put = [&](int buf) {
@@ -579,10 +579,11 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
 // behind a sequence's end: a thread for 8 channels of a key, 16 keys a workgroup.
 template <class T>
 __global__ __launch_bounds__(256) void k_grad_kv_join(AttnShape s, KeyPlan plan, int32_t dp, SideOut dk, SideOut dv) {
-    const int sub = (int)(blockIdx.x / 4 % plan.subs);
-    const int64_t entry = blockIdx.x / 4 / plan.subs;
+    const uint32_t e = blockIdx.x / 4 / (uint32_t)plan.subs, head = e / (uint32_t)s.nblocks;
+    const int sub = (int)(blockIdx.x / 4 - e * plan.subs);
+    const int64_t entry = e;
     const int32_t first = plan.first[entry], items = plan.first[entry + 1] - first;
-    const int c = (int)(entry % s.nblocks), g = (int)(entry / s.nblocks % s.k_heads), b = (int)(entry / s.nblocks / s.k_heads);
+    const int c = (int)(e - head * s.nblocks), b = head / (uint32_t)s.k_heads, g = head - b * s.k_heads;
     const int n = blockIdx.x % 4 * 16 + threadIdx.x / 16, d = threadIdx.x % 16 * 8, j = c * s.block + sub * 64 + n;
     if (d >= s.dim) return;
     if (j >= s.kl(b)) {

@@ -154,25 +154,29 @@ __device__ inline void products(const Tile<DP, ROWS> &tile, int at, const float 
 // Which of `total` parts of the work a workgroup has, -1 if none.  Consecutive ids go to
 // the 8 dies in turn; each die gets a contiguous stretch, so that parts that read the same
 // K and V meet in one L2.
-__device__ inline int64_t work_of(int64_t total) {
-    const int64_t per = (total + 7) / 8, n = blockIdx.x / 8, w = (int64_t)(blockIdx.x % 8) * per + n;
-    return n < per && w < total ? w : -1;
+// (All parts of a call are fewer than 2^31: 32-bit divisions, which take a fraction of the
+// instructions.)
+__device__ inline int32_t work_of(uint32_t total) {
+    const uint32_t per = (total + 7) / 8, n = blockIdx.x / 8, w = blockIdx.x % 8 * per + n;
+    return n < per && w < total ? (int32_t)w : -1;
 }
 // The same for `each` tiles of `heads` key heads, the last tiles of a head first: those of
 // a causal call walk furthest, and short walks at the end even it out (8192 tokens 587 ->
 // 538 us).  Where fewer heads than dies divide them, a head's tiles go to its dies in turn,
 // since a stretch of a head's first ones would be the shorter work.
-__device__ inline int64_t tile_of(int64_t heads, int64_t each) {
-    int64_t w;
-    if (heads < 8 && 8 % heads == 0) {
-        const int64_t dies = 8 / heads, die = blockIdx.x % 8, n = (int64_t)(blockIdx.x / 8) * dies + die / heads;
-        if (n >= each) return -1;
-        w = die % heads * each + n;
-    } else {
-        w = work_of(heads * each);
-        if (w < 0) return -1;
+struct Part {
+    int32_t head, tile;   // head -1: none
+};
+__device__ inline Part tile_of(uint32_t heads, uint32_t each) {
+    if (heads < 8 && (heads & (heads - 1)) == 0) {
+        const uint32_t shift = 31 - __clz(heads), die = blockIdx.x % 8, n = ((blockIdx.x / 8) << (3 - shift)) + (die >> shift);
+        if (n >= each) return {-1, 0};
+        return {(int32_t)(die & (heads - 1)), (int32_t)(each - 1 - n)};
     }
-    return w / each * each + each - 1 - w % each;
+    const int32_t w = work_of(heads * each);
+    if (w < 0) return {-1, 0};
+    const uint32_t head = (uint32_t)w / each;
+    return {(int32_t)head, (int32_t)(each - 1 - ((uint32_t)w - head * each))};
 }
 
 // The union of the blocks that the queries [i0, i0 + nq) chose and can read:
@@ -354,15 +358,13 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan,
     uint32_t *words = masks + plan.most;
     float *table = reinterpret_cast<float *>(words + 2 * ((s.nblocks + 31) / 32));
 
-    int64_t w = tile_of((int64_t)s.batch * s.k_heads, (int64_t)plan.tiles * plan.splits);
-    if (w < 0) return;
-    const int split = (int)(w % plan.splits);
-    w /= plan.splits;
-    const int64_t tile_id = w;
-    const int64_t i0 = (w % plan.tiles) / plan.parts * plan.nq;
-    const int h0 = (int)(w % plan.tiles % plan.parts) * plan.span;   // of the key head's query heads
-    w /= plan.tiles;
-    const int g = (int)(w % s.k_heads), b = (int)(w / s.k_heads);
+    const Part part = tile_of(s.batch * s.k_heads, plan.tiles * plan.splits);
+    if (part.head < 0) return;
+    const uint32_t tile_no = (uint32_t)part.tile / (uint32_t)plan.splits, step = tile_no / (uint32_t)plan.parts;
+    const int split = part.tile - tile_no * plan.splits;
+    const int64_t tile_id = (int64_t)part.head * plan.tiles + tile_no, i0 = (int64_t)step * plan.nq;
+    const int h0 = (int)(tile_no - step * plan.parts) * plan.span;   // of the key head's query heads
+    const int b = (uint32_t)part.head / (uint32_t)s.k_heads, g = part.head - b * s.k_heads;
     const int ql = s.ql(b), kl = s.kl(b);
     if (s.clear && split == 0 && i0 + plan.nq > ql)
         clear_rows(s, b, g, h0, min(plan.span, s.group - h0), max(i0, (int64_t)ql), min(i0 + plan.nq, s.q_len), out, lse);
@@ -561,14 +563,13 @@ template <class T>
 __global__ __launch_bounds__(64) void k_attend_join(AttnShape s, RowPlan plan, int32_t dp, int32_t tile_rows, float unit,
                                                     SideOut out, float *__restrict__ lse) {
     __shared__ float weight[64];
-    int64_t w = blockIdx.x;
-    const int r = (int)(w % (plan.nq * plan.span));
-    w /= plan.nq * plan.span;
-    const int64_t tile_id = w, i = (w % plan.tiles) / plan.parts * plan.nq + r / plan.span;
-    const int hh = (int)(w % plan.tiles % plan.parts) * plan.span + r % plan.span;
-    w /= plan.tiles;
-    const int g = (int)(w % s.k_heads), b = (int)(w / s.k_heads), lane = threadIdx.x;
-    const int64_t first = tile_id * plan.splits * tile_rows + r;   // splits: at most 64
+    const uint32_t tile_id = blockIdx.x / (uint32_t)(plan.nq * plan.span), head = tile_id / (uint32_t)plan.tiles;
+    const uint32_t tile_no = tile_id - head * plan.tiles, at_query = tile_no / (uint32_t)plan.parts;
+    const int r = blockIdx.x - tile_id * (plan.nq * plan.span), rq = plan.per_span(r);
+    const int64_t i = (int64_t)at_query * plan.nq + rq;
+    const int hh = (int)(tile_no - at_query * plan.parts) * plan.span + r - rq * plan.span;
+    const int b = head / (uint32_t)s.k_heads, g = head - b * s.k_heads, lane = threadIdx.x;
+    const int64_t first = (int64_t)tile_id * plan.splits * tile_rows + r;   // splits: at most 64
     const bool on = lane < plan.splits;
     const float m = on ? plan.stat[(first + (int64_t)lane * tile_rows) * 2] : -INFINITY;
     const float x = on ? plan.stat[(first + (int64_t)lane * tile_rows) * 2 + 1] : 0.0f;

@@ -67,10 +67,8 @@ template <class T>
 __global__ __launch_bounds__(256) void k_block_summary(AttnShape s, Side k, int64_t fresh, int32_t per,
                                                        uint16_t *__restrict__ out) {
     __shared__ double part[16][128];
-    int64_t w = blockIdx.x;
-    const int c0 = (int)(w % per);
-    w /= per;
-    const int g = (int)(w % s.k_heads), b = (int)(w / s.k_heads);
+    const uint32_t head = blockIdx.x / (uint32_t)per;
+    const int c0 = (int)(blockIdx.x - head * per), b = head / (uint32_t)s.k_heads, g = head - b * s.k_heads;
     const int kl = s.kl(b);
     int c = c0;
     if (fresh > 0) {

@@ -331,11 +331,9 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 256) void k_block_select(AttnShape
     constexpr int KS = DP / 32;
     extern __shared__ uint32_t keys[];                       // [nq][stride], then the norms, then each wave's bits
     uint32_t *qnorm = keys + plan.nq * plan.stride, *mnorm = qnorm + plan.nq;
-    int64_t w = tile_of((int64_t)s.batch * s.k_heads, plan.tiles);
-    if (w < 0) return;
-    const int i0 = (int)(w % plan.tiles) * plan.nq;
-    w /= plan.tiles;
-    const int g = (int)(w % s.k_heads), b = (int)(w / s.k_heads);
+    const Part part = tile_of(s.batch * s.k_heads, plan.tiles);
+    if (part.head < 0) return;
+    const int i0 = part.tile * plan.nq, b = (uint32_t)part.head / (uint32_t)s.k_heads, g = part.head - b * s.k_heads;
     const int ql = s.ql(b), kl = s.kl(b);
     if (s.clear && i0 + plan.nq > ql) {   // queries behind the sequence's end
         const int64_t from = max(i0, ql), to = min((int64_t)i0 + plan.nq, s.q_len);
@@ -347,7 +345,7 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 256) void k_block_select(AttnShape
     const int lane = tid % 64, col = lane & 15, quad = lane >> 4;
     const int nq = min(plan.nq, ql - i0), rows = nq * s.group;
     const int p0 = i0 + kl - ql, pl = p0 + nq - 1;
-    auto blocks_seen = [&](int p) { return s.causal ? (p < 0 ? 0 : p / s.block + 1) : (kl + s.block - 1) / s.block; };
+    auto blocks_seen = [&](int p) { return s.causal ? (p < 0 ? 0 : (int)((uint32_t)p / (uint32_t)s.block) + 1) : (int)((uint32_t)(kl + s.block - 1) / (uint32_t)s.block); };
     const int all = blocks_seen(pl);
     const uint16_t *mean = summary + ((int64_t)b * s.k_heads + g) * s.nblocks * s.dim;
 

@@ -465,6 +465,23 @@ def test_bias_arguments_are_refused():
     assert g(0, 2, 4, 5, 6, 7, x, 120, 30, 6, x, None, x, n.value, 0, None) == INVALID
 
 
+def test_struct_layouts_match_header(tmp_path):
+    import ctypes as C
+    import os
+    import subprocess
+
+    import ias
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "ias.h"\n'
+                   'int main(void){printf("%zu %zu %zu %zu\\n", sizeof(ias_heads), sizeof(ias_attention), '
+                   'offsetof(ias_attention, scale), offsetof(ias_attention, clear));return 0;}\n')
+    exe = tmp_path / "layout"
+    subprocess.run(["gcc", "-I", os.path.join(root, "include"), str(src), "-o", str(exe)], check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True).stdout.split()]
+    assert got == [C.sizeof(ias.Heads), C.sizeof(ias.Attention), ias.Attention.scale.offset, ias.Attention.clear.offset]
+
+
 def test_tensors_of_the_host_are_refused():
     from ias import attention
     q = torch.zeros(1, 4, 2, 64, dtype=torch.bfloat16)

@@ -236,8 +236,10 @@ ias_status check_workspace(const void *p, int64_t have, int64_t need) {
 }
 
 // A launch with `lds` bytes of dynamic LDS; more than 64 KB are asked for once a device.
+// A launch holds fewer than 2^32 threads.
 template <auto kernel, class... P>
 ias_status launch(int device, int64_t grid, int threads, size_t lds, void *stream, P... args) {
+    if (grid > (int64_t)UINT32_MAX / threads) REFUSE(IAS_ERROR_OVERFLOW, "%lld workgroups of %d threads in a launch", (long long)grid, threads);
     static std::atomic<bool> asked[64];
     if (lds > 64 * 1024 && !(device < 64 && asked[device].load(std::memory_order_relaxed))) {
         HIPC(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
@@ -399,11 +401,10 @@ extern "C" ias_status ias_block_summary(const ias_attention *a, const ias_heads 
     HIPC(on.to(a->device));
     const dev::AttnShape s = shape_of(a);
     const int32_t per = fresh > 0 ? (int32_t)std::min<int64_t>(s.nblocks, (std::min(fresh, a->k_len) + a->block - 2) / a->block + 1) : s.nblocks;
-    const dim3 grid((unsigned)(a->batch * a->k_heads * per));
+    const int64_t grid = a->batch * a->k_heads * per;
     uint16_t *o = static_cast<uint16_t *>(summary);
-    if (a->dtype == IAS_DTYPE_BF16) dev::k_block_summary<dev::Bf16><<<grid, 256, 0, (hipStream_t)a->stream>>>(s, side(k), fresh, per, o);
-    else dev::k_block_summary<dev::Fp16><<<grid, 256, 0, (hipStream_t)a->stream>>>(s, side(k), fresh, per, o);
-    return launched();
+    return a->dtype == IAS_DTYPE_BF16 ? launch<dev::k_block_summary<dev::Bf16>>(a->device, grid, 256, 0, a->stream, s, side(k), fresh, per, o)
+                                      : launch<dev::k_block_summary<dev::Fp16>>(a->device, grid, 256, 0, a->stream, s, side(k), fresh, per, o);
 }
 
 extern "C" ias_status ias_block_select(const ias_attention *a, const ias_heads *q, const void *summary, int32_t first,

@@ -2,12 +2,12 @@
 //
 // A workgroup takes up to ROWS rows of one key head: its query heads for a few
 // consecutive queries (row r is query r / span, head r % span), or some of the heads
-// of one query where there are more of them than rows.  It walks the union of the blocks that these queries chose, each block once:
-// neighbouring queries choose mostly the same blocks, and where they do not the
-// walk reads no more than the queries would one by one.  A row that did not
-// choose a block masks it.  The four waves share nothing while they walk: wave w
-// takes every fourth piece of 32 keys and keeps its own running maximum, sum and
-// output (softmax in one pass), and the four meet once at the end.
+// of one query where there are more of them than rows.  It walks the union of the blocks
+// that these queries chose, each block once: neighbouring queries choose mostly the same
+// blocks, and where they do not the walk reads no more than the queries would one by one.
+// A row that did not choose a block masks it.  The W waves share nothing while they walk:
+// wave w takes every W-th piece of 32 keys and keeps its own running maximum, sum and
+// output (softmax in one pass), and they meet once at the end.
 //
 // Per piece: K and V go from memory through registers (the next piece's loads run
 // under this one's work) into the wave's own LDS tiles.  S^T = K Q^T with Q^T
@@ -18,6 +18,13 @@
 // fp32.  V^T's fragments need the keys of one channel side by side: transposed
 // LDS reads.  The tiles' 32-byte columns are permuted by row, so that the 8 rows
 // which half a wave reads lie in 8 different groups of banks.
+//
+// Prompts are bound by the latency of a piece's chain (load, LDS, scores, exponentials,
+// product) with the two waves a SIMD that 256 registers a lane allow: 8192 tokens, 32/8 heads of 128, 16 blocks of 64 keys a query, random choices:
+// 0.53 to 0.56 ms, where a union of 8 queries has 39 blocks; matrix units are busy 22 % of
+// it, vector ALUs 40 %, LDS 35 %, the vector cache 47 %.  Single tokens are bound by the
+// read of K and V (16 users, 32 of up to 512 blocks, 8 heads of 128: 134 MB in 29.7 us,
+// 4.5 TB/s) and few of them by the launch and one chain of loads (13.6 us for one user).
 #pragma once
 
 #include "attention_kernels.hpp"

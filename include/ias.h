@@ -423,15 +423,15 @@ ias_status ias_dist_csr_mul_csr(ias_dist *dist, const ias_csr *A, const ias_csr 
  * Shapes: q, out, dout, dq are batch x q_len x q_heads x head_dim, k, v, dk, dv
  * batch x k_len x k_heads x head_dim (ias_heads: strides of the first three in
  * elements, the last is contiguous; data 16-byte aligned and the strides
- * multiples of 8, of tokens at most 2^24).  Query head h reads key head h / (q_heads / k_heads).  A
- * sequence's queries are its last tokens: with q_lens / k_lens (int32 per batch
- * element, NULL: all q_len / k_len; values are clamped to [0, q_len] and
- * [0, k_len]) query i stands at position i + k_lens[b] - q_lens[b], and causal
- * lets it read the keys up to that position.  Output rows at or beyond a
- * sequence's length are not written, or with `clear` written as 0 (lse:
- * -infinity, blocks: -1).  What a padded or masked key, or one of a
- * block that a query did not choose, holds (infinities and NaN too) does not
- * reach that query's results.
+ * multiples of 8, of tokens at most 2^24).  Query head h reads key head
+ * h / (q_heads / k_heads).  A sequence's queries are its last tokens: with
+ * q_lens / k_lens (int32 per batch element, NULL: all q_len / k_len; values are
+ * clamped to [0, q_len] and [0, k_len]) query i stands at position
+ * i + k_lens[b] - q_lens[b], and causal lets it read the keys up to that
+ * position.  Output rows at or beyond a sequence's length are not written, or
+ * with `clear` written as 0 (lse: -infinity, blocks: -1).  What a padded or
+ * masked key, or one of a block that a query did not choose, holds (infinities
+ * and NaN too) does not reach that query's results.
  *
  * Pattern (`blocks`, int32, batch x k_heads x q_len x keep): the blocks of
  * `block` keys that a query reads, one choice for the query heads of a key
@@ -444,7 +444,9 @@ ias_status ias_dist_csr_mul_csr(ias_dist *dist, const ias_csr *A, const ias_csr 
  *
  * Limits, IAS_ERROR_UNSUPPORTED beyond: dtype bf16 or f16; head_dim a multiple
  * of 8 up to 128; block a multiple of 64 up to 1024; keep up to 256; at most
- * 64 query heads for a key head, 16384 blocks, 64 buckets. */
+ * 64 query heads for a key head, 16384 blocks, 64 buckets, 2^24 queries of a
+ * sequence.  IAS_ERROR_OVERFLOW: batch x heads x length beyond 2^31 rows, or a
+ * launch of 2^32 threads or more. */
 typedef enum ias_dtype { IAS_DTYPE_F32 = 0, IAS_DTYPE_BF16 = 1, IAS_DTYPE_F16 = 2 } ias_dtype;
 
 typedef struct ias_heads {
@@ -477,7 +479,7 @@ ias_status ias_block_summary(const ias_attention *a, const ias_heads *k, int64_t
 /* blocks: for each query the first `first` of the blocks that it may read, the
  * last `local` of them (causal only), then those of the highest score, up to
  * `keep`; ascending, -1 behind.  A block's score is the largest q_h . mean of
- * the key head's query heads, compared in 64 bits (NaN below everything); of
+ * the key head's query heads, compared in 64 bits (NaN as -infinity); of
  * equal scores the lower block wins.  first + local <= keep. */
 ias_status ias_block_select(const ias_attention *a, const ias_heads *q, const void *summary,
                             int32_t first, int32_t local, int32_t *blocks);
@@ -502,7 +504,7 @@ ias_status ias_block_attention_grad(const ias_attention *a, const ias_heads *dou
 /* The bias by itself, a matrix of constant diagonals for each head:
  * out[h][i][j] = table[bucket(j - i - (k_len - q_len))][h] (heads x q_len x
  * k_len, contiguous; table num_buckets x heads; types f32, bf16, f16; at most
- * 64 buckets), and its gradient dtable[n][h] = sum of grad[b][h][i][j] over b
+ * 64 buckets, 2^16 heads, q_len and k_len 2^24 and their product 2^34), and its gradient dtable[n][h] = sum of grad[b][h][i][j] over b
  * and the (i, j) of bucket n, summed in f32 in a fixed order (grad: strides of
  * the first three in elements, the last is contiguous).  workspace:
  * ias_rel_bias_grad_workspace bytes. */

@@ -456,8 +456,11 @@ def test_bias_arguments_are_refused():
     assert f(0, 4, 5, 6, 7, None, x, x, 0, None) == INVALID
     assert f(0, 4, 5, 6, 7, x, None, x, 0, None) == INVALID
     assert f(0, 4, 1 << 31, 6, 7, x, x, x, 0, None) == OVERFLOW
+    assert f(0, 4, 1 << 18, 1 << 18, 7, x, x, x, 0, None) == OVERFLOW
     assert f(0, 4, 0, 6, 7, None, None, None, 0, None) == 0
     n = C.c_int64(0)
+    assert ias.lib.ias_rel_bias_grad_workspace(1, 1 << 16, 1, 1 << 24, 7, C.byref(n)) == OVERFLOW
+    assert ias.lib.ias_rel_bias_grad_workspace(1, 1, 1 << 17, 1 << 17, 7, C.byref(n)) == 0
     assert ias.lib.ias_rel_bias_grad_workspace(2, 4, 5, 6, 7, C.byref(n)) == 0 and n.value > 0
     g = ias.lib.ias_rel_bias_grad
     assert g(0, 2, 4, 5, 6, 7, x, 120, 30, 6, x, x, x, n.value - 4, 0, None) == CAPACITY
@@ -577,3 +580,16 @@ def test_first_call_is_captured(A):
             g.replay()
             for a, b in zip(h, check(A, c, x)):
                 assert torch.equal(a, b)
+
+
+@gpu
+def test_launches_beyond_32_bits_are_refused(A):
+    """2^24 + 8 workgroups of 256 threads."""
+    b = (1 << 24) + 8
+    q = torch.zeros(b, 1, 1, 8, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(Exception, match="threads in a launch"):
+        A.block_select(q, torch.empty(b, 1, 0, 8, dtype=torch.bfloat16, device="cuda"), 1, k_len=0, first=0)
+    with pytest.raises(Exception, match="threads in a launch"):
+        A.block_summary(q)
+    one = torch.zeros(1, 1, 3, 1, device="cuda").transpose(2, 3).contiguous().transpose(2, 3)   # one column, of any stride
+    assert (A.rel_bias_grad(one, torch.zeros(0, dtype=torch.int32, device="cuda")) == 0).all()

@@ -129,9 +129,9 @@ ias_status launched() {
     return IAS_SUCCESS;
 }
 
-ias_status bucket_map(const ias_attention *a, dev::AttnShape &s, uint8_t *map) {
+ias_status bucket_map(const ias_attention *a, dev::AttnShape &s, uint8_t *map, int32_t *count = nullptr, int64_t entries = 0) {
     const int64_t n = map_size(a);
-    dev::k_bucket_map<<<dim3((unsigned)ceil_div(n, 256)), 256, 0, (hipStream_t)a->stream>>>(a->k_len, n, a->num_buckets, a->edges, map);
+    dev::k_bucket_map<<<dim3((unsigned)ceil_div(n, 256)), 256, 0, (hipStream_t)a->stream>>>(a->k_len, n, a->num_buckets, a->edges, map, count, entries);
     s.map = map;
     return launched();
 }
@@ -352,14 +352,14 @@ ias_status grad_all(const ias_attention *a, const ias_heads *dout, const ias_hea
     dev::AttnShape s = shape_of(a);
     dev::GradPlan p = w.q;
     if (!dtable) p.sums = nullptr;
-    if (a->table) IAS_TRY(bucket_map(a, s, w.map));
+    if (a->table) IAS_TRY(bucket_map(a, s, w.map, w.count, w.k.entries));   // clears the counts too
     const int64_t bh = a->batch * a->k_heads;
     if (bh > 0 && a->q_len > 0) {
         if (w.rows.rows == 16) IAS_TRY((grad_rows<T, DP, 16>(a, s, p, w.rows.waves, dout, q, k, v, out, lse, blocks, dq)));
         else IAS_TRY((grad_rows<T, DP, 32>(a, s, p, w.rows.waves, dout, q, k, v, out, lse, blocks, dq)));
     }
     if (w.k.entries > 0) {
-        IAS_TRY((launch<dev::k_clear>(a->device, ceil_div(w.k.entries, 256), 256, 0, a->stream, w.k.entries, w.count)));
+        if (!a->table) IAS_TRY((launch<dev::k_clear>(a->device, ceil_div(w.k.entries, 256), 256, 0, a->stream, w.k.entries, w.count)));
         if (a->q_len > 0)
             IAS_TRY((launch<dev::k_invert>(a->device, bh * w.k.nw, 256, 4 * (size_t)s.nblocks, a->stream, s, w.k.nw, blocks, w.bits, w.count)));
         IAS_TRY((launch<dev::k_items>(a->device, 1, 1024, 0, a->stream, w.k.entries, w.k.per, w.count, w.first, w.slot)));
@@ -371,9 +371,10 @@ ias_status grad_all(const ias_attention *a, const ias_heads *dout, const ias_hea
             else
                 IAS_TRY((launch<dev::k_grad_kv<T, DP, false>>(a->device, grid, 256, lds, a->stream, s, w.k, side(dout), side(q), side(k), side(v), lse, side_out(dk), side_out(dv))));
         }
-        IAS_TRY((launch<dev::k_grad_kv_join<T>>(a->device, w.k.entries * w.k.subs * 4, 256, 0, a->stream, s, w.k, DP, side_out(dk), side_out(dv))));
-    }
-    if (dtable)
+        const int64_t table = dtable ? (int64_t)a->q_heads * a->num_buckets : 0;
+        IAS_TRY((launch<dev::k_grad_kv_join<T>>(a->device, w.k.entries * w.k.subs * 4 + table, 256, 0, a->stream, s, w.k, DP, side_out(dk), side_out(dv), p,
+                       static_cast<uint16_t *>(dtable))));
+    } else if (dtable)
         IAS_TRY((launch<dev::k_grad_table<T>>(a->device, (int64_t)a->q_heads * a->num_buckets, 256, 0, a->stream, s, p, static_cast<uint16_t *>(dtable))));
     return IAS_SUCCESS;
 }

@@ -143,8 +143,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
             tile.fill(vr, VT);
             float x[N], y[N];
             __builtin_amdgcn_s_setprio(1);
-            scores<T, DP, ROWS>(tile, KT, qf, x);
-            scores<T, DP, ROWS>(tile, VT, df, y);
+            scores<T, DP, ROWS, false>(tile, KT, qf, x);
+            scores<T, DP, ROWS, false>(tile, VT, df, y);
             __builtin_amdgcn_s_setprio(0);
             const int jn = __builtin_amdgcn_readfirstlane(id) * s.block + at.part * 32;
             const uint32_t maskn = __builtin_amdgcn_readfirstlane(chose) & only;
@@ -255,12 +255,12 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
     }
 }
 
-// dtable[n][h]: the tiles' sums, one workgroup for each (bucket, head).  4.6 us for 2 x 2048
-// tokens of 16 heads, 32 buckets: the launch.
-template <class T>
-__global__ __launch_bounds__(256) void k_grad_table(AttnShape s, GradPlan plan, uint16_t *__restrict__ dtable) {
+// dtable[n][h]: the tiles' sums, one workgroup for each (bucket, head), at the end of
+// k_grad_kv_join's where that is launched (2 x 2048 tokens of 16 heads, 32 buckets: a
+// launch of its own is 4.6 us).
+template <class T> __device__ void sum_table(const AttnShape &s, const GradPlan &plan, uint32_t w, uint16_t *__restrict__ dtable) {
     __shared__ float part[256];
-    const int h = blockIdx.x % s.q_heads, n = blockIdx.x / s.q_heads, g = h / s.group, hh = h % s.group;
+    const int h = w % (uint32_t)s.q_heads, n = w / (uint32_t)s.q_heads, g = h / s.group, hh = h % s.group;
     const int32_t each = plan.tiles / plan.parts;   // tiles with this head, of a batch element and key head
     float t = 0.0f;
     for (int64_t r = threadIdx.x; r < (int64_t)s.batch * each; r += 256) {
@@ -274,6 +274,10 @@ __global__ __launch_bounds__(256) void k_grad_table(AttnShape s, GradPlan plan, 
         __syncthreads();
     }
     if (threadIdx.x == 0) dtable[(int64_t)n * s.q_heads + h] = T::down(part[0]);
+}
+template <class T>
+__global__ __launch_bounds__(256) void k_grad_table(AttnShape s, GradPlan plan, uint16_t *__restrict__ dtable) {
+    sum_table<T>(s, plan, blockIdx.x, dtable);
 }
 
 // ------------------------------------------------------------------ the pattern's transpose
@@ -594,9 +598,16 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
 
 // dk and dv of the blocks that no query or more than one item read, and of the keys
 // behind a sequence's end: a thread for 8 channels of a key, 16 keys a workgroup, the
-// results of four items in flight.  Bound by reading those (8192 tokens: 52 us).
+// results of four items in flight.  Bound by reading those (8192 tokens: 52 us).  The
+// workgroups behind them sum the bias's gradient.
 template <class T>
-__global__ __launch_bounds__(256) void k_grad_kv_join(AttnShape s, KeyPlan plan, int32_t dp, SideOut dk, SideOut dv) {
+__global__ __launch_bounds__(256) void k_grad_kv_join(AttnShape s, KeyPlan plan, int32_t dp, SideOut dk, SideOut dv, GradPlan sums,
+                                                      uint16_t *__restrict__ dtable) {
+    const uint32_t joins = (uint32_t)plan.entries * plan.subs * 4;
+    if (blockIdx.x >= joins) {
+        sum_table<T>(s, sums, blockIdx.x - joins, dtable);
+        return;
+    }
     const uint32_t e = blockIdx.x / 4 / (uint32_t)plan.subs, head = e / (uint32_t)s.nblocks;
     const int sub = (int)(blockIdx.x / 4 - e * plan.subs);
     const int64_t entry = e;

@@ -133,14 +133,22 @@ template <int DP, int ROWS = 16> struct Tile {
 };
 
 // x[e] for the N keys of a lane: a tile's 32 keys against the rows whose operands are q.
-template <class T, int DP, int ROWS>
+// AHEAD: all reads before the first product, where there are registers for that; the
+// compiler alone keeps one or two under way (k_attend 537 -> 529 us for 8192 tokens; in
+// k_grad_q other operands would be spilled, 306 -> 420).
+template <class T, int DP, int ROWS, bool AHEAD>
 __device__ inline void scores(const Tile<DP, ROWS> &tile, int at, const s16x8 *q, float *x) {
     typedef Form<ROWS> F;
+    constexpr int KS = DP / F::K;
+    s16x8 f[32 / ROWS * KS];
+#pragma unroll
+    for (int n = 0; n < 32 / ROWS * KS; ++n) f[n] = tile.natural(at, ROWS * (n / KS), n % KS);
+    if (AHEAD) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int sub = 0; sub < 32 / ROWS; ++sub) {
         typename F::Acc acc{};
 #pragma unroll
-        for (int ks = 0; ks < DP / F::K; ++ks) acc = Mma<T>::run(tile.natural(at, ROWS * sub, ks), q[ks], acc);
+        for (int ks = 0; ks < KS; ++ks) acc = Mma<T>::run(f[sub * KS + ks], q[ks], acc);
 #pragma unroll
         for (int e = 0; e < F::N * ROWS / 32; ++e) x[sub * (F::N * ROWS / 32) + e] = acc[e];
     }
@@ -310,10 +318,12 @@ template <int DP> struct Piece {
                 f[n] = *reinterpret_cast<const s16x8 *>(reinterpret_cast<const char *>(row) + off);
             return;
         }
-        const int d = lane % CH * 8;
+        int here = lane;
+        asm volatile("" : "+v"(here));   // else every row's offset stays in a register all the way
+        const int d = here % CH * 8;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int j = j0 + n * (64 / CH) + lane / CH;
+            const int j = j0 + n * (64 / CH) + here / CH;
             const s16x8 x = load8(base + min(j, last) * token + (d < dim ? d : 0));
             f[n] = j < end && d < dim ? x : s16x8{};
         }
@@ -438,7 +448,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan,
             tile.fill(kr, KT);
             float y[N];
             __builtin_amdgcn_s_setprio(1);   // the SIMD's other wave has its turn between the products
-            scores<T, DP, ROWS>(tile, KT, qf, y);
+            scores<T, DP, ROWS, true>(tile, KT, qf, y);
             __builtin_amdgcn_s_setprio(0);
             tile.fill(vr, VT);
             const int jn = __builtin_amdgcn_readfirstlane(id) * s.block + at.part * 32;

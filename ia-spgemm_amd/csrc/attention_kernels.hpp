@@ -124,10 +124,13 @@ __device__ inline uint32_t four_buckets(int d, const int32_t *edges, int num_buc
     return got;
 }
 
-// map[d + k_len - 1] = how many edges are <= d, for every distance of a call.
+// map[d + k_len - 1] = how many edges are <= d, for every distance of a call; clears
+// `count` for a backward pass, which saves it a launch.  4.5 us: the launch.
 __global__ __launch_bounds__(256) void k_bucket_map(int64_t k_len, int64_t n, int32_t num_buckets,
-                                                    const int32_t *__restrict__ edges, uint8_t *__restrict__ map) {
+                                                    const int32_t *__restrict__ edges, uint8_t *__restrict__ map,
+                                                    int32_t *__restrict__ count, int64_t entries) {
     const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    for (int64_t c = e; c < entries; c += (int64_t)gridDim.x * 256) count[c] = 0;
     if (e >= n) return;
     map[e] = (uint8_t)bucket_of(e - (k_len - 1), edges, num_buckets);
 }

@@ -13,9 +13,9 @@
 // (bound: 0.005) where the formula in separate fp32 operators has 0.0017.  dS in two parts brought
 // it to 0.0024, since delta's part stays, and cost 8 to 13 % of a training step.
 //
-// 8192 tokens, 16/2 heads of 128, 16 blocks a query, all 0.88 ms with the forward: k_grad_q
-// 306 us and k_grad_kv 320 us, both bound by latency at two and three waves a SIMD as the
-// forward is (it makes 5 products where the forward makes 2), k_grad_kv_join 52 us, bound
+// 8192 tokens, 16/2 heads of 128, 16 blocks a query, all 0.86 ms with the forward: k_grad_q
+// 307 us and k_grad_kv 322 us, both bound by latency at two and three waves a SIMD as the
+// forward is (it makes 5 products where the forward makes 2), k_grad_kv_join 50 us, bound
 // by its read of partial results (64 KB an item); the pattern's transpose 17 us in three
 // launches.
 #pragma once
@@ -598,7 +598,7 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
 
 // dk and dv of the blocks that no query or more than one item read, and of the keys
 // behind a sequence's end: a thread for 8 channels of a key, 16 keys a workgroup, the
-// results of four items in flight.  Bound by reading those (8192 tokens: 52 us).  The
+// results of four items in flight.  Bound by reading those (8192 tokens: 50 us).  The
 // workgroups behind them sum the bias's gradient.
 template <class T>
 __global__ __launch_bounds__(256) void k_grad_kv_join(AttnShape s, KeyPlan plan, int32_t dp, SideOut dk, SideOut dv, GradPlan sums,

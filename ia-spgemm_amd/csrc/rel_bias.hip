@@ -203,13 +203,14 @@ ias_status check_bias(int32_t dtype, int64_t batch, int32_t heads, int64_t q_len
 
 // How the gradient is shared out: spans of 512 diagonals, and so many rows that
 // about 4096 workgroups are there (half of them hold corners outside the matrix), 16
-// at least (each ends in sums of its own).
+// at least (each ends in sums of its own) and all that there are at most (2^24: the
+// kernel takes 32 bits; a tall matrix of many heads would ask for 2^31 and more).
 struct Chunks {
     int64_t spans = 0, rows = 1, all = 0;
     Chunks(int64_t batch, int32_t heads, int64_t q_len, int64_t k_len) {
         if (batch == 0 || heads == 0 || q_len == 0 || k_len == 0) return;
         spans = ceil_div(q_len + k_len - 1, SPAN);
-        rows = std::max<int64_t>(16, ceil_div(q_len * spans * heads, 4096));
+        rows = std::min<int64_t>(q_len, std::max<int64_t>(16, ceil_div(q_len * spans * heads, 4096)));
         all = spans * ceil_div(q_len, rows);
     }
 };

@@ -1,0 +1,29 @@
+"""Block-sparse attention and the relative bias at the ends of their types' and sizes' ranges."""
+import math
+
+import pytest
+import torch
+
+import attention_ref as ref
+from test_attention import A, DT, case, check, kw, make, near  # noqa: F401
+
+gpu = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ dense bias
+@gpu
+@pytest.mark.parametrize("dtype,n,nk,h", [
+    ("bf16", 1 << 24, 1, 16), ("fp32", 1 << 24, 3, 16), ("fp16", 12_000_000, 1, 32), ("bf16", 1 << 23, 1, 64)])
+def test_gradient_of_a_tall_bias(A, dtype, n, nk, h):
+    """q_len x spans x heads beyond 2^43.  A constant gradient, of stride 0: sums are counts, exact in fp32 up to 2^24."""
+    grad = torch.full((1, 1, 1, nk), 2.0 ** -10, device="cuda").to(DT[dtype]).expand(1, h, n, nk)
+    edges = torch.tensor([-(n // 2), -1000, 0], dtype=torch.int32, device="cuda")
+    got = A.rel_bias_grad(grad, edges).double()
+    want = torch.zeros(4, dtype=torch.float64, device="cuda")
+    for j in range(nk):    # distances j - i - (nk - n), i < n: the n values that end at j - (nk - n)
+        lo, hi = j - nk + 1, j - nk + n
+        cut = [lo] + [min(max(e, lo), hi + 1) for e in (-(n // 2), -1000, 0)] + [hi + 1]
+        for t in range(4):
+            want[t] += (cut[t + 1] - cut[t]) * 2.0 ** -10
+    bound = (2.0 ** -12 + torch.finfo(DT[dtype]).eps / 2) * want
+    assert ((got - want[:, None]).abs() <= bound[:, None]).all()

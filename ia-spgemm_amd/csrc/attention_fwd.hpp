@@ -625,7 +625,7 @@ __global__ __launch_bounds__(64) void k_attend_join(AttnShape s, RowPlan plan, i
         *reinterpret_cast<uint32_t *>(to) = (uint32_t)T::down(y[0] * inv) | (uint32_t)T::down(y[1] * inv) << 16;
     }
     if (lse && lane == 0)
-        lse[((int64_t)b * s.q_heads + h) * s.q_len + i] = l == 0.0f ? -INFINITY : (all * unit + __builtin_amdgcn_logf(l)) * LN2;
+        lse[((int64_t)b * s.q_heads + h) * s.q_len + i] = l == 0.0f ? -INFINITY : (unit == 1.0f ? all * LN2 : all) + __builtin_amdgcn_logf(l) * LN2;
 }
 
 }  // namespace dev

@@ -27,3 +27,19 @@ def test_gradient_of_a_tall_bias(A, dtype, n, nk, h):
             want[t] += (cut[t + 1] - cut[t]) * 2.0 ** -10
     bound = (2.0 ** -12 + torch.finfo(DT[dtype]).eps / 2) * want
     assert ((got - want[:, None]).abs() <= bound[:, None]).all()
+
+
+# ------------------------------------------------------------------ biases of the type's lowest value
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("sq,sk,hq,hkv,d", [(300, 300, 4, 4, 128), (1, 6000, 4, 2, 64), (40, 2000, 2, 1, 64)])
+def test_log_sums_of_the_lowest_bias(A, dtype, sq, sk, hq, hkv, d):
+    """Walks shared by workgroups: the log of the sum is the lowest value too, not -infinity."""
+    c = case(dtype, sq=sq, sk=sk, hq=hq, hkv=hkv, d=d, keep=-(-sk // 64), nb=3, all=True)
+    s = make(c, 35)
+    s["q"] *= 0        # beside 65504 fp32 does not hold a score to fp16's half step
+    s["table"][:] = torch.finfo(DT[dtype]).min
+    want, bound = ref.attention(s["q"], s["k"], s["v"], s["blocks"], 64, True, d ** -0.5, None, None, s["table"], s["edges"])
+    out, lse = A.block_attention(s["q"], s["k"], s["v"], s["blocks"], **kw(c, s))
+    near(out, want["out"], bound["out"], "out")
+    near(lse, want["lse"], bound["lse"], "lse")

@@ -208,6 +208,8 @@ struct Backward {
         q.tiles = rows.plan.tiles; q.most = rows.plan.most;
         map = a->table ? w.part<uint8_t>(map_size(a)) : nullptr;
         q.delta = w.part<float>(a->batch * a->q_heads * a->q_len);
+        q.shift = a->table ? w.part<float>(a->batch * a->q_heads * a->q_len) : nullptr;
+        q.corr = a->table ? w.part<float>(a->batch * a->q_heads * a->q_len) : nullptr;
         q.sums = a->table ? w.part<float>(bh * q.tiles * q.span * a->num_buckets) : nullptr;
         k.nw = (int32_t)ceil_div(a->q_len, 32);
         k.subs = a->block / 64;
@@ -222,7 +224,7 @@ struct Backward {
         k.count = count = w.part<int32_t>(k.entries);
         k.first = first = w.part<int32_t>(k.entries + 1);
         k.slot = slot = w.part<int32_t>(k.entries + 1);
-        k.delta = q.delta;
+        k.delta = q.delta; k.shift = q.shift; k.corr = q.corr;
         k.part = w.part<float>(2 * chosen / k.per * result / 4);
     }
 };
@@ -363,7 +365,7 @@ ias_status grad_all(const ias_attention *a, const ias_heads *dout, const ias_hea
         if (a->q_len > 0)
             IAS_TRY((launch<dev::k_invert>(a->device, bh * w.k.nw, 256, 4 * (size_t)s.nblocks, a->stream, s, w.k.nw, blocks, w.bits, w.count)));
         IAS_TRY((launch<dev::k_items>(a->device, 1, 1024, 0, a->stream, w.k.entries, w.k.per, w.count, w.first, w.slot)));
-        const size_t lds = 4 * 32 * (size_t)DP * 2 + 2 * 5 * 32 * 4 + 4 * (size_t)w.k.per + 32 + 4 * (size_t)s.group * s.num_buckets;
+        const size_t lds = 4 * 32 * (size_t)DP * 2 + 2 * dev::FIGURES * 32 * 4 + 4 * (size_t)w.k.per + 32 + 4 * (size_t)s.group * s.num_buckets;
         const int64_t grid = ceil_div(w.items * w.k.subs, 8) * 8;
         if (a->q_len > 0) {
             if (a->table)

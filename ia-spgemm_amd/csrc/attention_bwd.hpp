@@ -31,6 +31,7 @@ struct GradPlan {
     uint32_t inverse;
     float *delta;                           // [batch][q_heads][q_len]
     float *sums;                            // [tile][span][num_buckets], null: no dtable
+    float *shift, *corr;                    // as delta, with a bias only: P = exp2((x - shift) log2(e) - corr)
     __device__ int per_span(int r) const { return (int)((uint32_t)r * inverse >> 16); }
 };
 
@@ -42,6 +43,42 @@ inline int grad_q_area(int dp, int rows, int waves, int buckets, bool sums) {
 }
 inline size_t grad_q_lds(int area, int nblocks, int most, int span, int buckets) {
     return area + 8 * (size_t)((nblocks + 31) / 32) + 8 * (size_t)most + 16 + 4 * (size_t)span * buckets;
+}
+
+// The largest score of a row over its part of the union and log2 of the sum of
+// exponentials beside it, by one wave.
+struct RowSum {
+    float top, log;
+};
+template <class T>
+__device__ RowSum row_sums(const AttnShape &s, const uint16_t *__restrict__ q, const Side &k, int b, int g, int end, int pos, int found,
+                           const int32_t *ids, const uint32_t *masks, int query, const float *table, int span, int lane) {
+    float top = -INFINITY, sum = 0.0f;
+    for (int n = 0; n < found; ++n) {
+        if (!(masks[n] >> query & 1u)) continue;
+        const int j0 = ids[n] * s.block;
+        for (int j = j0 + lane; j < min(end, j0 + s.block); j += 64) {
+            const uint16_t *row = k.at(b, j, g);
+            float x = 0.0f;
+            for (int d = 0; d < s.dim; d += 8) {
+                const s16x8 u = load8(q + d), v = load8(row + d);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x = __builtin_fmaf(T::up((uint16_t)u[e]), T::up((uint16_t)v[e]), x);
+            }
+            x = __builtin_fmaf(x, s.scale, table[s.map[(int64_t)j - pos + s.k_len - 1] * span]);
+            if (!(x > -INFINITY)) continue;
+            if (x > top) {
+                sum *= __builtin_amdgcn_exp2f((top - x) * LOG2E);
+                top = x;
+            }
+            sum += __builtin_amdgcn_exp2f((x - top) * LOG2E);
+        }
+    }
+    float all = top;
+    for (int d = 32; d; d >>= 1) all = fmaxf(all, __shfl_xor(all, d));
+    sum = top == -INFINITY ? 0.0f : sum * __builtin_amdgcn_exp2f((top - all) * LOG2E);
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    return {all, __builtin_amdgcn_logf(sum)};
 }
 
 template <class T, int DP, int ROWS, int W, bool BIAS>
@@ -87,8 +124,30 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
     const int found = __builtin_amdgcn_readfirstlane(block_union(s, blocks, b, g, i0, nq, ql, kl, words, ids, masks, scratch));
 
     const Row<DP, ROWS> row(lane, rows, plan.per_span(lane % ROWS), h0, plan.span, (int)i0, kl, ql, s.causal);
+    float delta = 0.0f, shift, corr = 0.0f;
+    // a row that read nothing has lse = -inf: exp(x - inf) = 0
+    if (BIAS) {
+        const int64_t at = ((int64_t)b * s.q_heads + (int64_t)g * s.group + row.head) * s.q_len + i0 + row.query;
+        const float l = row.there ? lse[at] : -INFINITY;
+        shift = l == -INFINITY ? INFINITY : l == INFINITY ? NAN : l;   // infinite: a score was
+        // Beside a bias of the type's lowest value fp32 holds no log of a sum: at 4096 lse is off
+        // by up to 2^-13, far beyond it a row of equals would get P = 1 for each.  Such rows (hardly
+        // ever any) find their maximum and sum again.
+        for (unsigned long long wild = __ballot(lane < ROWS && fabsf(l) >= 4096.0f && fabsf(l) < INFINITY); wild; wild &= wild - 1) {
+            const int r = __ffsll(wild) - 1, rq = plan.per_span(r), hr = r - rq * plan.span, pos = (int)i0 + rq + kl - ql;
+            const RowSum got = row_sums<T>(s, q.at(b, i0 + rq, (int64_t)g * s.group + h0 + hr), k, b, g, s.causal ? min(kl, pos + 1) : kl, pos,
+                                           found, ids, masks, rq, table + hr, plan.span, lane);
+            if (lane % ROWS == r && got.top > -INFINITY) {
+                shift = got.top;
+                corr = got.log;
+            }
+        }
+        if (wave == 0 && row.part == 0 && row.there) {
+            plan.shift[at] = shift;
+            plan.corr[at] = corr;
+        }
+    }
     s16x8 qf[DP / F::K], df[DP / F::K];
-    float delta = 0.0f, shift;
     {
         const int64_t h = (int64_t)g * s.group + row.head, at = ((int64_t)b * s.q_heads + h) * s.q_len + i0 + row.query;
         row.load(df, dout.at(b, i0 + row.query, h), s.dim);
@@ -102,9 +161,10 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
         if (s.scale < 0.0f)
 #pragma unroll
             for (int ks = 0; ks < DP / F::K; ++ks) qf[ks] = negated(qf[ks]);
-        const float l = row.there ? lse[at] : -INFINITY;
-        // a row that read nothing has lse = -inf: exp(x - inf) = 0
-        shift = l == -INFINITY ? INFINITY : BIAS ? l : l * LOG2E;
+        if (!BIAS) {
+            const float l = row.there ? lse[at] : -INFINITY;
+            shift = l == -INFINITY ? INFINITY : l * LOG2E;
+        }
         if (wave == 0 && row.part == 0 && row.there) plan.delta[at] = delta;
     }
     const float c = fabsf(BIAS ? s.scale : s.scale * LOG2E);
@@ -162,7 +222,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
                 for (int e = n; e < n + 4; ++e) {
                     float p;
                     if (BIAS)
-                        p = __builtin_amdgcn_exp2f((__builtin_fmaf(x[e], c, table[(bucket[n / 4] >> (8 * (e - n)) & 255) * plan.span + row.head - h0]) - off) * LOG2E);
+                        p = __builtin_amdgcn_exp2f(__builtin_fmaf(__builtin_fmaf(x[e], c, table[(bucket[n / 4] >> (8 * (e - n)) & 255) * plan.span + row.head - h0]) - off, LOG2E, -corr));
                     else
                         p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], c, -off));
                     y[e] = p * (y[e] - delta);
@@ -357,9 +417,11 @@ struct KeyPlan {
     int64_t entries;            // batch x k_heads x nblocks
     const uint32_t *bits;
     const int32_t *count, *first, *slot;
-    const float *delta;
+    const float *delta, *shift, *corr;
     float *part;                // [slot][sub][dk, dv][64][DP]: items of blocks with more than one
 };
+
+constexpr int FIGURES = 6;   // of each row in k_grad_kv's LDS
 
 // One workgroup for an item and 64 of its block's keys; wave w has 16 of them,
 // with K and V resident as the right operands of S = Q K^T and dP = dO V^T.
@@ -374,8 +436,8 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
                                                     const float *__restrict__ lse, SideOut dk, SideOut dv) {
     constexpr int KS = DP / 32, DT = DP / 16, CH = DP / 8, TILE = 32 * DP * 2, LD = 32 * CH / 256;
     extern __shared__ __attribute__((aligned(16))) char lds[];   // [2][Q, dO] tiles
-    float *fig = reinterpret_cast<float *>(lds + 4 * TILE);       // [2][32] of (shift, delta, end, position, head)
-    int32_t *list = reinterpret_cast<int32_t *>(fig + 2 * 5 * 32);
+    float *fig = reinterpret_cast<float *>(lds + 4 * TILE);       // [2][32] of (shift, delta, end, position, head, corr)
+    int32_t *list = reinterpret_cast<int32_t *>(fig + 2 * FIGURES * 32);
     int32_t *scratch = list + plan.per;                           // flag, prefix of the list's words
     float *table = reinterpret_cast<float *>(scratch + 8);
 
@@ -437,7 +499,7 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
 #pragma unroll
     for (int t = 0; t < DT; ++t) ak[t] = av[t] = f32x4{};
     s16x8 qn[LD], dn[LD];
-    float fn[5];
+    float fn[FIGURES];
     auto fetch = [&](int r0) {
 #pragma unroll
         for (int n = 0; n < LD; ++n) {
@@ -454,8 +516,13 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
             const bool on = r < rows;
             const int rr = min(r, rows - 1), rq = (uint32_t)rr / (uint32_t)s.group, i = list[rq], p = i + kl - ql;
             const int64_t at = ((int64_t)b * s.q_heads + (int64_t)g * s.group + rr - rq * s.group) * s.q_len + i;
-            const float l = on ? lse[at] : -INFINITY;
-            fn[0] = l == -INFINITY ? INFINITY : BIAS ? l : l * LOG2E;
+            if (BIAS) {
+                fn[0] = on ? plan.shift[at] : INFINITY;
+                fn[5] = plan.corr[at];
+            } else {
+                const float l = on ? lse[at] : -INFINITY;
+                fn[0] = l == -INFINITY ? INFINITY : l * LOG2E;
+            }
             fn[1] = plan.delta[at];
             fn[2] = __int_as_float(!on ? 0 : s.causal ? min(kl, p + 1) : kl);
             fn[3] = __int_as_float(p);
@@ -472,7 +539,7 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
         }
         if (tid < 32)
 #pragma unroll
-            for (int f = 0; f < 5; ++f) fig[(buf * 5 + f) * 32 + tid] = fn[f];
+            for (int f = 0; f < (BIAS ? 6 : 3); ++f) fig[(buf * FIGURES + f) * 32 + tid] = fn[f];
     };
     fetch(0);
     int buf = 0;
@@ -481,7 +548,7 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
         __syncthreads();
         if (r0 + 32 < rows) fetch(r0 + 32);
         const int qt = buf * 2 * TILE, dt = qt + TILE;
-        const float *f = fig + buf * 5 * 32;
+        const float *f = fig + buf * FIGURES * 32;
         float p[8], ds[8];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
@@ -500,7 +567,7 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
                 float y;
                 if (BIAS) {
                     const int pos = __float_as_int(f[96 + at + e]), hr = __float_as_int(f[128 + at + e]);
-                    y = __builtin_amdgcn_exp2f((__builtin_fmaf(x[e], cs, table[s.map[(int64_t)key - pos + s.k_len - 1] * s.group + hr]) - shift[e]) * LOG2E);
+                    y = __builtin_amdgcn_exp2f(__builtin_fmaf(__builtin_fmaf(x[e], cs, table[s.map[(int64_t)key - pos + s.k_len - 1] * s.group + hr]) - shift[e], LOG2E, -f[160 + at + e]));
                 } else {
                     y = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], cs, -shift[e]));
                 }
@@ -558,8 +625,8 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
         for (int r = 0; r < rows; ++r) {
             const int i = list[r / s.group], pos = i + kl - ql, hr = r % s.group;
             const int64_t h = (int64_t)g * s.group + hr, at = ((int64_t)b * s.q_heads + h) * s.q_len + i;
-            const float l = lse[at];
-            if ((s.causal && j > pos) || l == -INFINITY) continue;
+            const float shift = BIAS ? plan.shift[at] : lse[at] == -INFINITY ? INFINITY : lse[at], corr = BIAS ? plan.corr[at] : 0.0f;
+            if ((s.causal && j > pos) || shift == INFINITY) continue;
             const uint16_t *qr = q.at(b, i, h), *dr = dout.at(b, i, h);
             float x = 0.0f, dp = 0.0f;
 #pragma unroll
@@ -574,7 +641,7 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
             }
             x *= s.scale;
             if (BIAS) x += table[s.map[(int64_t)j - pos + s.k_len - 1] * s.group + hr];
-            const float p = __builtin_amdgcn_exp2f((x - l) * LOG2E), ds = p * (dp - plan.delta[at]);
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x - shift, LOG2E, -corr)), ds = p * (dp - plan.delta[at]);
 #pragma unroll
             for (int d = 0; d < C; ++d)
                 if (d0 + d < s.dim) {

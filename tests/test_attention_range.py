@@ -43,3 +43,22 @@ def test_log_sums_of_the_lowest_bias(A, dtype, sq, sk, hq, hkv, d):
     out, lse = A.block_attention(s["q"], s["k"], s["v"], s["blocks"], **kw(c, s))
     near(out, want["out"], bound["out"], "out")
     near(lse, want["lse"], bound["lse"], "lse")
+
+@gpu
+@pytest.mark.parametrize("sq,hq,hkv,d", [(80, 2, 1, 64), (300, 4, 4, 128), (3, 4, 2, 64)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_gradients_of_rows_of_the_lowest_bias(A, dtype, sq, hq, hkv, d):
+    """Rows that see nothing but a bucket at the type's lowest value are rows of equals, beside ordinary ones."""
+    c = case(dtype, b=2, sq=sq, sk=sq + 7, hq=hq, hkv=hkv, d=d, keep=6, nb=3, all=True, q_lens=[sq, sq - 1], k_lens=[sq, sq + 3])
+    s = make(c, 34)
+    s["edges"] = torch.tensor([-30, -20], dtype=torch.int32, device="cuda")
+    if dtype == "fp16":
+        s["q"] = torch.where(s["q"].isnan(), s["q"], 0.0).half()    # scores of 65504 differ by what fp32 holds there
+    for low in (torch.finfo(DT[dtype]).min, -3e4):
+        if low == -3e4:
+            s["q"] = torch.where(s["q"].isnan(), s["q"], 0.0).to(DT[dtype])
+        s["table"][2] = low         # the keys at distances of -20 and more: all that the first rows see
+        check(A, c, s)
+        check(A, c, s, scale=-0.3)
+        s["table"][:] = low
+        check(A, c, s)

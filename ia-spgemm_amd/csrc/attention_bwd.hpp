@@ -45,6 +45,26 @@ inline size_t grad_q_lds(int area, int nblocks, int most, int span, int buckets)
     return area + 8 * (size_t)((nblocks + 31) / 32) + 8 * (size_t)most + 16 + 4 * (size_t)span * buckets;
 }
 
+// fp16 holds 65504 at most and 11 bits only down to 2^-14, and dS goes by the size of dout
+// and v: 160000 from values and gradients of 200, 2^-24 from a small loss over many keys.
+// So before it is rounded a row (a key, in k_grad_kv) multiplies it by a power of two, which
+// its sum loses again at the end.  It starts with 2^80 (dS is below 2^40: 128 products of two
+// fp16) and is lowered, with what was summed by then, only where a dS would pass 2^15, so
+// that the largest comes to [2^11, 2^12): that is the first piece and hardly ever another.  Of
+// the largest that the row has met, everything down to 2^-25 keeps its 11 bits.  bf16 has the
+// range of fp32 and needs none of this.
+constexpr int FACTOR_START = 80;   // exponents of the factors
+constexpr float FACTOR_TOP = 0x1p15f;
+__device__ inline float times(float x, int exponent) { return __builtin_amdgcn_ldexpf(x, exponent); }
+__device__ inline int factor_for(float big) { return 11 + 127 - (int)(__float_as_uint(big) >> 23); }   // infinite: -117
+template <class T> __device__ inline float unscaled(float x, int exponent) { return T::NARROW ? times(x, -exponent) : x; }
+template <int N> __device__ inline float largest(const float *y) {
+    float big = 0.0f;   // NaN is passed over: it stays NaN whatever the factor
+#pragma unroll
+    for (int e = 0; e < N; ++e) big = fmaxf(big, fabsf(y[e]));
+    return big;
+}
+
 // The largest score of a row over its part of the union and log2 of the sum of
 // exponentials beside it, by one wave.
 struct RowSum {
@@ -179,6 +199,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
         typename F::Acc o[DP / ROWS];
 #pragma unroll
         for (int t = 0; t < DP / ROWS; ++t) o[t] = typename F::Acc{};
+        int factor = FACTOR_START;   // of the row's dS and o
         s16x8 kr[VL], vr[VL];
         Walk<W> at(wave, per_block);
         auto skip = [&]() {
@@ -213,7 +234,9 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
                 vp.load(vr, jn, vend);
             }
             const bool sel = mask >> row.query & 1u;
-            const float off = sel ? shift : INFINITY;   // exp(x - inf) = 0
+            // exp(x - inf) = 0; a row's factor lies in its exponentials
+            const float off = !sel ? INFINITY : T::NARROW && !BIAS ? shift - (float)factor : shift;
+            const float less = T::NARROW ? corr - (float)factor : corr;
             uint32_t bucket[N / 4];
 #pragma unroll
             for (int n = 0; n < N; n += 4) {
@@ -222,7 +245,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
                 for (int e = n; e < n + 4; ++e) {
                     float p;
                     if (BIAS)
-                        p = __builtin_amdgcn_exp2f(__builtin_fmaf(__builtin_fmaf(x[e], c, table[(bucket[n / 4] >> (8 * (e - n)) & 255) * plan.span + row.head - h0]) - off, LOG2E, -corr));
+                        p = __builtin_amdgcn_exp2f(__builtin_fmaf(__builtin_fmaf(x[e], c, table[(bucket[n / 4] >> (8 * (e - n)) & 255) * plan.span + row.head - h0]) - off, LOG2E, -less));
                     else
                         p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], c, -off));
                     y[e] = p * (y[e] - delta);
@@ -245,10 +268,27 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
                 for (int n = 0; n < N; n += 4) {
                     const uint32_t to = bucket[n / 4] & 255;
                     if (__all(bucket[n / 4] == to * 0x01010101u)) {
-                        mine[to * THREADS] += (y[n] + y[n + 1]) + (y[n + 2] + y[n + 3]);
+                        mine[to * THREADS] += unscaled<T>((y[n] + y[n + 1]) + (y[n + 2] + y[n + 3]), factor);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) mine[(bucket[n / 4] >> (8 * e) & 255) * THREADS] += y[n + e];
+                        for (int e = 0; e < 4; ++e) mine[(bucket[n / 4] >> (8 * e) & 255) * THREADS] += unscaled<T>(y[n + e], factor);
+                    }
+                }
+            }
+            if (T::NARROW) {
+                float big = largest<N>(y);
+                if (__builtin_expect(__any(big > FACTOR_TOP) != 0, 0)) {
+                    big = row_max<F::PARTS>(big);
+                    const int down = big > FACTOR_TOP ? factor_for(big) : 0;
+                    const float f = times(1.0f, down);
+#pragma unroll
+                    for (int t = 0; t < DP / ROWS; ++t) o[t] *= f;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) y[e] *= f;
+                    factor += down;
+                    if (more) {   // again, so that their registers are free here (else 24 more are spilled)
+                        kp.load(kr, jn, vend);
+                        vp.load(vr, jn, vend);
                     }
                 }
             }
@@ -279,13 +319,14 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
             __syncthreads();
         }
         const int r0 = lane % ROWS;
+        const float back = T::NARROW ? times(1.0f, -factor) : 1.0f;
 #pragma unroll
         for (int t = 0; t < DP / ROWS; ++t)
 #pragma unroll
             for (int n = 0; n < (int)(sizeof(typename F::Acc) / 4); n += 4) {
                 f32x4 z;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) z[e] = o[t][n + e];
+                for (int e = 0; e < 4; ++e) z[e] = T::NARROW ? o[t][n + e] * back : o[t][n + e];
                 *reinterpret_cast<f32x4 *>(sums + (wave * ROWS + r0) * (DP + 4) + ROWS * t + row.key(n) + 4 * row.part) = z;
             }
         __syncthreads();
@@ -498,6 +539,7 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
     f32x4 ak[DT], av[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t) ak[t] = av[t] = f32x4{};
+    int factor = FACTOR_START;   // of this lane's key: its dS and its sum of them
     s16x8 qn[LD], dn[LD];
     float fn[FIGURES];
     auto fetch = [&](int r0) {
@@ -576,6 +618,25 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
                 ds[4 * m + e] = on ? y * (dp[e] - delta[e]) : 0.0f;
             }
         }
+        if (T::NARROW) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ds[e] = times(ds[e], factor);
+            float big = largest<8>(ds);
+            if (__any(big > FACTOR_TOP)) {
+                big = row_max<4>(big);
+                const int down = big > FACTOR_TOP ? factor_for(big) : 0;
+                const float f = times(1.0f, down);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ds[e] *= f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float c = __shfl(f, 4 * quad + e);
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) ak[t][e] *= c;
+                }
+                factor += down;
+            }
+        }
         const s16x8 pf = Mma<T>::pack(p), sf = Mma<T>::pack(ds);
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
@@ -584,6 +645,13 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
             ak[t] = Mma<T>::run(sf, tile.transposed(qt, t), ak[t]);
         }
     }
+    if (T::NARROW)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float back = times(1.0f, -__shfl(factor, 4 * quad + e));
+#pragma unroll
+            for (int t = 0; t < DT; ++t) ak[t][e] *= back;
+        }
     if (tid == 0) scratch[0] = 0;
     __syncthreads();
     const bool alone = items == 1;

@@ -43,6 +43,7 @@ struct AttnShape {
 };
 
 struct Bf16 {
+    static constexpr bool NARROW = false;   // 8 bits of exponent, as fp32
     static __device__ float up(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
     static __device__ uint16_t down(float f) {
         __hip_bfloat16 h = __float2bfloat16(f);
@@ -50,6 +51,7 @@ struct Bf16 {
     }
 };
 struct Fp16 {
+    static constexpr bool NARROW = true;    // 5 bits of exponent
     static __device__ float up(uint16_t x) { return __half2float(*reinterpret_cast<__half *>(&x)); }
     static __device__ uint16_t down(float f) {
         __half h = __float2half(f);

@@ -62,3 +62,66 @@ def test_gradients_of_rows_of_the_lowest_bias(A, dtype, sq, hq, hkv, d):
         check(A, c, s, scale=-0.3)
         s["table"][:] = low
         check(A, c, s)
+
+
+# ------------------------------------------------------------------ fp16
+def two_keys(value, dout, key):
+    """Head 8, two keys of equal score: dS = +-8 value dout / 2, dq = dS key 2 / sqrt(8)."""
+    t = lambda x: torch.tensor(x, device="cuda").to(torch.float16)  # noqa: E731
+    sign = torch.tensor([1.0, -1.0], device="cuda")[None, :, None, None].expand(1, 2, 1, 8)
+    return dict(q=t([0.0]).expand(1, 1, 1, 8).contiguous(), k=(sign * key).to(torch.float16), v=(sign * value).to(torch.float16),
+                dout=t([dout]).expand(1, 1, 1, 8).contiguous(), q_lens=None, k_lens=None, table=None, edges=None,
+                blocks=torch.zeros(1, 1, 1, 1, dtype=torch.int32, device="cuda"))
+
+
+@gpu
+@pytest.mark.parametrize("nb", [0, 3])
+def test_score_gradients_beyond_fp16(A, nb):
+    """dS = 160000, dq = 1131: an ordinary number from one that the type does not hold."""
+    c = case("fp16", sq=1, sk=2, hq=1, hkv=1, d=8, keep=1, causal=False)
+    s = two_keys(200.0, 200.0, 0.01)
+    if nb:
+        s["table"] = torch.zeros(nb, 1, dtype=torch.float16, device="cuda")
+        s["edges"] = torch.tensor([-1, 0], dtype=torch.int32, device="cuda")
+        want = ref.attention(s["q"], s["k"], s["v"], s["blocks"], 64, False, 8 ** -0.5, None, None, s["table"], s["edges"], s["dout"])
+        out, lse = A.block_attention(s["q"], s["k"], s["v"], s["blocks"], **kw(c, s))
+        got = A.block_attention_grad(s["dout"], s["q"], s["k"], s["v"], out, lse, s["blocks"], **kw(c, s))
+        for name, x in zip(("dq", "dk", "dv"), got):
+            near(x, want[0][name], want[1][name], name)
+        return
+    dq = check(A, c, s)[2]
+    assert 1100 < float(dq.abs().max()) < 1160
+
+
+@gpu
+@pytest.mark.parametrize("nb", [0, 9])
+@pytest.mark.parametrize("sq,sk,hq,hkv,d", [(70, 70, 4, 2, 64), (1, 130, 6, 1, 128), (33, 200, 2, 1, 128)])
+def test_large_score_gradients_fp16(A, sq, sk, hq, hkv, d, nb):
+    """Gradients of 1000 (a scaled loss) and values of 30."""
+    c = case("fp16", sq=sq, sk=sk, hq=hq, hkv=hkv, d=d, keep=-(-sk // 64), all=True, nb=nb)
+    s = make(c, 31)
+    s["dout"] *= 1000
+    s["v"] *= 30
+    s["q"] *= 0.02
+    s["k"] *= 0.02
+    s["table"] = None if nb == 0 else s["table"] * 0.125
+    want, bound = ref.attention(s["q"], s["k"], s["v"], s["blocks"], 64, True, d ** -0.5, None, None, s["table"], s["edges"], s["dout"])
+    assert all(want[n].abs().max() < 60000 for n in ("dq", "dk", "dv"))
+    out, lse = A.block_attention(s["q"], s["k"], s["v"], s["blocks"], **kw(c, s))
+    got = A.block_attention_grad(s["dout"], s["q"], s["k"], s["v"], out, lse, s["blocks"], **kw(c, s))
+    for name, x in zip(("dq", "dk", "dv"), got):
+        near(x, want[name], bound[name], name)
+
+
+@gpu
+@pytest.mark.parametrize("sq,keys", [(1024, 4096), (1, 4096), (300, 2048)])
+def test_small_score_gradients_fp16(A, sq, keys):
+    """dS of some 2^-22, all alike, whose sums are ordinary numbers; every step of fp16 there is 2^-24."""
+    c = case("fp16", sq=sq, sk=keys, hq=1, hkv=1, d=64, keep=keys // 64, causal=False, all=True)
+    s = make(c, 32)
+    sign = torch.where(torch.arange(keys, device="cuda") % 2 == 0, 1.0, -1.0)[None, :, None, None]
+    s["k"] = (4 * sign).expand(1, keys, 1, 64).half().contiguous()
+    s["v"] = (0.25 * keys / 4096 * sign).expand(1, keys, 1, 64).half().contiguous()
+    s["q"] = (4 * (1 - 2 * (torch.arange(64, device="cuda") % 2))).expand(1, sq, 1, 64).half().contiguous()   # q.k = 0
+    s["dout"] = torch.full((1, sq, 1, 64), 1e-4, device="cuda").half()
+    check(A, c, s)

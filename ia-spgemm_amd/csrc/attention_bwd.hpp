@@ -57,6 +57,9 @@ constexpr int FACTOR_START = 80;   // exponents of the factors
 constexpr float FACTOR_TOP = 0x1p15f;
 __device__ inline float times(float x, int exponent) { return __builtin_amdgcn_ldexpf(x, exponent); }
 __device__ inline int factor_for(float big) { return 11 + 127 - (int)(__float_as_uint(big) >> 23); }   // infinite: -117
+// k_grad_kv's P is at most 1 (up to roundings) and as small as one over the keys: 2^15 times
+// it keeps its 11 bits down to 2^-29.  The exponentials' argument takes the 15.
+template <class T> constexpr float LIFT = T::NARROW ? 15.0f : 0.0f;
 template <class T> __device__ inline float unscaled(float x, int exponent) { return T::NARROW ? times(x, -exponent) : x; }
 template <int N> __device__ inline float largest(const float *y) {
     float big = 0.0f;   // NaN is passed over: it stays NaN whatever the factor
@@ -539,7 +542,7 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
     f32x4 ak[DT], av[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t) ak[t] = av[t] = f32x4{};
-    int factor = FACTOR_START;   // of this lane's key: its dS and its sum of them
+    int factor = FACTOR_START - (int)LIFT<T>;   // of this lane's key: its dS and its sum of them
     s16x8 qn[LD], dn[LD];
     float fn[FIGURES];
     auto fetch = [&](int r0) {
@@ -560,10 +563,10 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
             const int64_t at = ((int64_t)b * s.q_heads + (int64_t)g * s.group + rr - rq * s.group) * s.q_len + i;
             if (BIAS) {
                 fn[0] = on ? plan.shift[at] : INFINITY;
-                fn[5] = plan.corr[at];
+                fn[5] = plan.corr[at] - LIFT<T>;
             } else {
                 const float l = on ? lse[at] : -INFINITY;
-                fn[0] = l == -INFINITY ? INFINITY : l * LOG2E;
+                fn[0] = l == -INFINITY ? INFINITY : l * LOG2E - LIFT<T>;
             }
             fn[1] = plan.delta[at];
             fn[2] = __int_as_float(!on ? 0 : s.causal ? min(kl, p + 1) : kl);
@@ -648,9 +651,12 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
     if (T::NARROW)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float back = times(1.0f, -__shfl(factor, 4 * quad + e));
+            const float back = times(1.0f, -__shfl(factor, 4 * quad + e) - (int)LIFT<T>);
 #pragma unroll
-            for (int t = 0; t < DT; ++t) ak[t][e] *= back;
+            for (int t = 0; t < DT; ++t) {
+                ak[t][e] *= back;
+                av[t][e] = times(av[t][e], -(int)LIFT<T>);
+            }
         }
     if (tid == 0) scratch[0] = 0;
     __syncthreads();

@@ -125,3 +125,17 @@ def test_small_score_gradients_fp16(A, sq, keys):
     s["q"] = (4 * (1 - 2 * (torch.arange(64, device="cuda") % 2))).expand(1, sq, 1, 64).half().contiguous()   # q.k = 0
     s["dout"] = torch.full((1, sq, 1, 64), 1e-4, device="cuda").half()
     check(A, c, s)
+
+
+@gpu
+@pytest.mark.parametrize("nb", [0, 4])
+def test_probabilities_of_many_keys_in_the_gradient_fp16(A, nb):
+    """200,000 keys: probabilities of 2^-17.6, below what fp16 holds to its 11 bits."""
+    c = case("fp16", sq=2, sk=200_000, hq=2, hkv=1, d=64, block=1024, keep=196, causal=False, all=True, nb=nb)
+    s = make(c, 33)
+    s["q"] *= 0.05
+    s["dout"] *= 200
+    if nb:
+        s["table"] = s["table"] * 0.1
+        s["edges"] = torch.tensor([-150_000, -77_777, -5], dtype=torch.int32, device="cuda")
+    check(A, c, s)

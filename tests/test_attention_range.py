@@ -139,3 +139,23 @@ def test_probabilities_of_many_keys_in_the_gradient_fp16(A, nb):
         s["table"] = s["table"] * 0.1
         s["edges"] = torch.tensor([-150_000, -77_777, -5], dtype=torch.int32, device="cuda")
     check(A, c, s)
+
+
+# ------------------------------------------------------------------ long walks
+@gpu
+@pytest.mark.parametrize("nb", [0, 2])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_log_sums_of_long_walks(A, dtype, nb):
+    """One key e^16.5 times as likely as each of 2^17 others of its wave: singly they vanish beside it in fp32."""
+    n, sq, d = 1 << 18, 16384, 64
+    q = torch.full((1, sq, 1, d), 0.5, device="cuda").to(DT[dtype])
+    k, v = torch.zeros(1, n, 1, d, device="cuda").to(DT[dtype]), torch.ones(1, n, 1, d, device="cuda").to(DT[dtype])
+    for first in (0, 32):          # pieces of 32 keys go to two waves in turn
+        k[0, first] = 4.21875      # a score of 16.875, exact in both types
+    blocks = torch.arange(256, device="cuda", dtype=torch.int32).expand(1, 1, sq, 256).contiguous()
+    table = torch.zeros(nb, 1, device="cuda").to(DT[dtype]) if nb else None
+    edges = torch.tensor([0], dtype=torch.int32, device="cuda") if nb else None
+    lse = A.block_attention(q, k, v, blocks, block=1024, causal=False, table=table, edges=edges)[1]
+    score = (q[0, 0, 0].double() @ k[0, :, 0].double().t()) * 0.125
+    # 4096 pieces a wave, each sum rounded by at most 2^-24 of what it has by then
+    assert (lse.double() - torch.logsumexp(score, 0)).abs().max() <= 4096 * 2.0 ** -24 + ref.C / 8

@@ -69,6 +69,14 @@ template <> struct Mma<Fp16> {
     }
 };
 
+// k_attend's probabilities are relative to a maximum that is moved only where exponentials
+// would pass 2^SLACK.  fp16 has 11 bits down to 2^-14 only, and 2^18 keys of 2^-24 each are
+// worth 1.5 % of one of 1: they are rounded at 2^11 times their size, 2^15 at most, which
+// holds 11 bits down to 2^-25.  The exponentials' argument takes the 11.
+template <class T> constexpr float SLACK = T::NARROW ? 4.0f : 8.0f;
+template <class T> constexpr float RAISE = T::NARROW ? 11.0f : 0.0f;
+template <class T> constexpr float LOWER = T::NARROW ? 0x1p-11f : 1.0f;
+
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 __device__ inline s16x8 load8(const uint16_t *p) { return *reinterpret_cast<const s16x8 *>(p); }
@@ -481,8 +489,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan,
             if (!BIAS) big *= c;
             big = sel ? big : -INFINITY;
             // the maximum is moved only where it grew by so much that exponentials would
-            // get large (2^8): that is the first piece and hardly ever another
-            if (__any(big > top + 8.0f / unit)) {
+            // get large: that is the first piece and hardly ever another
+            if (__any(big > top + SLACK<T> / unit)) {
                 const float now = fmaxf(top, big);
                 const float f = __builtin_amdgcn_exp2f((top - (now == -INFINITY ? 0.0f : now)) * unit);
                 sum *= f;
@@ -491,10 +499,10 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan,
                 top = now;
             }
             // a row that did not choose the block: exp(x - inf) = 0
-            const float shift = sel ? (top == -INFINITY ? 0.0f : top) : INFINITY;
+            const float shift = !sel ? INFINITY : (top == -INFINITY ? 0.0f : top) - (BIAS ? 0.0f : RAISE<T>);
 #pragma unroll
             for (int e = 0; e < N; ++e)
-                y[e] = __builtin_amdgcn_exp2f(BIAS ? (y[e] - shift) * LOG2E : __builtin_fmaf(y[e], c, -shift));
+                y[e] = __builtin_amdgcn_exp2f(BIAS ? __builtin_fmaf(y[e] - shift, LOG2E, RAISE<T>) : __builtin_fmaf(y[e], c, -shift));
             // the piece's sum first: beside the first key's 1 single terms of 2^-25 would be lost, 2^16 of them 0.2 %
             float few[N / 4];
 #pragma unroll
@@ -512,7 +520,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan,
         }
         // the waves meet
         const int r0 = lane % ROWS;
-        sum = row_sum<F::PARTS>(sum);
+        sum = row_sum<F::PARTS>(sum) * LOWER<T>;
         if (row.part == 0) {
             stat[(wave * ROWS + r0) * 2] = top;
             stat[(wave * ROWS + r0) * 2 + 1] = sum;
@@ -522,7 +530,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend(AttnShape s, RowPlan plan,
         {
             float all = -INFINITY;
             for (int n = 0; n < W; ++n) all = fmaxf(all, stat[(n * ROWS + r0) * 2]);
-            const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((top - all) * unit);
+            const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((top - all) * unit) * LOWER<T>;
             const bool none = top == -INFINITY && sum == sum;   // a wave that read nothing for a row adds nothing
 #pragma unroll
             for (int t = 0; t < DP / ROWS; ++t)

@@ -159,3 +159,30 @@ def test_log_sums_of_long_walks(A, dtype, nb):
     score = (q[0, 0, 0].double() @ k[0, :, 0].double().t()) * 0.125
     # 4096 pieces a wave, each sum rounded by at most 2^-24 of what it has by then
     assert (lse.double() - torch.logsumexp(score, 0)).abs().max() <= 4096 * 2.0 ** -24 + ref.C / 8
+
+
+@gpu
+@pytest.mark.parametrize("nb", [0, 2])
+def test_small_probabilities_beside_a_large_one_fp16(A, nb):
+    """One key e^16.8 times as likely as each of 2^18 others, which make 1 % of the result together."""
+    n, sq, d, x = 1 << 18, 16384, 64, 16.8
+    c = case("fp16", sq=sq, sk=n, hq=1, hkv=1, d=d, block=1024, keep=256, causal=False, all=True, nb=nb)
+    q = torch.full((1, sq, 1, d), 0.5, device="cuda").half()
+    k, v = torch.zeros(1, n, 1, d, device="cuda").half(), torch.ones(1, n, 1, d, device="cuda").half()
+    k[0, ::131072] = x * 0.25       # 0.125 * 64 * 0.5 * 4.2 = 16.8; the first key of each of two waves
+    k[0, 32::131072] = x * 0.25
+    v[0, ::131072] = 0
+    v[0, 32::131072] = 0
+    blocks = torch.arange(256, device="cuda", dtype=torch.int32).expand(1, 1, sq, 256).contiguous()
+    table = edges = None
+    if nb:
+        table = torch.zeros(nb, 1, dtype=torch.float16, device="cuda")
+        edges = torch.tensor([0], dtype=torch.int32, device="cuda")
+    out, lse = A.block_attention(q, k, v, blocks, block=1024, causal=False, table=table, edges=edges)
+    score = (q[0, 0, 0].double() @ k[0, :, 0].double().t()) * 0.125
+    p = torch.softmax(score, 0)
+    want = float(p @ v[0, :, 0, 0].double())
+    assert 0.002 < want < 0.1
+    # half a step of the result, and of each probability; fp32 elsewhere
+    assert (out.double() - want).abs().max() <= (2.0 ** -11 * 2 + ref.C) * want
+    assert (lse.double() - torch.logsumexp(score, 0)).abs().max() <= ref.C / 8 * 18

@@ -12,7 +12,10 @@ allocator on that stream, so the calls can be captured into a graph.
     out, lse = block_attention(q, k, v, blocks)
     dq, dk, dv, _ = block_attention_grad(dout, q, k, v, out, lse, blocks)
 
-There is no autograd function here: the gradient is a call of its own.
+There is no autograd function here: the gradient is a call of its own.  A call whose
+tensors require a gradient is refused where torch records (its results would be without
+one and nobody would notice): call it under torch.no_grad(), in an autograd function of
+yours, or on detached tensors.  block_select takes any, since a pattern has no gradient.
 """
 from __future__ import annotations
 
@@ -24,6 +27,20 @@ import torch
 from . import Attention, Heads, check, lib
 
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _no_graph(**tensors: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled():
+        for name, t in tensors.items():
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{name} requires a gradient, and this call records none: use torch.no_grad() and the "
+                                 "gradient's own call")
+
+
+def _written(t: torch.Tensor) -> None:
+    """Tells torch of a write through an address."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
 
 
 def _device(t: torch.Tensor) -> int:
@@ -89,12 +106,16 @@ def block_summary(k: torch.Tensor, *, block: int = 64, k_lens: Optional[torch.Te
     b, n, h, d = k.shape
     if fresh and out is None:
         raise ValueError("fresh brings an existing summary up to date: pass it as out")
+    _no_graph(k=k, out=out)
     a = _attention(k, b, 0, n, h, h, d, block, 1, True, None, None, k_lens)
     shape = (b, h, -(-n // block) if block > 0 else 0, d)
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(shape, dtype=k.dtype, device=k.device)
     check(lib.ias_block_summary(C.byref(a), C.byref(_heads(k, k.shape, k.dtype, k.device, "k")), fresh,
                                 _plain(out, shape, k.dtype, k.device, "out")), "ias_block_summary")
+    if given:
+        _written(out)
     return out
 
 
@@ -107,7 +128,8 @@ def block_select(q: torch.Tensor, summary: torch.Tensor, keep: int, *, k_len: in
     b, n, hq, d = q.shape
     a = _attention(q, b, n, k_len, hq, summary.shape[1], d, block, keep, causal, None, q_lens, k_lens)
     m = -(-k_len // block) if block > 0 else 0
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((b, summary.shape[1], n, max(keep, 0)), dtype=torch.int32, device=q.device)
         a.clear = 1
     check(lib.ias_block_select(C.byref(a), C.byref(_heads(q, q.shape, q.dtype, q.device, "q")),
@@ -115,6 +137,8 @@ def block_select(q: torch.Tensor, summary: torch.Tensor, keep: int, *, k_len: in
                                local if causal else 0,
                                _plain(out, (b, summary.shape[1], n, keep), torch.int32, q.device, "out")),
           "ias_block_select")
+    if given:
+        _written(out)
     return out
 
 
@@ -144,6 +168,7 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, blocks: t
     """(out, lse): softmax(scale q k^T + bias) v over the pattern, and the
     logarithm of each row's sum, (batch, q_heads, q_len) in fp32.  Rows behind
     q_lens are 0 / -inf in new tensors and left alone in a given `out`."""
+    _no_graph(q=q, k=k, v=v, table=table, out=out)
     a, qs, ks, pb = _shapes(q, k, blocks, block, causal, scale, q_lens, k_lens, table, edges)
     dtype, device = q.dtype, q.device
     if out is None:
@@ -159,6 +184,8 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, blocks: t
     check(lib.ias_block_attention(pa, C.byref(_heads(q, qs, dtype, device, "q")), C.byref(_heads(k, ks, dtype, device, "k")),
                                   C.byref(_heads(v, ks, dtype, device, "v")), pb, C.byref(ho), lse.data_ptr(), _address(ws), n),
           "ias_block_attention")
+    if not a.clear:
+        _written(out)
     return out, lse
 
 
@@ -169,6 +196,7 @@ def block_attention_grad(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v
                          edges: Optional[torch.Tensor] = None):
     """(dq, dk, dv, dtable) from the forward call's arguments and results;
     dtable is None without a table."""
+    _no_graph(dout=dout, q=q, k=k, v=v, out=out, lse=lse, table=table)
     a, qs, ks, pb = _shapes(q, k, blocks, block, causal, scale, q_lens, k_lens, table, edges)
     dtype, device = q.dtype, q.device
     (dq, hq), (dk, hk), (dv, hv) = _new(qs, dtype, device), _new(ks, dtype, device), _new(ks, dtype, device)
@@ -188,6 +216,7 @@ def block_attention_grad(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v
 def rel_bias(table: torch.Tensor, edges: torch.Tensor, q_len: int, k_len: int) -> torch.Tensor:
     """(heads, q_len, k_len): table[bucket(j - i - (k_len - q_len)), h], where
     bucket(d) is how many of the ascending `edges` are <= d."""
+    _no_graph(table=table)
     device = _device(table)
     if table.dtype not in _DTYPE:
         raise ValueError(f"{table.dtype} is not supported")
@@ -202,6 +231,7 @@ def rel_bias(table: torch.Tensor, edges: torch.Tensor, q_len: int, k_len: int) -
 def rel_bias_grad(grad: torch.Tensor, edges: torch.Tensor) -> torch.Tensor:
     """(buckets, heads) of grad's type: the sum of grad (batch, heads, q_len,
     k_len) over each bucket of each head."""
+    _no_graph(grad=grad)
     device = _device(grad)
     if grad.dtype not in _DTYPE or grad.dim() != 4:
         raise ValueError(f"grad: {grad.dtype} {tuple(grad.shape)} is not supported")

@@ -186,3 +186,54 @@ def test_small_probabilities_beside_a_large_one_fp16(A, nb):
     # half a step of the result, and of each probability; fp32 elsewhere
     assert (out.double() - want).abs().max() <= (2.0 ** -11 * 2 + ref.C) * want
     assert (lse.double() - torch.logsumexp(score, 0)).abs().max() <= ref.C / 8 * 18
+
+
+# ------------------------------------------------------------------ torch's graph
+@pytest.mark.parametrize("name", ["q", "k", "v", "table", "dout", "out", "lse"])
+def test_tensors_that_require_gradients_are_refused(name):
+    """Results without a graph would lose a gradient in silence; refused before anything else is looked at."""
+    from ias import attention
+    t = {n: torch.zeros(1, 4, 2, 64, dtype=torch.bfloat16) for n in ("q", "k", "v", "dout", "out")}
+    t.update(table=torch.zeros(3, 2, dtype=torch.bfloat16), lse=torch.zeros(1, 2, 4))
+    edges, blocks = torch.zeros(2, dtype=torch.int32), torch.zeros(1, 2, 4, 1, dtype=torch.int32)
+    t[name].requires_grad_()
+    forward = lambda: attention.block_attention(t["q"], t["k"], t["v"], blocks, table=t["table"], edges=edges, out=t["out"])  # noqa: E731
+    grad = lambda: attention.block_attention_grad(  # noqa: E731
+        t["dout"], t["q"], t["k"], t["v"], t["out"], t["lse"], blocks, table=t["table"], edges=edges)
+    calls = [grad] + ([forward] if name not in ("dout", "lse") else [])
+    calls += {"k": [lambda: attention.block_summary(t["k"])], "table": [lambda: attention.rel_bias(t["table"], edges, 4, 4)],
+              "dout": [lambda: attention.rel_bias_grad(t["dout"], edges)]}.get(name, [])
+    for call in calls:
+        with pytest.raises(ValueError, match=f"{name if call is not calls[-1] or name != 'dout' else 'grad'} requires a gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="HIP device"):    # goes on to the next check
+            call()
+
+
+@gpu
+def test_leaves_without_recording_and_given_outputs(A):
+    """Under no_grad leaves are taken; a given output counts as written."""
+    c = case(b=1, sq=70, sk=130, hq=4, hkv=2, d=64, keep=2)
+    s = make(c, 36)
+    plain = A.block_attention(s["q"], s["k"], s["v"], s["blocks"], **kw(c, s))
+    for n in ("q", "k", "v"):
+        s[n] = s[n].clone().requires_grad_()
+    with torch.no_grad():
+        assert all(torch.equal(x, y) for x, y in zip(plain, A.block_attention(s["q"], s["k"], s["v"], s["blocks"], **kw(c, s))))
+        m = A.block_summary(s["k"])
+        out, blocks = torch.empty_like(s["q"]), torch.empty_like(s["blocks"])
+        before = [x._version for x in (out, blocks, m)]
+        A.block_summary(s["k"], fresh=1, out=m)
+        A.block_select(s["q"], m, 2, k_len=130, out=blocks)
+        A.block_attention(s["q"], s["k"], s["v"], s["blocks"], out=out, **kw(c, s))
+        assert all(x._version > v for x, v in zip((out, blocks, m), before))
+    assert A.block_select(s["q"], m, 2, k_len=130).shape == blocks.shape
+    with torch.inference_mode():
+        out = torch.empty_like(s["q"])
+        A.block_attention(s["q"], s["k"], s["v"], s["blocks"], out=out, **kw(c, s))
+    x = torch.ones_like(plain[0], requires_grad=True)
+    held = torch.zeros_like(plain[0])
+    y = (x * held).sum()
+    A.block_attention(s["q"].detach(), s["k"].detach(), s["v"].detach(), s["blocks"], out=held, **kw(c, s))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()

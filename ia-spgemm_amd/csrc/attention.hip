@@ -237,11 +237,16 @@ ias_status check_workspace(const void *p, int64_t have, int64_t need) {
     return IAS_SUCCESS;
 }
 
-// A launch with `lds` bytes of dynamic LDS; more than 64 KB are asked for once a device.
 // A launch holds fewer than 2^32 threads.
+ias_status check_grid(int64_t grid, int threads) {
+    if (grid > (int64_t)UINT32_MAX / threads) REFUSE(IAS_ERROR_OVERFLOW, "%lld workgroups of %d threads in a launch", (long long)grid, threads);
+    return IAS_SUCCESS;
+}
+
+// A launch with `lds` bytes of dynamic LDS; more than 64 KB are asked for once a device.
 template <auto kernel, class... P>
 ias_status launch(int device, int64_t grid, int threads, size_t lds, void *stream, P... args) {
-    if (grid > (int64_t)UINT32_MAX / threads) REFUSE(IAS_ERROR_OVERFLOW, "%lld workgroups of %d threads in a launch", (long long)grid, threads);
+    IAS_TRY(check_grid(grid, threads));
     static std::atomic<bool> asked[64];
     if (lds > 64 * 1024 && !(device < 64 && asked[device].load(std::memory_order_relaxed))) {
         HIPC(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
@@ -254,6 +259,27 @@ ias_status launch(int device, int64_t grid, int threads, size_t lds, void *strea
 // Workgroups for tile_of: 8 dies, each with its share of a head's tiles or of all.
 int64_t tile_grid(int64_t heads, int64_t each) {
     return 8 * (heads < 8 && 8 % heads == 0 ? ceil_div(each, 8 / heads) : ceil_div(heads * each, 8));
+}
+
+// Grids of the calls with more than one launch, which are all looked at before the first.
+int64_t attend_grid(const ias_attention *a, const Rows &r) { return tile_grid(a->batch * a->k_heads, (int64_t)r.plan.tiles * r.plan.splits); }
+int64_t join_grid(const Rows &r) { return r.plan.splits > 1 ? r.tiles * r.plan.nq * r.plan.span : 0; }
+int64_t invert_grid(const ias_attention *a, const Backward &w) { return a->batch * a->k_heads * w.k.nw; }
+int64_t grad_kv_grid(const Backward &w) { return ceil_div(w.items * w.k.subs, 8) * 8; }
+int64_t grad_kv_join_grid(const ias_attention *a, const Backward &w, bool table) {
+    return w.k.entries * w.k.subs * 4 + (table ? (int64_t)a->q_heads * a->num_buckets : 0);
+}
+int grad_q_waves(const Rows &r) { return r.rows == 16 ? 4 : r.waves; }
+
+ias_status check_grids(const ias_attention *a, const Forward &f) {
+    IAS_TRY(check_grid(attend_grid(a, f.rows), 64 * f.rows.waves));
+    return check_grid(join_grid(f.rows), 64);
+}
+ias_status check_grids(const ias_attention *a, const Backward &w, bool table) {
+    IAS_TRY(check_grid(tile_grid(a->batch * a->k_heads, w.q.tiles), 64 * grad_q_waves(w.rows)));
+    IAS_TRY(check_grid(invert_grid(a, w), 256));
+    IAS_TRY(check_grid(grad_kv_grid(w), 256));
+    return check_grid(grad_kv_join_grid(a, w, table), 256);
 }
 
 template <class T, int DP, int MT>
@@ -289,14 +315,14 @@ ias_status select(const ias_attention *a, const ias_heads *q, const void *summar
 template <class T, int DP, int ROWS, int W>
 ias_status attend_waves(const ias_attention *a, const dev::AttnShape &s, const ias_heads *q, const ias_heads *k,
                        const ias_heads *v, const int32_t *blocks, const ias_heads *out, float *lse, const Rows &r) {
-    const int64_t grid = tile_grid(a->batch * a->k_heads, (int64_t)r.plan.tiles * r.plan.splits);
+    const int64_t grid = attend_grid(a, r);
     const size_t lds = dev::attend_lds(DP, ROWS, W, s.nblocks, r.plan.most, s.num_buckets * (r.plan.span + 1));
     if (a->table)
         IAS_TRY((launch<dev::k_attend<T, DP, ROWS, W, true>>(a->device, grid, 64 * W, lds, a->stream, s, r.plan, side(q), side(k), side(v), blocks, side_out(out), lse)));
     else
         IAS_TRY((launch<dev::k_attend<T, DP, ROWS, W, false>>(a->device, grid, 64 * W, lds, a->stream, s, r.plan, side(q), side(k), side(v), blocks, side_out(out), lse)));
     if (r.plan.splits > 1)
-        IAS_TRY((launch<dev::k_attend_join<T>>(a->device, r.tiles * r.plan.nq * r.plan.span, 64, 0, a->stream, s, r.plan, DP, ROWS,
+        IAS_TRY((launch<dev::k_attend_join<T>>(a->device, join_grid(r), 64, 0, a->stream, s, r.plan, DP, ROWS,
                        a->table ? dev::LOG2E : 1.0f, side_out(out), lse)));
     return IAS_SUCCESS;
 }
@@ -363,18 +389,17 @@ ias_status grad_all(const ias_attention *a, const ias_heads *dout, const ias_hea
     if (w.k.entries > 0) {
         if (!a->table) IAS_TRY((launch<dev::k_clear>(a->device, ceil_div(w.k.entries, 256), 256, 0, a->stream, w.k.entries, w.count)));
         if (a->q_len > 0)
-            IAS_TRY((launch<dev::k_invert>(a->device, bh * w.k.nw, 256, 4 * (size_t)s.nblocks, a->stream, s, w.k.nw, blocks, w.bits, w.count)));
+            IAS_TRY((launch<dev::k_invert>(a->device, invert_grid(a, w), 256, 4 * (size_t)s.nblocks, a->stream, s, w.k.nw, blocks, w.bits, w.count)));
         IAS_TRY((launch<dev::k_items>(a->device, 1, 1024, 0, a->stream, w.k.entries, w.k.per, w.count, w.first, w.slot)));
         const size_t lds = 4 * 32 * (size_t)DP * 2 + 2 * dev::FIGURES * 32 * 4 + 4 * (size_t)w.k.per + 32 + 4 * (size_t)s.group * s.num_buckets;
-        const int64_t grid = ceil_div(w.items * w.k.subs, 8) * 8;
+        const int64_t grid = grad_kv_grid(w);
         if (a->q_len > 0) {
             if (a->table)
                 IAS_TRY((launch<dev::k_grad_kv<T, DP, true>>(a->device, grid, 256, lds, a->stream, s, w.k, side(dout), side(q), side(k), side(v), lse, side_out(dk), side_out(dv))));
             else
                 IAS_TRY((launch<dev::k_grad_kv<T, DP, false>>(a->device, grid, 256, lds, a->stream, s, w.k, side(dout), side(q), side(k), side(v), lse, side_out(dk), side_out(dv))));
         }
-        const int64_t table = dtable ? (int64_t)a->q_heads * a->num_buckets : 0;
-        IAS_TRY((launch<dev::k_grad_kv_join<T>>(a->device, w.k.entries * w.k.subs * 4 + table, 256, 0, a->stream, s, w.k, DP, side_out(dk), side_out(dv), p,
+        IAS_TRY((launch<dev::k_grad_kv_join<T>>(a->device, grad_kv_join_grid(a, w, dtable), 256, 0, a->stream, s, w.k, DP, side_out(dk), side_out(dv), p,
                        static_cast<uint16_t *>(dtable))));
     } else if (dtable)
         IAS_TRY((launch<dev::k_grad_table<T>>(a->device, (int64_t)a->q_heads * a->num_buckets, 256, 0, a->stream, s, p, static_cast<uint16_t *>(dtable))));
@@ -454,6 +479,7 @@ extern "C" ias_status ias_block_attention(const ias_attention *a, const ias_head
     Space w;
     w.base = static_cast<char *>(workspace);
     const Forward f(a, w);
+    IAS_TRY(check_grids(a, f));
     OnDevice on;
     HIPC(on.to(a->device));
     return a->dtype == IAS_DTYPE_BF16 ? attend<dev::Bf16>(a, q, k, v, blocks, out, lse, f)
@@ -482,6 +508,7 @@ extern "C" ias_status ias_block_attention_grad(const ias_attention *a, const ias
     Space w;
     w.base = static_cast<char *>(workspace);
     const Backward f(a, w);
+    IAS_TRY(check_grids(a, f, dtable));
     OnDevice on;
     HIPC(on.to(a->device));
     return a->dtype == IAS_DTYPE_BF16 ? gradients<dev::Bf16>(a, dout, q, k, v, out, lse, blocks, dq, dk, dv, dtable, f)

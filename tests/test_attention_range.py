@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import attention_ref as ref
-from test_attention import A, DT, case, check, kw, make, near  # noqa: F401
+from test_attention import A, DT, OVERFLOW, _call, case, check, kw, make, near  # noqa: F401
 
 gpu = pytest.mark.gpu
 
@@ -237,3 +237,16 @@ def test_leaves_without_recording_and_given_outputs(A):
     A.block_attention(s["q"].detach(), s["k"].detach(), s["v"].detach(), s["blocks"], out=held, **kw(c, s))
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+# ------------------------------------------------------------------ refusals (no GPU)
+@pytest.mark.parametrize("name,change", [
+    # k_grad_q has few workgroups, the join 2^22 x 4 of 256 threads; the transpose and the items' kernel
+    ("grad", dict(batch=1 << 13, q_len=1, k_len=1 << 15, q_heads=1, k_heads=1)),
+    ("grad", dict(batch=1 << 24, q_len=1, k_len=64, q_heads=1, k_heads=1)),
+    ("grad", dict(batch=1 << 10, q_len=1, k_len=1 << 18, q_heads=1, k_heads=1, block=1024)),
+    ("attend", dict(batch=1 << 24, q_len=1, k_len=64, q_heads=1, k_heads=1)),
+])
+def test_a_call_is_refused_before_its_first_launch(name, change):
+    """Shapes of which some launch has 2^32 threads: known before any is made (here: before a device is looked for)."""
+    assert _call(name, nws=1 << 62, **change) == OVERFLOW

@@ -63,8 +63,8 @@ ias_status check_attention(const ias_attention *a, bool pattern) {
     if (a->block < 64 || a->block > 1024 || a->block % 64)
         REFUSE(IAS_ERROR_UNSUPPORTED, "block %d: a multiple of 64 up to 1024", a->block);
     if (pattern && (a->keep < 1 || a->keep > 256)) REFUSE(IAS_ERROR_UNSUPPORTED, "keep %d: 1 to 256", a->keep);
-    if (ceil_div(a->k_len, a->block) > 16384)
-        REFUSE(IAS_ERROR_UNSUPPORTED, "%lld blocks of keys: at most 16384", (long long)ceil_div(a->k_len, a->block));
+    if (a->k_len > 16384ll * a->block)   // and not by ceil_div, which passes 64 bits at the largest lengths
+        REFUSE(IAS_ERROR_UNSUPPORTED, "k_len %lld: at most 16384 blocks of %d", (long long)a->k_len, a->block);
     if (a->q_len > (1 << 24)) REFUSE(IAS_ERROR_UNSUPPORTED, "q_len %lld: at most 2^24", (long long)a->q_len);
     if (!std::isfinite(a->scale)) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "scale is not finite");
     if (a->table) {

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import attention_ref as ref
-from test_attention import A, DT, OVERFLOW, _call, case, check, kw, make, near  # noqa: F401
+from test_attention import A, DT, OVERFLOW, UNSUPPORTED, _call, case, check, kw, make, near  # noqa: F401
 
 gpu = pytest.mark.gpu
 
@@ -250,3 +250,11 @@ def test_leaves_without_recording_and_given_outputs(A):
 def test_a_call_is_refused_before_its_first_launch(name, change):
     """Shapes of which some launch has 2^32 threads: known before any is made (here: before a device is looked for)."""
     assert _call(name, nws=1 << 62, **change) == OVERFLOW
+
+
+@pytest.mark.parametrize("name", ["summary", "select", "attend", "grad"])
+@pytest.mark.parametrize("batch", [0, 1])
+def test_the_largest_length_is_refused(name, batch):
+    """The number of blocks of 2^63 - 1 keys is not one of 64-bit arithmetic."""
+    assert _call(name, batch=batch, k_len=(1 << 63) - 1) == UNSUPPORTED
+    assert _call(name, batch=batch, k_len=(1 << 63) - 40, block=1024) == UNSUPPORTED

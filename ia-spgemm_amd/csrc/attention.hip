@@ -90,6 +90,22 @@ ias_status check_heads(const ias_heads *h, const char *name, int64_t batch, int6
     return IAS_SUCCESS;
 }
 
+// An output's rows may not lie over each other (an expanded tensor's do): some order of its
+// axes has each stride at least as long as all of the axes within.
+ias_status check_apart(const ias_heads *h, const char *name, int64_t batch, int64_t n, int64_t heads, int32_t dim) {
+    if (batch == 0 || n == 0) return IAS_SUCCESS;
+    struct { int64_t size, stride; } axis[3] = {{batch, h->batch}, {n, h->token}, {heads, h->head}};
+    std::sort(axis, axis + 3, [](const auto &x, const auto &y) { return std::abs((double)x.stride) < std::abs((double)y.stride); });
+    double within = dim;   // elements from the first to the last of the axes so far
+    for (const auto &x : axis) {
+        if (x.size <= 1) continue;
+        if (std::abs((double)x.stride) < within)
+            REFUSE(IAS_ERROR_INVALID_ARGUMENT, "%s: rows of an output that lie over each other (strides %lld, %lld, %lld)", name, (long long)h->batch, (long long)h->token, (long long)h->head);
+        within += std::abs((double)x.stride) * (double)(x.size - 1);
+    }
+    return IAS_SUCCESS;
+}
+
 dev::AttnShape shape_of(const ias_attention *a) {
     dev::AttnShape s{};
     s.q_len = a->q_len; s.k_len = a->k_len;
@@ -480,6 +496,7 @@ extern "C" ias_status ias_block_attention(const ias_attention *a, const ias_head
     w.base = static_cast<char *>(workspace);
     const Forward f(a, w);
     IAS_TRY(check_grids(a, f));
+    IAS_TRY(check_apart(out, "out", a->batch, a->q_len, a->q_heads, a->head_dim));
     OnDevice on;
     HIPC(on.to(a->device));
     return a->dtype == IAS_DTYPE_BF16 ? attend<dev::Bf16>(a, q, k, v, blocks, out, lse, f)
@@ -509,6 +526,9 @@ extern "C" ias_status ias_block_attention_grad(const ias_attention *a, const ias
     w.base = static_cast<char *>(workspace);
     const Backward f(a, w);
     IAS_TRY(check_grids(a, f, dtable));
+    IAS_TRY(check_apart(dq, "dq", a->batch, a->q_len, a->q_heads, a->head_dim));
+    IAS_TRY(check_apart(dk, "dk", a->batch, a->k_len, a->k_heads, a->head_dim));
+    IAS_TRY(check_apart(dv, "dv", a->batch, a->k_len, a->k_heads, a->head_dim));
     OnDevice on;
     HIPC(on.to(a->device));
     return a->dtype == IAS_DTYPE_BF16 ? gradients<dev::Bf16>(a, dout, q, k, v, out, lse, blocks, dq, dk, dv, dtable, f)

@@ -423,7 +423,9 @@ ias_status ias_dist_csr_mul_csr(ias_dist *dist, const ias_csr *A, const ias_csr 
  * Shapes: q, out, dout, dq are batch x q_len x q_heads x head_dim, k, v, dk, dv
  * batch x k_len x k_heads x head_dim (ias_heads: strides of the first three in
  * elements, the last is contiguous; data 16-byte aligned and the strides
- * multiples of 8, of tokens at most 2^24).  Query head h reads key head
+ * multiples of 8, of tokens at most 2^24; an input may repeat rows by a stride of
+ * 0, an output's rows may not lie over each other (IAS_ERROR_INVALID_ARGUMENT),
+ * nor over anything that the call reads).  Query head h reads key head
  * h / (q_heads / k_heads).  A sequence's queries are its last tokens: with
  * q_lens / k_lens (int32 per batch element, NULL: all q_len / k_len; values are
  * clamped to [0, q_len] and [0, k_len]) query i stands at position

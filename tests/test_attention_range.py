@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import attention_ref as ref
-from test_attention import A, DT, OVERFLOW, UNSUPPORTED, _call, case, check, kw, make, near  # noqa: F401
+from test_attention import A, CAPACITY, DT, INVALID, OVERFLOW, UNSUPPORTED, _call, case, check, kw, make, near  # noqa: F401
 
 gpu = pytest.mark.gpu
 
@@ -258,3 +258,19 @@ def test_the_largest_length_is_refused(name, batch):
     """The number of blocks of 2^63 - 1 keys is not one of 64-bit arithmetic."""
     assert _call(name, batch=batch, k_len=(1 << 63) - 1) == UNSUPPORTED
     assert _call(name, batch=batch, k_len=(1 << 63) - 40, block=1024) == UNSUPPORTED
+
+
+def test_outputs_whose_rows_lie_over_each_other_are_refused():
+    """4 queries and 128 keys of 4 and 2 heads of 64: strides (batch, token, head)."""
+    import ias
+    for name, heads, n in (("out", 4, 4), ("dq", 4, 4), ("dk", 2, 128), ("dv", 2, 128)):
+        call = "attend" if name == "out" else "grad"
+        for strides in ((0, 0, 64), (heads * n * 64, heads * 64, 0), (heads * n * 64, 0, 64), (heads * n * 64, 64 * heads, 56),
+                        (heads * n * 64, 64 * heads - 8, 64), (0, 64, 64 * n - 64)):
+            assert _call(call, heads={name: ias.Heads(1 << 20, *strides)}) == INVALID, (name, strides)
+        assert _call(call, batch=2, heads={name: ias.Heads(1 << 20, 64 * heads * n - 64, 64 * heads, 64)}) == INVALID
+        # heads before tokens, wider rows, an axis of one element, and inputs that repeat rows: on to the next check
+        bias = dict(table=1 << 20, num_buckets=3, edges=1 << 20, nws=64)
+        for strides in ((0, 64, 64 * n), (heads * n * 64, 64 * heads + 8, 64), (heads * n * 64, heads * 64, 64), (0, heads * 64, 64)):
+            assert _call(call, heads={name: ias.Heads(1 << 20, *strides)}, **bias) == CAPACITY, (name, strides)
+        assert _call(call, heads={"q": ias.Heads(1 << 20, 0, 0, 0), "k": ias.Heads(1 << 20, 0, 256, 0)}, **bias) == CAPACITY

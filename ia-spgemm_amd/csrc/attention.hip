@@ -15,37 +15,6 @@
 namespace ias {
 namespace {
 
-#define HIPC(x)                                                                   \
-    do {                                                                          \
-        hipError_t _e = (x);                                                      \
-        if (_e != hipSuccess) {                                                   \
-            set_last_error("%s failed: %s", #x, hipGetErrorString(_e));           \
-            return _e == hipErrorOutOfMemory ? IAS_ERROR_OUT_OF_MEMORY : IAS_ERROR_DEVICE; \
-        }                                                                         \
-    } while (0)
-
-// Makes `device` current for the call and puts the caller's back.
-struct OnDevice {
-    int before = -1;
-    hipError_t to(int device) {
-        hipError_t e = hipGetDevice(&before);
-        if (e == hipSuccess && before != device) e = hipSetDevice(device);
-        else if (e == hipSuccess) before = -1;
-        return e;
-    }
-    ~OnDevice() {
-        if (before >= 0) (void)hipSetDevice(before);
-    }
-};
-
-#define REFUSE(status, ...)          \
-    do {                             \
-        set_last_error(__VA_ARGS__); \
-        return status;               \
-    } while (0)
-
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 ias_status check_attention(const ias_attention *a, bool pattern) {
     if (!a) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "no ias_attention");
     if (a->dtype != IAS_DTYPE_BF16 && a->dtype != IAS_DTYPE_F16)
@@ -139,11 +108,6 @@ struct Space {
 
 // every distance from a position to a key, the last block's end included
 int64_t map_size(const ias_attention *a) { return 2 * a->k_len + a->q_len + a->block + 8; }
-
-ias_status launched() {
-    HIPC(hipGetLastError());
-    return IAS_SUCCESS;
-}
 
 ias_status bucket_map(const ias_attention *a, dev::AttnShape &s, uint8_t *map, int32_t *count = nullptr, int64_t entries = 0) {
     const int64_t n = map_size(a);
@@ -250,12 +214,6 @@ ias_status check_workspace(const void *p, int64_t have, int64_t need) {
     if (!p || have < need)
         REFUSE(IAS_ERROR_INSUFFICIENT_CAPACITY, "workspace of %lld bytes: %lld are needed", (long long)(p ? have : 0), (long long)need);
     if ((uintptr_t)p & 255) REFUSE(IAS_ERROR_INVALID_ARGUMENT, "the workspace has to be aligned to 256 bytes");
-    return IAS_SUCCESS;
-}
-
-// A launch holds fewer than 2^32 threads.
-ias_status check_grid(int64_t grid, int threads) {
-    if (grid > (int64_t)UINT32_MAX / threads) REFUSE(IAS_ERROR_OVERFLOW, "%lld workgroups of %d threads in a launch", (long long)grid, threads);
     return IAS_SUCCESS;
 }
 

@@ -389,7 +389,7 @@ __global__ __launch_bounds__(256) void k_grad_table(AttnShape s, GradPlan plan, 
 // it; count[..][block]: how many.  One workgroup for 32 queries, so that a block's word
 // has one writer; integer atomics, whose order does not show.  8192 queries, 2 heads, 128
 // blocks: 6.8 us.
-__global__ __launch_bounds__(256) inline void k_invert(AttnShape s, int32_t nw, const int32_t *__restrict__ blocks,
+__global__ __launch_bounds__(256) void k_invert(AttnShape s, int32_t nw, const int32_t *__restrict__ blocks,
                                                        uint32_t *__restrict__ bits, int32_t *__restrict__ count) {
     extern __shared__ uint32_t word[];   // nblocks
     const uint32_t head = blockIdx.x / (uint32_t)nw;
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(256) inline void k_invert(AttnShape s, int32_t nw, 
 // first[e] = items of the blocks before e, an item being up to `per` queries of a block;
 // slot[e] = items before e of blocks with more than one, whose results are joined.
 // first[n], slot[n] = all.  One workgroup's scan: 5 us up to some thousand blocks.
-__global__ __launch_bounds__(1024) inline void k_items(int64_t n, int32_t per, const int32_t *__restrict__ count, int32_t *__restrict__ first,
+__global__ __launch_bounds__(1024) void k_items(int64_t n, int32_t per, const int32_t *__restrict__ count, int32_t *__restrict__ first,
                                                        int32_t *__restrict__ slot) {
     __shared__ int32_t part[2][1024];
     const int tid = threadIdx.x;
@@ -450,7 +450,7 @@ __global__ __launch_bounds__(1024) inline void k_items(int64_t n, int32_t per, c
     }
 }
 
-__global__ __launch_bounds__(256) inline void k_clear(int64_t n, int32_t *__restrict__ p) {
+__global__ __launch_bounds__(256) void k_clear(int64_t n, int32_t *__restrict__ p) {
     const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (e < n) p[e] = 0;
 }

@@ -111,6 +111,7 @@ template <int DP, int ROWS = 16> struct Tile {
     static __device__ uint32_t offset(const char *lds) {
         return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)lds;
     }
+    template <class P> static __device__ P *lds(uint32_t at) { return (P *)(uintptr_t)at; }
     uint32_t even, odd, nat, tr;
     __device__ Tile(const char *lds, int lane) {
         const uint32_t base = offset(lds);
@@ -124,18 +125,18 @@ template <int DP, int ROWS = 16> struct Tile {
     __device__ void fill(const s16x8 (&f)[N], int at) const {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            if (STEP == 8) *(lds8 *)(even + at + n * 8 * ROW) = f[n];
-            else *(lds8 *)((n % 2 ? odd : even) + at + n / 2 * 8 * ROW) = f[n];
+            if (STEP == 8) *lds<lds8>(even + at + n * 8 * ROW) = f[n];
+            else *lds<lds8>((n % 2 ? odd : even) + at + n / 2 * 8 * ROW) = f[n];
         }
     }
     // Left operand from the tile as it is: row row0 + lane % ROWS, channels K * ks + 8 * (lane / ROWS) + 0..7.
-    __device__ s16x8 natural(int at, int row0, int ks) const { return *(lds8 *)((nat ^ (ks * 2 * Form<ROWS>::K)) + at + row0 * ROW); }
+    __device__ s16x8 natural(int at, int row0, int ks) const { return *lds<lds8>((nat ^ (ks * 2 * Form<ROWS>::K)) + at + row0 * ROW); }
     // Operand from the transposed tile: channel ROWS * c + lane % ROWS, rows row0 + 4 * (lane / ROWS) + 0..3
     // and 4 PARTS further.
     __device__ s16x8 transposed(int at, int c, int row0 = 0) const {
         const uint32_t a = (tr ^ (c * 2 * ROWS)) + at + row0 * ROW;
-        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)a);
-        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(a + 4 * Form<ROWS>::PARTS * ROW));
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds<lds4>(a));
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds<lds4>(a + 4 * Form<ROWS>::PARTS * ROW));
         return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     }
 };

@@ -7,6 +7,8 @@
 
 #include <cstdint>
 
+#include "call.hpp"
+
 namespace ias {
 namespace dev {
 
@@ -105,16 +107,6 @@ __global__ __launch_bounds__(256) void k_block_summary(AttnShape s, Side k, int6
 }
 
 // ------------------------------------------------------------------ buckets
-// How many of the ascending edges are <= d.
-__device__ inline int bucket_of(int64_t d, const int32_t *edges, int num_buckets) {
-    int lo = 0, hi = num_buckets - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (edges[mid] <= d) lo = mid + 1;
-        else hi = mid;
-    }
-    return lo;
-}
 // The buckets of d .. d + 3, a byte each.
 __device__ inline uint32_t four_buckets(int d, const int32_t *edges, int num_buckets) {
     int n = bucket_of(d, edges, num_buckets);

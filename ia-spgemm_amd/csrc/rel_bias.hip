@@ -2,6 +2,7 @@
 // gradient (ias_rel_bias* of include/ias.h).  The reference has no counterpart.
 #include "ias.h"
 #include "ias_internal.hpp"
+#include "call.hpp"
 
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
@@ -13,46 +14,12 @@
 namespace ias {
 namespace {
 
-#define HIPC(x)                                                                   \
-    do {                                                                          \
-        hipError_t _e = (x);                                                      \
-        if (_e != hipSuccess) {                                                   \
-            set_last_error("%s failed: %s", #x, hipGetErrorString(_e));           \
-            return _e == hipErrorOutOfMemory ? IAS_ERROR_OUT_OF_MEMORY : IAS_ERROR_DEVICE; \
-        }                                                                         \
-    } while (0)
-
-struct OnDevice {
-    int before = -1;
-    hipError_t to(int device) {
-        hipError_t e = hipGetDevice(&before);
-        if (e == hipSuccess && before != device) e = hipSetDevice(device);
-        else if (e == hipSuccess) before = -1;
-        return e;
-    }
-    ~OnDevice() {
-        if (before >= 0) (void)hipSetDevice(before);
-    }
-};
-
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 __device__ inline float up(float x) { return x; }
 __device__ inline float up(__hip_bfloat16 x) { return __bfloat162float(x); }
 __device__ inline float up(__half x) { return __half2float(x); }
 __device__ inline void down(float x, float *o) { *o = x; }
 __device__ inline void down(float x, __hip_bfloat16 *o) { *o = __float2bfloat16(x); }
 __device__ inline void down(float x, __half *o) { *o = __float2half(x); }
-
-__device__ inline int bucket_of(int64_t d, const int32_t *edges, int nb) {
-    int lo = 0, hi = nb - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (edges[mid] <= d) lo = mid + 1;
-        else hi = mid;
-    }
-    return lo;
-}
 
 constexpr int V = 8;         // consecutive values of a thread of k_rel_bias
 constexpr int HEADS = 16;    // heads of a workgroup
@@ -80,7 +47,7 @@ __global__ __launch_bounds__(256) void k_rel_bias(int32_t heads, int64_t q_len, 
     if (e0 >= size) return;
     const int64_t i = e0 / k_len;
     int64_t j = e0 - i * k_len, d = j - i - (k_len - q_len);
-    int at[V], n = bucket_of(d, es, nb);
+    int at[V], n = dev::bucket_of(d, es, nb);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         at[v] = n * HEADS;
@@ -90,7 +57,7 @@ __global__ __launch_bounds__(256) void k_rel_bias(int32_t heads, int64_t q_len, 
         } else {   // on to the next row
             j = 0;
             d -= k_len;
-            n = bucket_of(d, es, nb);
+            n = dev::bucket_of(d, es, nb);
         }
     }
     for (int h = 0; h < hn; ++h) {
@@ -183,12 +150,6 @@ __global__ __launch_bounds__(64) void k_rel_bias_sum(int64_t chunks, int32_t hea
     if (threadIdx.x == 0) down(t, dtable + (int64_t)n * heads + h);
 }
 
-#define REFUSE(status, ...)          \
-    do {                             \
-        set_last_error(__VA_ARGS__); \
-        return status;               \
-    } while (0)
-
 ias_status check_bias(int32_t dtype, int64_t batch, int32_t heads, int64_t q_len, int64_t k_len, int32_t nb, int32_t device) {
     if (dtype < IAS_DTYPE_F32 || dtype > IAS_DTYPE_F16) REFUSE(IAS_ERROR_UNSUPPORTED, "dtype %d", dtype);
     if (batch < 0 || heads < 0 || q_len < 0 || k_len < 0 || device < 0)
@@ -214,11 +175,6 @@ struct Chunks {
         all = spans * ceil_div(q_len, rows);
     }
 };
-
-ias_status launched() {
-    HIPC(hipGetLastError());
-    return IAS_SUCCESS;
-}
 
 template <class T>
 ias_status bias(int32_t heads, int64_t q_len, int64_t k_len, int32_t nb, const void *table, const int32_t *edges,

@@ -75,6 +75,11 @@ __global__ __launch_bounds__(256) void k_rel_bias(int32_t heads, int64_t q_len, 
     }
 }
 
+// Values of a diagonal are summed by eights, and 2048 or more of them (batch elements of short
+// matrices) by themselves: 2^16 added one by one to what has grown to their sum can be off by
+// 2^-9 of it.
+constexpr int RUN = 2048;
+
 // Sums over diagonals.  A thread has 2 neighbouring diagonals and goes down some rows
 // of every batch element, its loads moving one to the right with each row: the sums
 // stay in registers, and buckets matter only at the end, where each is one stretch of
@@ -95,7 +100,8 @@ __global__ __launch_bounds__(256) void k_rel_bias_grad(int64_t batch, int32_t he
     // column of the thread's first diagonal in row i: c0 + i
     const int64_t first = chunk % spans * SPAN - (q_len - 1), c0 = first + tid * E;
     if (tid < nb - 1) es[tid] = edges[tid];
-    float acc[E] = {};
+    float all[E] = {}, acc[E] = {};
+    int64_t held = 0;   // values in acc
     // rows where both columns are there, and those beside them where one is
     const int64_t ia = max(r0, -c0), ib = min(r1, k_len - E + 1 - c0);
     for (int64_t b = 0; b < batch; ++b) {
@@ -108,9 +114,16 @@ __global__ __launch_bounds__(256) void k_rel_bias_grad(int64_t batch, int32_t he
 #pragma unroll
                 for (int u = 0; u < U; ++u) __builtin_memcpy(y[u], x + (i + u) * (sr + 1), sizeof y[u]);
 #pragma unroll
-                for (int u = 0; u < U; ++u)
+                for (int e = 0; e < E; ++e) {
+                    float z[U];
 #pragma unroll
-                    for (int e = 0; e < E; ++e) acc[e] += up(y[u][e]);
+                    for (int u = 0; u < U; ++u) z[u] = up(y[u][e]);
+#pragma unroll
+                    for (int n = 1; n < U; n *= 2)
+#pragma unroll
+                        for (int u = 0; u < U; u += 2 * n) z[u] += z[u + n];
+                    acc[e] += z[0];
+                }
             }
         };
         rows_down(std::integral_constant<int, 8>{});
@@ -123,9 +136,17 @@ __global__ __launch_bounds__(256) void k_rel_bias_grad(int64_t batch, int32_t he
                 for (int e = 0; e < E; ++e)
                     if (c0 + n + e >= 0 && c0 + n + e < k_len) acc[e] += up(x[n * (sr + 1) + e]);
         }
+        if ((held += r1 - r0) >= RUN) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                all[e] += acc[e];
+                acc[e] = 0.0f;
+            }
+            held = 0;
+        }
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) sums[tid * E + e] = acc[e];
+    for (int e = 0; e < E; ++e) sums[tid * E + e] = all[e] + acc[e];
     __syncthreads();
     // bucket n is the stretch of diagonals from edge n - 1 to edge n
     const int lane = tid % 64;

@@ -64,6 +64,22 @@ def test_gradients_of_rows_of_the_lowest_bias(A, dtype, sq, hq, hkv, d):
         check(A, c, s)
 
 
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("b,n,nk", [(4096, 16, 64), (1, 60_000, 60_000), (300, 700, 900)])
+def test_bias_gradient_of_many_terms(A, dtype, b, n, nk):
+    """A constant gradient, of stride 0: the roundings of a long sum go the same way."""
+    grad = torch.full((nk,), 0.1, device="cuda").to(DT[dtype]).expand(b, 1, n, nk)
+    edges = torch.tensor([-(n // 2), 0, 3], dtype=torch.int32, device="cuda")
+    got = A.rel_bias_grad(grad, edges).double()[:, 0]
+    i = torch.arange(n, device="cuda").double() + (nk - n)      # position of each query: keys j with j - i in a bucket
+    cut = [torch.zeros_like(i)] + [(i + e).clamp(0, nk) for e in edges.tolist()] + [torch.full_like(i, nk)]
+    want = torch.stack([(cut[t + 1] - cut[t]).sum() for t in range(4)]) * b * float(grad[0, 0, 0, 0])
+    # chains of at most 3443 / 8 sums of eight (or 2048 values singly, where rows are fewer than eight), 32 such
+    # chains, 8 + 6 of a workgroup, 66 + 6 of all: below 2^10 roundings of 2^-24 here
+    assert ((got - want).abs() <= (2.0 ** -14 + torch.finfo(DT[dtype]).eps / 2) * want).all()
+
+
 # ------------------------------------------------------------------ fp16
 def two_keys(value, dout, key):
     """Head 8, two keys of equal score: dS = +-8 value dout / 2, dq = dS key 2 / sqrt(8)."""

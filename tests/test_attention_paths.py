@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import attention_ref as ref
-from test_attention import A, DT, case, check, kw, make  # noqa: F401
+from test_attention import A, DT, case, check, kw, make, near  # noqa: F401
 
 gpu = pytest.mark.gpu
 
@@ -102,3 +102,49 @@ def test_gradients_of_other_sizes(A, c, size):
     s = make(c, 46)
     s["dout"] = (s["dout"].float() * size).to(s["dout"].dtype)
     check(A, c, s)
+
+
+@gpu
+def test_select_by_the_smallest_numbers_fp16(A):
+    """Queries or summaries below fp16's normal numbers: their bits count."""
+    gen = torch.Generator(device="cuda").manual_seed(47)
+    q = torch.randn(1, 40, 8, 64, device="cuda", generator=gen)
+    m = torch.randn(1, 2, 100, 64, device="cuda", generator=gen)
+    for a, b in ((2.0 ** -18, 1.0), (1.0, 2.0 ** -18), (2.0 ** -16, 2.0 ** -17)):
+        x, y = (q * a).half(), (m * b).half()
+        got = A.block_select(x, y, 9, k_len=6400)
+        assert torch.equal(got.cpu(), ref.select(x, y, 9, 6400, 64, True, 1, 1, None, None))
+
+
+@gpu
+@pytest.mark.parametrize("name", ["q", "k", "v", "dout"])
+def test_inputs_of_the_smallest_numbers_fp16(A, name):
+    c = case("fp16", b=2, sq=90, sk=200, hq=4, hkv=2, d=64, nb=8)
+    s = make(c, 48)
+    s[name] = (s[name].float() * 2.0 ** -17).half()
+    if name in ("q", "k"):
+        other = "k" if name == "q" else "q"
+        s[other] = (s[other].float() * 256).half()      # so that scores come of it
+        s["dout"] = (s["dout"].float() / 64).half()
+    check(A, c, s)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_one_row_sees_values_that_another_must_not(A, dtype):
+    """Largest finite values and keys in places that only some rows read: their size reaches nobody else's precision."""
+    c = case(dtype, b=1, sq=150, sk=256, hq=4, hkv=2, d=64, keep=2, nb=5)
+    s = make(c, 49)
+    s["blocks"][..., 0] = 0
+    s["blocks"][..., 1] = torch.arange(150, device="cuda") % 3
+    want, bound = ref.attention(s["q"], s["k"], s["v"], s["blocks"], 64, True, 0.125, None, None, s["table"], s["edges"], s["dout"])
+    top = torch.finfo(DT[dtype]).max
+    k, v = s["k"].clone(), s["v"].clone()
+    k[0, 140:150], v[0, 140:150] = -top, top      # block 2
+    v[0, 150:160] = -top
+    out, lse = A.block_attention(s["q"], k, v, s["blocks"], **kw(c, s))
+    dq = A.block_attention_grad(s["dout"], s["q"], k, v, out, lse, s["blocks"], **kw(c, s))[0]
+    i = torch.arange(150, device="cuda")
+    free = ~((i % 3 == 2) & (i + 106 >= 140))
+    for got, name in ((out, "out"), (dq, "dq")):
+        near(got[0, free], want[name][0, free], bound[name][0, free], name)

@@ -173,7 +173,10 @@ struct Forward {
 // 1024 items where there are few rows.  An item of a block that many queries chose
 // writes 64 KB of f32 results, so small ones cost more to join than they even out
 // (8192 tokens, 16/2 heads of 128, both kernels: 421, 382 and 415 us with 768, 1024
-// and 2048 rows).
+// and 2048 rows).  Large calls take longer items, so that all results stay within 1 GiB,
+// up to 8192 queries (their list is in LDS): there are enough of them then (4 x 8192 tokens,
+// 32/8 heads of 128, 32 blocks a query: 4096 rows, a training step 11.1 ms and a peak of 2.3
+// GiB; with 1024 rows 11.3 ms and 5.3 GiB).
 struct Backward {
     uint8_t *map;
     Rows rows;

@@ -13,10 +13,11 @@
 // (bound: 0.005) where the formula in separate fp32 operators has 0.0017.  dS in two parts brought
 // it to 0.0024, since delta's part stays, and cost 8 to 13 % of a training step.
 //
-// 8192 tokens, 16/2 heads of 128, 16 blocks a query, all 0.86 ms with the forward: k_grad_q
-// 307 us and k_grad_kv 322 us, both bound by latency at two and three waves a SIMD as the
-// forward is (it makes 5 products where the forward makes 2), k_grad_kv_join 50 us, bound
-// by its read of partial results (64 KB an item); the pattern's transpose 17 us in three
+// 8192 tokens, 16/2 heads of 128, 16 blocks a query, 0.83 to 0.85 ms with the forward's 228 us:
+// k_grad_q 282 us and k_grad_kv 271 us, both bound by latency at two and three waves a SIMD
+// as the forward is (together 7 products where the forward makes 2; matrix units busy in 28
+// and 19 % of the cycles, LDS in 44 and 28 %), k_grad_kv_join 49 us, bound
+// by its read of partial results (64 KB an item); the pattern's transpose 18 us in three
 // launches.
 #pragma once
 
@@ -472,9 +473,9 @@ constexpr int FIGURES = 6;   // of each row in k_grad_kv's LDS
 // Their results hold one key and 2 x 4 rows in a lane, as the left operands of
 // dV += P^T dO and dK += dS^T Q want them; dO and Q come from LDS both ways.
 // P and dS are rounded to the inputs' type for these products (half a step of
-// each), sums are fp32.  Three workgroups a CU need fewer than 168 registers, hence the
-// barriers that keep the compiler from reading ahead (with spills 1.29 ms, without
-// 1.16 ms for 8192 tokens' training step then).
+// each), sums are fp32.  Three workgroups a CU need at most 168 registers, hence the
+// barriers that keep the compiler from reading ahead (with 35 spilled 1.29 ms, with few
+// 1.16 ms for 8192 tokens' training step then; 2 are left for bf16 heads of 128, 6 for fp16).
 template <class T, int DP, bool BIAS>
 __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(AttnShape s, KeyPlan plan, Side dout, Side q, Side k, Side v,
                                                     const float *__restrict__ lse, SideOut dk, SideOut dv) {

@@ -20,11 +20,14 @@
 // which half a wave reads lie in 8 different groups of banks.
 //
 // Prompts are bound by the latency of a piece's chain (load, LDS, scores, exponentials,
-// product) with the two waves a SIMD that 256 registers a lane allow: 8192 tokens, 32/8 heads of 128, 16 blocks of 64 keys a query, random choices:
-// 0.53 to 0.54 ms, where a union of 8 queries has 39 blocks; matrix units are busy 22 % of
-// it, vector ALUs 40 %, LDS 35 %, the vector cache 47 %.  Single tokens are bound by the
-// read of K and V (16 users, 32 of up to 512 blocks, 8 heads of 128: 134 MB in 29.7 us,
-// 4.5 TB/s) and few of them by the launch and one chain of loads (13.6 us for one user).
+// product) with the two waves a SIMD that 256 registers a lane allow (three for heads of
+// 64): 8192 tokens, 32/8 heads of 128, 16 blocks of 64 keys a query, random choices: 0.52 to
+// 0.55 ms, where a union of 8 queries has 39 blocks.  Of the CUs' cycles the matrix units are
+// busy in 26 % (SQ_VALU_MFMA_BUSY_CYCLES), the vector ALUs in 35 % (SQ_ACTIVE_INST_VALU), LDS in
+// 48 % (SQ_LDS_IDX_ACTIVE), the vector cache in 54 % (TCP_TOTAL_CACHE_ACCESSES).  Single tokens are bound by the
+// read of K and V (16 users, 32 of up to 512 blocks, 8 heads of 128: 134 MB in 28.8 us,
+// 4.7 TB/s) and few of them by one workgroup's chain of loads for each key head (13.7 us
+// for one user).
 #pragma once
 
 #include "attention_kernels.hpp"

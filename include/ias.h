@@ -482,11 +482,17 @@ ias_status ias_block_summary(const ias_attention *a, const ias_heads *k, int64_t
  * last `local` of them (causal only), then those of the highest score, up to
  * `keep`; ascending, -1 behind.  A block's score is the largest q_h . mean of
  * the key head's query heads, compared in 64 bits (NaN as -infinity); of
- * equal scores the lower block wins.  first + local <= keep. */
+ * equal scores the lower block wins.  first + local <= keep.  The mean of the
+ * block that holds a causal query also holds the keys behind the query: with
+ * local = 0 that block competes by it, and what is chosen then depends on later
+ * tokens (local >= 1 takes the block whatever its score). */
 ias_status ias_block_select(const ias_attention *a, const ias_heads *q, const void *summary,
                             int32_t first, int32_t local, int32_t *blocks);
 /* Bytes of workspace that ias_block_attention (forward) and
- * ias_block_attention_grad (backward) take for these shapes; either may be NULL. */
+ * ias_block_attention_grad (backward) take for these shapes; either may be NULL.
+ * Backward: batch x k_heads x blocks x q_len / 8 bytes for the pattern's
+ * transpose, and partial results of up to about 1 GiB (more for patterns of
+ * some 2^26 entries and beyond). */
 ias_status ias_block_attention_workspace(const ias_attention *a, int64_t *forward, int64_t *backward);
 /* out = softmax(scale q k^T + bias) v over the pattern; lse (f32, batch x
  * q_heads x q_len, NULL: not wanted) = log of the sum of the exponentials.  A

@@ -153,7 +153,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_grad_q(AttnShape s, GradPlan plan
     if (BIAS) {
         const int64_t at = ((int64_t)b * s.q_heads + (int64_t)g * s.group + row.head) * s.q_len + i0 + row.query;
         const float l = row.there ? lse[at] : -INFINITY;
-        shift = l == -INFINITY ? INFINITY : l == INFINITY ? NAN : l;   // infinite: a score was
+        shift = l == -INFINITY ? INFINITY : l;
         // Beside a bias of the type's lowest value fp32 holds no log of a sum: at 4096 lse is off
         // by up to 2^-13, far beyond it a row of equals would get P = 1 for each.  Such rows (hardly
         // ever any) find their maximum and sum again.
@@ -700,8 +700,8 @@ __global__ __launch_bounds__(256, BIAS && DP == 128 ? 2 : 3) void k_grad_kv(Attn
         for (int r = 0; r < rows; ++r) {
             const int i = list[r / s.group], pos = i + kl - ql, hr = r % s.group;
             const int64_t h = (int64_t)g * s.group + hr, at = ((int64_t)b * s.q_heads + h) * s.q_len + i;
-            const float shift = BIAS ? plan.shift[at] : lse[at] == -INFINITY ? INFINITY : lse[at], corr = BIAS ? plan.corr[at] : 0.0f;
-            if ((s.causal && j > pos) || shift == INFINITY) continue;
+            const float l = lse[at], shift = BIAS ? plan.shift[at] : l, corr = BIAS ? plan.corr[at] : 0.0f;
+            if ((s.causal && j > pos) || l == -INFINITY) continue;
             const uint16_t *qr = q.at(b, i, h), *dr = dout.at(b, i, h);
             float x = 0.0f, dp = 0.0f;
 #pragma unroll

@@ -148,3 +148,26 @@ def test_one_row_sees_values_that_another_must_not(A, dtype):
     free = ~((i % 3 == 2) & (i + 106 >= 140))
     for got, name in ((out, "out"), (dq, "dq")):
         near(got[0, free], want[name][0, free], bound[name][0, free], name)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("nb", [0, 9])
+def test_padded_batches_without_a_mask(A, dtype, nb):
+    """Both directions, lengths of their own, more queries than keys among them."""
+    c = case(dtype, b=5, sq=77, sk=300, hq=6, hkv=2, d=72, keep=4, causal=False, nb=nb, q_lens=[77, 0, 1, 40, 77], k_lens=[300, 200, 1, 64, 0])
+    check(A, c, make(c, 50))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("low", [float("-inf"), -1e4])
+@pytest.mark.parametrize("sq,sk,hq,hkv", [(150, 200, 4, 2), (4, 700, 4, 1), (1, 5000, 2, 1)])
+def test_buckets_that_mask(A, dtype, low, sq, sk, hq, hkv):
+    """A bias of -infinity, or of -10000, keeps far keys out, and near ones for another head."""
+    c = case(dtype, sq=sq, sk=sk, hq=hq, hkv=hkv, d=64, keep=-(-sk // 64), nb=4, all=True)
+    s = make(c, 51)
+    s["edges"] = torch.tensor([-sk + 70, -90, -3], dtype=torch.int32, device="cuda")
+    s["table"][0] = low
+    s["table"][3, 1] = low
+    check(A, c, s)
